@@ -21,6 +21,7 @@
 #define CERTEX_B200_H_
 
 #include <stdbool.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -317,6 +318,101 @@ CERTEX_B200_EXPORT cuvsError_t certexB200PlanSegments(int32_t n_query_tiles, int
  *  the check); *finite = 1 when every value is finite in float16. Waits for the resources' stream. */
 CERTEX_B200_EXPORT cuvsError_t certexB200ToHalf(cuvsResources_t res, const void* src, int32_t kind, int64_t n, void* dst,
                                                 int32_t* finite);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * A paged cache of keys and values, and what a decoding step does with it. The reference selects positions
+ * (certex/attention.py:44-114, certex/flashinfer.py:50-138) and leaves the attention over them to its callers; these entry
+ * points keep keys and values in pages, turn queries and keys by their positions, append, and attend, over a whole sequence or
+ * over positions that were selected before. No counterpart in the reference.
+ *
+ * All memory is device memory of the resources' device, which must be the current one; everything is enqueued on the
+ * resources' stream, nothing is allocated, and nothing waits, so that every call may be captured in a graph. dtype is 0
+ * (float32), 1 (float16) or 2 (bfloat16), the same for cache, queries and outputs. Strides are in elements; the coordinates
+ * of a head lie next to one another. n_rows = 0 is a call that does nothing.
+ *
+ * Indices are read on the device and checked there: a row of a sequence that the table does not have, an entry of the table
+ * that is no page, a position or a length beyond the table reads and writes nothing (attention goes on without that key) and
+ * sets *fault to 1, where the caller may look.
+ */
+/** [rows, heads, dim] */
+typedef struct {
+  void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} certexB200Rows_t;
+
+/** The rotation of pairs of a head's first rotary_dim coordinates, (2i, 2i + 1) when interleaved, else (i, i + rotary_dim / 2):
+ *  turns[i] (device memory, rotary_dim / 2 of them) is what a position adds to pair i's angle, as a fraction of a turn in
+ *  units of 2^-64 (a negative angle wraps); results are multiplied by magnitude. */
+typedef struct {
+  const uint64_t* turns;
+  int64_t rotary_dim;
+  int64_t interleaved;
+  double magnitude;
+} certexB200Rotary_t;
+
+/** key_strides / value_strides: from a page, a token of a page and a head to the next. keys, values and all strides are
+ *  multiples of 16 bytes; head_dim is a multiple of 8 and at most 256. fault: one int32 of device memory. */
+typedef struct {
+  void* keys;
+  void* values;
+  int64_t key_strides[3];
+  int64_t value_strides[3];
+  int64_t n_pages;
+  int64_t page_size;
+  int64_t n_kv_heads;
+  int64_t head_dim;
+  int64_t dtype;
+  int32_t* fault;
+} certexB200PagedCache_t;
+
+/** Token t of sequence b lies at place t % page_size of page pages[b * row_stride + t / page_size]; row i of a call belongs
+ *  to sequence row_to_sequence[i] (NULL: i). */
+typedef struct {
+  const int32_t* pages;
+  int64_t row_stride;
+  int64_t n_sequences;
+  int64_t pages_per_sequence;
+  const int32_t* row_to_sequence;
+} certexB200PageTable_t;
+
+/** y = x turned by positions[row] (int32, or int64 when positions_64), or turned back when inverse, which is also the
+ *  gradient. y may be x. head_dim is even; coordinates behind rotary_dim are copied. */
+CERTEX_B200_EXPORT cuvsError_t certexB200Rotate(cuvsResources_t res, const certexB200Rotary_t* rotary, const certexB200Rows_t* x,
+                                                const certexB200Rows_t* y, int64_t n_rows, int64_t n_heads, int64_t head_dim,
+                                                int32_t dtype, const void* positions, int32_t positions_64, int32_t inverse);
+
+/** Row i of k and v (n_kv_heads heads) goes to position positions[i] of its sequence; a negative position is a row without a
+ *  token. With rotary (may be NULL) keys are turned by their positions on the way, and so are the n_q_heads heads of q, which
+ *  go to q_out (q and q_out may be NULL, with n_q_heads = 0). Rows of one call have different places. */
+CERTEX_B200_EXPORT cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCache_t* cache,
+                                                     const certexB200Rotary_t* rotary, const certexB200PageTable_t* table,
+                                                     const certexB200Rows_t* k, const certexB200Rows_t* v,
+                                                     const certexB200Rows_t* q, const certexB200Rows_t* q_out, int64_t n_rows,
+                                                     int64_t n_q_heads, const void* positions, int32_t positions_64);
+
+/** Bytes of device memory that an attention of these sizes wants as its workspace (16-byte aligned; it belongs to one call at
+ *  a time). n_lists: 0 for certexB200PagedAttend; k: its pages_per_sequence * page_size, or the length of a list. */
+CERTEX_B200_EXPORT cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedCache_t* cache, int64_t n_rows,
+                                                        int64_t n_heads, int64_t n_lists, int64_t k, size_t* bytes);
+
+/** out[i, h] = the values that row i sees, weighed by the softmax of scale * <q[i, h], key> over KV head h / (n_heads /
+ *  n_kv_heads). Row i sees the first lengths[i] tokens of its sequence, of those the last `window` if window > 0; a row that
+ *  sees none gets zeros. lse (may be NULL) [n_rows, n_heads]: the logarithm of the sum of exponentials (-inf for such a row). */
+CERTEX_B200_EXPORT cuvsError_t certexB200PagedAttend(cuvsResources_t res, const certexB200PagedCache_t* cache,
+                                                     const certexB200PageTable_t* table, const int32_t* lengths, int64_t window,
+                                                     const certexB200Rows_t* q, const certexB200Rows_t* out, int64_t n_rows,
+                                                     int64_t n_heads, float scale, float* lse, void* workspace,
+                                                     size_t workspace_bytes);
+
+/** The same over selected [n_rows, n_lists, k] positions of the cache, page * page_size + place (int32, or int64 when
+ *  selected_64), negative ones left out; one that is named twice counts twice. n_lists is n_heads (a list per query head),
+ *  n_kv_heads (per KV head) or 1 (for all heads). */
+CERTEX_B200_EXPORT cuvsError_t certexB200PagedAttendSelected(cuvsResources_t res, const certexB200PagedCache_t* cache,
+                                                             const void* selected, int32_t selected_64, int64_t n_lists,
+                                                             int64_t k, const certexB200Rows_t* q, const certexB200Rows_t* out,
+                                                             int64_t n_rows, int64_t n_heads, float scale, float* lse,
+                                                             void* workspace, size_t workspace_bytes);
 
 /** Filter words of a mask of n bytes in device memory (non-zero: keep): bit j of words[i] = entry 32 i + j, (n + 31) / 32
  *  words, bits beyond n are 0. Enqueued on the resources' stream. */

@@ -11,6 +11,8 @@ PyTorch fallback.
 from ._lib import CertexError
 from .attention import KeyCache, topk
 from .index import Index, ShardedIndex, merge_shards, search, search_stats, verify
+from .paged import PagedCache, Rotary
 
 __version__ = "0.2.0"
-__all__ = ["CertexError", "KeyCache", "topk", "Index", "ShardedIndex", "merge_shards", "search", "search_stats", "verify", "__version__"]
+__all__ = ["CertexError", "KeyCache", "topk", "Index", "ShardedIndex", "merge_shards", "search", "search_stats", "verify", "PagedCache", "Rotary",
+           "__version__"]

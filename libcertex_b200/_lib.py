@@ -117,6 +117,8 @@ SYMBOLS = [
     "certexB200DistributedSearch", "certexB200ScreenTrace", "certexB200PlanChunked",
     "certexB200DistributedSearchBegin", "certexB200DistributedSearchEnd", "certexB200OrderByLabel",
     "certexB200PackMask", "certexB200ToHalf", "certexB200LabelSample",
+    "certexB200Rotate", "certexB200PagedAppend", "certexB200PagedWorkspace", "certexB200PagedAttend",
+    "certexB200PagedAttendSelected",
 ]
 
 # void hook(void* ctx, int32_t* keys, int64_t n, cudaStream_t stream)
@@ -200,6 +202,13 @@ def lib():
                 L.certexB200DistributedSearchEnd.argtypes = [vp]
                 L.certexB200ToHalf.argtypes = [vp, vp, ctypes.c_int32, i64, vp, P(ctypes.c_int32)]
                 L.certexB200PackMask.argtypes = [vp, vp, i64, vp]
+                # structures of these cross as packed bytes
+                i32, f32, sz = ctypes.c_int32, ctypes.c_float, ctypes.c_size_t
+                L.certexB200Rotate.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, vp, i32, i32]
+                L.certexB200PagedAppend.argtypes = [vp] * 8 + [i64, i64, vp, i32]
+                L.certexB200PagedWorkspace.argtypes = [vp, vp, i64, i64, i64, i64, P(sz)]
+                L.certexB200PagedAttend.argtypes = [vp, vp, vp, vp, i64, vp, vp, i64, i64, f32, vp, vp, sz]
+                L.certexB200PagedAttendSelected.argtypes = [vp, vp, vp, i32, i64, i64, vp, vp, i64, i64, f32, vp, vp, sz]
                 L.certexB200ScreenTrace.argtypes = [vp, ctypes.c_int32]
                 L.certexB200LabelSample.argtypes = [ctypes.c_int32, i64, ctypes.c_int32, P(i64)]
                 L.certexB200OrderByLabel.argtypes = [P(ctypes.c_int32), i64, P(ctypes.c_int32)]

@@ -3,11 +3,13 @@
 #include "../../include/certex_b200.h"
 
 #include "engine.hpp"
+#include "paged.cuh"
 #include "screen_i8.cuh"
 
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <exception>
 #include <fstream>
 #include <memory>
@@ -581,6 +583,190 @@ cuvsError_t certexB200ToHalf(cuvsResources_t res, const void* src, int32_t kind,
     CERTEX_CUDA(cudaGetLastError());
     r.sync();
     *finite = *static_cast<volatile int*>(bad) == 0 ? 1 : 0;
+  });
+}
+
+namespace {
+
+const certexB200Rotary_t& checked_rotary(const certexB200Rotary_t* r, int64_t head_dim)
+{
+  CERTEX_EXPECTS(r != nullptr && r->turns != nullptr, "certex: null rotation");
+  CERTEX_EXPECTS(r->rotary_dim >= 2 && r->rotary_dim % 2 == 0 && r->rotary_dim <= head_dim,
+                 "certex: the rotation takes an even number of a head's coordinates");
+  return *r;
+}
+
+void check_dtype(int64_t dtype)
+{
+  CERTEX_EXPECTS(dtype >= 0 && dtype <= 2, "certex: the dtype is 0 (float32), 1 (float16) or 2 (bfloat16)");
+}
+
+/// The resources, whose device must be the current one: what is launched goes to the current device.
+const Resources& current_res(cuvsResources_t res)
+{
+  const Resources& r = as_res(res);
+  int device         = -1;
+  CERTEX_CUDA(cudaGetDevice(&device));
+  CERTEX_EXPECTS(device == r.device, "certex: the resources belong to device " + std::to_string(r.device) + ", but device " +
+                                       std::to_string(device) + " is current");
+  return r;
+}
+
+const certexB200PagedCache_t& checked_cache(const certexB200PagedCache_t* c)
+{
+  CERTEX_EXPECTS(c != nullptr && c->keys != nullptr && c->values != nullptr && c->fault != nullptr, "certex: null cache");
+  check_dtype(c->dtype);
+  CERTEX_EXPECTS(c->n_pages >= 1 && c->page_size >= 1 && c->n_kv_heads >= 1 && c->n_pages < (int64_t(1) << 31) &&
+                   c->page_size < (int64_t(1) << 31) && c->n_kv_heads <= 65535,
+                 "certex: the cache needs pages, tokens in them and KV heads");
+  CERTEX_EXPECTS(c->head_dim >= 8 && c->head_dim % 8 == 0 && c->head_dim <= kPagedMaxDim,
+                 "certex: the head dimension of a paged cache is a multiple of 8 and at most " + std::to_string(kPagedMaxDim));
+  const int64_t size = paged_type_size(static_cast<int>(c->dtype));
+  bool fine          = reinterpret_cast<uintptr_t>(c->keys) % 16 == 0 && reinterpret_cast<uintptr_t>(c->values) % 16 == 0;
+  for (int i = 0; i < 3; ++i) { fine = fine && c->key_strides[i] * size % 16 == 0 && c->value_strides[i] * size % 16 == 0; }
+  CERTEX_EXPECTS(fine, "certex: keys, values and the strides of a paged cache must be multiples of 16 bytes");
+  return *c;
+}
+
+void check_rows(const certexB200Rows_t* r, const char* what)
+{
+  CERTEX_EXPECTS(r != nullptr && r->data != nullptr, std::string("certex: null ") + what);
+}
+
+void check_table(const certexB200PageTable_t* t)
+{
+  CERTEX_EXPECTS(t != nullptr && t->n_sequences >= 0 && t->pages_per_sequence >= 0 &&
+                   (t->pages != nullptr || t->n_sequences == 0 || t->pages_per_sequence == 0),
+                 "certex: null page table");
+}
+
+/// What both attentions share: heads, outputs, the workspace.
+void attend_impl(cuvsResources_t res, AttendArgs a, const certexB200PagedCache_t* cache, const certexB200Rows_t* q,
+                 const certexB200Rows_t* out, size_t workspace_bytes)
+{
+  a.cache = checked_cache(cache);
+  CERTEX_EXPECTS(a.n_heads >= 1 && a.n_heads <= 65535 && a.n_heads % a.cache.n_kv_heads == 0,
+                 "certex: the query heads must be a multiple of the KV heads");
+  CERTEX_EXPECTS(a.n_rows >= 0 && a.n_rows * a.n_heads < (int64_t(1) << 31), "certex: too many rows");
+  CERTEX_EXPECTS(std::isfinite(a.scale), "certex: the scale must be finite");
+  if (a.n_rows == 0) { return; }
+  check_rows(q, "queries");
+  check_rows(out, "output");
+  a.q                = *q;
+  a.out              = *out;
+  const Resources& r = current_res(res);
+  const size_t need  = paged_attend_workspace(a, r.sm_count);
+  CERTEX_EXPECTS(workspace_bytes >= need && (need == 0 || (a.workspace != nullptr && reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0)),
+                 "certex: the attention needs a 16-byte aligned workspace of " + std::to_string(need) + " bytes");
+  launch_paged_attend(a, r.sm_count, r.stream);
+  CERTEX_CUDA(cudaGetLastError());
+}
+
+}  // namespace
+
+cuvsError_t certexB200Rotate(cuvsResources_t res, const certexB200Rotary_t* rotary, const certexB200Rows_t* x,
+                             const certexB200Rows_t* y, int64_t n_rows, int64_t n_heads, int64_t head_dim, int32_t dtype,
+                             const void* positions, int32_t positions_64, int32_t inverse)
+{
+  return translate([=] {
+    check_dtype(dtype);
+    CERTEX_EXPECTS(head_dim >= 2 && head_dim % 2 == 0 && head_dim <= 65536, "certex: the head dimension must be even");
+    const certexB200Rotary_t& plan = checked_rotary(rotary, head_dim);
+    CERTEX_EXPECTS(n_rows >= 0 && n_heads >= 1 && n_heads <= 65535 && n_rows < (int64_t(1) << 31) / n_heads, "certex: too many rows");
+    if (n_rows == 0) { return; }
+    check_rows(x, "rows");
+    check_rows(y, "output");
+    CERTEX_EXPECTS(positions != nullptr, "certex: null positions");
+    launch_rotate(plan, *x, *y, n_rows, n_heads, head_dim, dtype, positions, positions_64 != 0, inverse != 0, current_res(res).stream);
+    CERTEX_CUDA(cudaGetLastError());
+  });
+}
+
+cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCache_t* cache, const certexB200Rotary_t* rotary,
+                                  const certexB200PageTable_t* table, const certexB200Rows_t* k, const certexB200Rows_t* v,
+                                  const certexB200Rows_t* q, const certexB200Rows_t* q_out, int64_t n_rows, int64_t n_q_heads,
+                                  const void* positions, int32_t positions_64)
+{
+  return translate([=] {
+    const certexB200PagedCache_t& c = checked_cache(cache);
+    if (rotary != nullptr) { checked_rotary(rotary, c.head_dim); }
+    CERTEX_EXPECTS(n_q_heads >= 0 && n_q_heads <= 65535, "certex: too many query heads");
+    CERTEX_EXPECTS(n_q_heads == 0 || rotary != nullptr, "certex: queries come along to be turned: give a rotation");
+    CERTEX_EXPECTS(n_rows >= 0 && n_rows < (int64_t(1) << 31) / (n_q_heads + 2 * c.n_kv_heads), "certex: too many rows");
+    check_table(table);
+    if (n_rows == 0) { return; }
+    check_rows(k, "keys");
+    check_rows(v, "values");
+    if (n_q_heads > 0) {
+      check_rows(q, "queries");
+      check_rows(q_out, "output");
+    }
+    CERTEX_EXPECTS(positions != nullptr, "certex: null positions");
+    const certexB200Rows_t none{};
+    launch_paged_append(c, rotary, *table, *k, *v, n_q_heads > 0 ? *q : none, n_q_heads > 0 ? *q_out : none, n_rows, n_q_heads,
+                        positions, positions_64 != 0, current_res(res).stream);
+    CERTEX_CUDA(cudaGetLastError());
+  });
+}
+
+cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedCache_t* cache, int64_t n_rows, int64_t n_heads,
+                                     int64_t n_lists, int64_t k, size_t* bytes)
+{
+  return translate([=] {
+    CERTEX_EXPECTS(bytes != nullptr && n_rows >= 0 && n_lists >= 0 && k >= 0, "certex: null argument");
+    AttendArgs a{};
+    a.cache = checked_cache(cache);
+    CERTEX_EXPECTS(n_heads >= 1 && n_heads % a.cache.n_kv_heads == 0, "certex: the query heads must be a multiple of the KV heads");
+    a.n_rows                   = n_rows;
+    a.n_heads                  = n_heads;
+    a.n_lists                  = n_lists;
+    a.k                        = k;
+    a.table.pages_per_sequence = n_lists > 0 ? 0 : (k + a.cache.page_size - 1) / a.cache.page_size;
+    *bytes                     = n_rows > 0 ? paged_attend_workspace(a, as_res(res).sm_count) : 0;
+  });
+}
+
+cuvsError_t certexB200PagedAttend(cuvsResources_t res, const certexB200PagedCache_t* cache, const certexB200PageTable_t* table,
+                                  const int32_t* lengths, int64_t window, const certexB200Rows_t* q, const certexB200Rows_t* out,
+                                  int64_t n_rows, int64_t n_heads, float scale, float* lse, void* workspace, size_t workspace_bytes)
+{
+  return translate([=] {
+    check_table(table);
+    CERTEX_EXPECTS(window >= 0, "certex: the window must not be negative");
+    CERTEX_EXPECTS(lengths != nullptr || n_rows == 0, "certex: null lengths");
+    AttendArgs a{};
+    a.table     = *table;
+    a.lengths   = lengths;
+    a.window    = window;
+    a.n_rows    = n_rows;
+    a.n_heads   = n_heads;
+    a.scale     = scale;
+    a.lse       = lse;
+    a.workspace = workspace;
+    attend_impl(res, a, cache, q, out, workspace_bytes);
+  });
+}
+
+cuvsError_t certexB200PagedAttendSelected(cuvsResources_t res, const certexB200PagedCache_t* cache, const void* selected,
+                                          int32_t selected_64, int64_t n_lists, int64_t k, const certexB200Rows_t* q,
+                                          const certexB200Rows_t* out, int64_t n_rows, int64_t n_heads, float scale, float* lse,
+                                          void* workspace, size_t workspace_bytes)
+{
+  return translate([=] {
+    CERTEX_EXPECTS(cache != nullptr && (n_lists == 1 || n_lists == n_heads || n_lists == cache->n_kv_heads),
+                   "certex: one list of positions per query head, per KV head or for all heads");
+    CERTEX_EXPECTS(k >= 0 && k < (int64_t(1) << 31) && (selected != nullptr || k == 0 || n_rows == 0), "certex: null positions");
+    AttendArgs a{};
+    a.selected    = selected;
+    a.selected_64 = selected_64 != 0;
+    a.n_lists     = n_lists;
+    a.k           = k;
+    a.n_rows      = n_rows;
+    a.n_heads     = n_heads;
+    a.scale       = scale;
+    a.lse         = lse;
+    a.workspace   = workspace;
+    attend_impl(res, a, cache, q, out, workspace_bytes);
   });
 }
 

@@ -1,0 +1,307 @@
+// Rotation of queries and keys by their positions, alone (certexB200Rotate) and on the way into a paged cache
+// (certexB200PagedAppend).
+//
+// A pair (x0, x1) of a head's first r coordinates is turned by the angle a = position * w_i:
+//   y0 = m (x0 cos a - x1 sin a),  y1 = m (x1 cos a + x0 sin a),
+// pairs (2i, 2i + 1) when interleaved, (i, i + r / 2) otherwise. The inverse turns by -a, which is also the gradient.
+//
+// Angles. cos and sin see the angle modulo one turn only, so w_i is kept as a fraction of a turn in units of 2^-64 and
+// position * w_i is the wrapping 64-bit product: the reduction to one turn is exact at every position, with an error of
+// position * 2^-65 turns from the rounding of w_i. Its upper 32 bits, read as a signed fraction, are the angle in
+// [-1/2, 1/2) turns. float32 outputs take sincospif of it; 16-bit outputs the hardware's sine and cosine, whose absolute
+// error of 2^-20.9 on [-pi, pi] lies far below half a step of their types (2^-12 relative and more).
+//
+// Both kernels move bytes: everything is read once and written once, and what bounds them is HBM (large calls) or the
+// launch (a decoding step). A thread owns one "unit" of a head: two vectors of 16 bytes that hold V whole pairs
+// (neighbouring vectors when interleaved, a vector of each half otherwise), so that a pair never crosses threads and the
+// call may be in place. It goes through up to eight heads with the same V sines and cosines: they depend on the row and the
+// pair alone.
+#include "paged.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace certex_b200 {
+namespace {
+
+template <typename T>
+struct Convert;
+template <>
+struct Convert<float> {
+  static __device__ float up(float v) { return v; }
+  static __device__ float down(float v) { return v; }
+};
+template <>
+struct Convert<__half> {
+  static __device__ float up(__half v) { return __half2float(v); }
+  static __device__ __half down(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Convert<__nv_bfloat16> {
+  static __device__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+};
+
+/// V elements that move as one access (V * sizeof(T) is 16, or V is 1).
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Pack {
+  T e[V];
+};
+
+/// Heads that are treated alike: [rows, heads, dim] from `src` to `dst`, or to the cache (pages != null).
+template <typename T>
+struct Section {
+  const T* src;
+  int64_t src_row, src_head;
+  T* dst;
+  int64_t dst_row, dst_head;       // into rows; into pages: dst_row is the page's stride
+  int64_t dst_token;               // into pages: a token's stride
+  int32_t heads;
+  int32_t chunks;                  // ceil(heads / heads of a thread)
+  bool turn, paged;
+};
+
+template <typename T>
+struct TurnArgs {
+  Section<T> sec[3];
+  int32_t n_sec;
+  const uint64_t* turns;
+  int32_t rotary_dim, dim;
+  float magnitude;
+  bool inverse;
+  const void* positions;
+  bool positions_64;
+  int64_t n_rows;
+  // pages
+  certexB200PageTable_t table;
+  int64_t n_pages, page_size;
+  int32_t* fault;
+};
+
+/// The sine and cosine of `turn` (in units of 2^-64 of a turn).
+template <bool EXACT>
+__device__ __forceinline__ void turn_sincos(uint64_t turn, float& s, float& c)
+{
+  const float a = static_cast<float>(static_cast<int32_t>(turn >> 32));
+  if (EXACT) {
+    sincospif(a * 0x1p-31f, &s, &c);
+  } else {
+    const float r = a * (3.14159265358979f * 0x1p-31f);
+    s             = __sinf(r);
+    c             = __cosf(r);
+  }
+}
+
+template <typename T, int V, bool INTERLEAVED, int HEADS>
+__global__ void __launch_bounds__(256) turn_rows_kernel(const TurnArgs<T> a)
+{
+  constexpr bool kExact = sizeof(T) == 4;
+  const int units       = a.dim / (2 * V);  // of a head
+  int chunks            = 0;
+  for (int i = 0; i < a.n_sec; ++i) { chunks += a.sec[i].chunks; }
+  const int64_t item = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t per  = int64_t(chunks) * units;
+  const int64_t row  = item / per;
+  if (row >= a.n_rows) { return; }
+  const int in_row = static_cast<int>(item - row * per);
+  int chunk        = in_row / units;
+  const int unit   = in_row - chunk * units;
+  int which        = 0;
+  while (chunk >= a.sec[which].chunks) { chunk -= a.sec[which++].chunks; }
+  const Section<T> sec = which == 0 ? a.sec[0] : which == 1 ? a.sec[1] : a.sec[2];
+
+  const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[row] : static_cast<const int32_t*>(a.positions)[row];
+  int64_t to        = row * sec.dst_row;
+  if (sec.paged) {
+    if (pos < 0) { return; }  // a row that holds no token
+    const int64_t b = a.table.row_to_sequence ? a.table.row_to_sequence[row] : row;
+    const int64_t p = pos / a.page_size;
+    int64_t page    = -1;
+    if (b >= 0 && b < a.table.n_sequences && p < a.table.pages_per_sequence) { page = a.table.pages[b * a.table.row_stride + p]; }
+    if (page < 0 || page >= a.n_pages) {
+      if (a.fault) { *a.fault = 1; }
+      return;
+    }
+    to = page * sec.dst_row + (pos - p * a.page_size) * sec.dst_token;
+  }
+
+  // where the unit's two vectors lie, and its first pair
+  const int turned = a.rotary_dim / (2 * V);  // units that are turned
+  const bool turn  = sec.turn && unit < turned;
+  int lo = unit * 2 * V, hi = lo + V;
+  if (!INTERLEAVED && unit < turned) {
+    lo = unit * V;
+    hi = lo + a.rotary_dim / 2;
+  }
+  float c[V], s[V];
+  if (turn) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      turn_sincos<kExact>(static_cast<uint64_t>(pos) * a.turns[unit * V + i], s[i], c[i]);
+      c[i] *= a.magnitude;
+      s[i] *= a.inverse ? -a.magnitude : a.magnitude;
+    }
+  }
+
+  using P           = Pack<T, V>;
+  const int first   = chunk * HEADS;
+  const T* from     = sec.src + row * sec.src_row + int64_t(first) * sec.src_head;
+  T* dst            = sec.dst + to + int64_t(first) * sec.dst_head;
+  const int n       = min(HEADS, sec.heads - first);
+  constexpr int kAt = HEADS < 4 ? HEADS : 4;  // heads whose loads are in flight together
+#pragma unroll 1
+  for (int h0 = 0; h0 < n; h0 += kAt) {
+    P x[kAt], y[kAt];
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      if (h0 + j < n) {
+        x[j] = *reinterpret_cast<const P*>(from + (h0 + j) * sec.src_head + lo);
+        y[j] = *reinterpret_cast<const P*>(from + (h0 + j) * sec.src_head + hi);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      if (h0 + j < n) {
+        if (turn) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            // pair i: (x[i], y[i]), or when interleaved the elements 2i and 2i + 1 of both vectors in a row
+            T& e0 = INTERLEAVED ? (2 * i < V ? x[j].e[(2 * i) % V] : y[j].e[(2 * i) % V]) : x[j].e[i];
+            T& e1 = INTERLEAVED ? (2 * i + 1 < V ? x[j].e[(2 * i + 1) % V] : y[j].e[(2 * i + 1) % V]) : y[j].e[i];
+            const float u = Convert<T>::up(e0), w = Convert<T>::up(e1);
+            e0 = Convert<T>::down(u * c[i] - w * s[i]);
+            e1 = Convert<T>::down(w * c[i] + u * s[i]);
+          }
+        }
+        *reinterpret_cast<P*>(dst + (h0 + j) * sec.dst_head + lo) = x[j];
+        *reinterpret_cast<P*>(dst + (h0 + j) * sec.dst_head + hi) = y[j];
+      }
+    }
+  }
+}
+
+template <typename T, int V, int HEADS>
+void run(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
+{
+  int64_t chunks = 0;
+  for (int i = 0; i < a.n_sec; ++i) {
+    a.sec[i].chunks = (a.sec[i].heads + HEADS - 1) / HEADS;
+    chunks += a.sec[i].chunks;
+  }
+  const int64_t items = a.n_rows * chunks * (a.dim / (2 * V));
+  const int threads   = 256;
+  const auto grid     = static_cast<unsigned>((items + threads - 1) / threads);
+  if (interleaved) {
+    turn_rows_kernel<T, V, true, HEADS><<<grid, threads, 0, s>>>(a);
+  } else {
+    turn_rows_kernel<T, V, false, HEADS><<<grid, threads, 0, s>>>(a);
+  }
+}
+
+template <typename T, int V>
+void run(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
+{
+  int64_t heads = 0;
+  for (int i = 0; i < a.n_sec; ++i) { heads += a.sec[i].heads; }
+  // eight heads of a thread share its sines and cosines once there are threads enough to fill the GPU without that
+  const int64_t items = a.n_rows * heads * (a.dim / (2 * V));
+  if (items >= int64_t(8) * 148 * 2048) {
+    run<T, V, 8>(a, interleaved, s);
+  } else {
+    run<T, V, 1>(a, interleaved, s);
+  }
+}
+
+/// Whether every vector of these rows lies on its 16 bytes.
+template <typename T>
+bool aligned(const Section<T>& s)
+{
+  constexpr int V = 16 / sizeof(T);
+  return reinterpret_cast<uintptr_t>(s.src) % 16 == 0 && reinterpret_cast<uintptr_t>(s.dst) % 16 == 0 && s.src_row % V == 0 &&
+         s.src_head % V == 0 && s.dst_row % V == 0 && s.dst_head % V == 0 && s.dst_token % V == 0;
+}
+
+template <typename T>
+void turn(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
+{
+  constexpr int V = 16 / sizeof(T);
+  bool wide       = a.dim % (2 * V) == 0 && a.rotary_dim % (2 * V) == 0;
+  for (int i = 0; i < a.n_sec; ++i) { wide = wide && aligned(a.sec[i]); }
+  wide ? run<T, V>(a, interleaved, s) : run<T, 1>(a, interleaved, s);
+}
+
+template <typename T>
+Section<T> section(const certexB200Rows_t& x, const certexB200Rows_t& y, int64_t heads, bool turned)
+{
+  return {static_cast<const T*>(x.data), x.row_stride, x.head_stride, static_cast<T*>(y.data), y.row_stride, y.head_stride, 0,
+          static_cast<int32_t>(heads), 0, turned, false};
+}
+
+template <typename T>
+TurnArgs<T> turn_args(const certexB200Rotary_t* plan, int64_t dim, const void* positions, bool positions_64, int64_t n_rows)
+{
+  TurnArgs<T> a{};
+  a.turns        = plan ? plan->turns : nullptr;
+  a.rotary_dim   = plan ? static_cast<int32_t>(plan->rotary_dim) : 0;
+  a.magnitude    = plan ? static_cast<float>(plan->magnitude) : 1.0f;
+  a.dim          = static_cast<int32_t>(dim);
+  a.positions    = positions;
+  a.positions_64 = positions_64;
+  a.n_rows       = n_rows;
+  a.page_size    = 1;
+  return a;
+}
+
+template <typename F>
+void by_type(int dtype, F&& f)
+{
+  if (dtype == kPagedF32) {
+    f(float{});
+  } else if (dtype == kPagedF16) {
+    f(__half{});
+  } else {
+    f(__nv_bfloat16{});
+  }
+}
+
+}  // namespace
+
+void launch_rotate(const certexB200Rotary_t& plan, const certexB200Rows_t& x, const certexB200Rows_t& y, int64_t n_rows,
+                   int64_t n_heads, int64_t head_dim, int dtype, const void* positions, bool positions_64, bool inverse,
+                   cudaStream_t s)
+{
+  by_type(dtype, [&](auto t) {
+    using T         = decltype(t);
+    TurnArgs<T> a   = turn_args<T>(&plan, head_dim, positions, positions_64, n_rows);
+    a.inverse       = inverse;
+    a.sec[a.n_sec++] = section<T>(x, y, n_heads, true);
+    turn(a, plan.interleaved != 0, s);
+  });
+}
+
+void launch_paged_append(const certexB200PagedCache_t& cache, const certexB200Rotary_t* plan, const certexB200PageTable_t& table,
+                         const certexB200Rows_t& k, const certexB200Rows_t& v, const certexB200Rows_t& q,
+                         const certexB200Rows_t& q_out, int64_t n_rows, int64_t n_q_heads, const void* positions,
+                         bool positions_64, cudaStream_t s)
+{
+  by_type(static_cast<int>(cache.dtype), [&](auto t) {
+    using T       = decltype(t);
+    TurnArgs<T> a = turn_args<T>(plan, cache.head_dim, positions, positions_64, n_rows);
+    a.table       = table;
+    a.n_pages     = cache.n_pages;
+    a.page_size   = cache.page_size;
+    a.fault       = cache.fault;
+    auto pages    = [&](const certexB200Rows_t& from, void* to, const int64_t* strides, bool turned) {
+      Section<T> x = section<T>(from, {to, strides[0], strides[2]}, cache.n_kv_heads, turned);
+      x.dst_token  = strides[1];
+      x.paged      = true;
+      return x;
+    };
+    if (n_q_heads > 0) { a.sec[a.n_sec++] = section<T>(q, q_out, n_q_heads, true); }
+    a.sec[a.n_sec++] = pages(k, cache.keys, cache.key_strides, plan != nullptr);
+    a.sec[a.n_sec++] = pages(v, cache.values, cache.value_strides, false);
+    turn(a, plan && plan->interleaved != 0, s);
+  });
+}
+
+}  // namespace certex_b200
