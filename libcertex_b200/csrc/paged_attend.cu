@@ -3,122 +3,1076 @@
 //
 //   s_j = scale <q, k_j>,  out = sum_j exp(s_j) v_j / sum_j exp(s_j),  lse = log sum_j exp(s_j)
 //
-// over the positions j that the row may see; a row that sees none gets zeros and -infinity. Scores, the running maximum m,
-// the running sum and the output are held in float32; exp is taken of s_j - m.
+// over the positions j that the row may see; a row that sees none gets zeros and -infinity.
+//
+// What bounds it: every key and value is read once from HBM, for at most a few dozen operations per byte (two products for
+// each query head that shares the KV head). So the work is a stream of rows of 2 d bytes from addresses that the page table or
+// the list of positions names, and everything else has to fit beside it:
+//
+//  * One pass. Scores, the running maximum m, the running sum l and the output stay in registers in float32;
+//    when m grows, l and the output are multiplied by exp2(m_old - m_new). Scores are kept in units of log2 e, so that a
+//    weight is one multiply-add and one exp2.
+//  * The stream is split evenly. The tokens that all rows of the call see, in steps of kStep, are one sequence of work that
+//    is cut into equal shares, a share per resident block ("worker"), wherever the cuts fall: 1 row of 131 072 keys and 64
+//    rows of 1 to 8192 keys load the GPU alike, and lengths are read on the device only. A row and KV head ("unit") that
+//    a cut divides leaves a partial result (m, l, output) per share, which a second, small kernel joins in the order of the
+//    shares: results do not depend on timing. It is launched while the first still runs and waits for it.
+//    Calls whose units are known to be short take a block per unit and one launch.
+//  * Loads are asynchronous copies (cp.async) into a ring of kStages tiles of kKeys keys that belongs to one warp: no
+//    barrier between warps until a unit ends. The table's entries for a tile are fetched one step before its copies.
+//
+// Copies of rows that are not to be seen are zero-filled and their scores set to -infinity, so nothing that lies there (NaN,
+// infinity, another sequence's tokens) has an effect.
 #include "paged.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 namespace certex_b200 {
 namespace {
 
-__device__ __forceinline__ float up(float v) { return v; }
-__device__ __forceinline__ float up(__half v) { return __half2float(v); }
-__device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+constexpr int kWarps   = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStep    = 64;  // tokens of a step of the work split
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2   = 0.6931471805599453f;
 
-constexpr int kThreads = 128;
+/// What the kernels need, in the sizes that they compute with.
+struct Params {
+  const void* keys;
+  const void* values;
+  int64_t k_page, k_token, k_head, v_page, v_token, v_head;  // elements
+  int64_t n_places;                                            // n_pages * page_size
+  int32_t n_pages;
+  uint32_t page_size;
+  int32_t dim;
+  int32_t* fault;
+  // what a row sees
+  const int32_t* pages;
+  int64_t page_row;
+  int64_t n_sequences, most;  // most: tokens that the table can hold
+  const int32_t* row_to_sequence;
+  const int32_t* lengths;     // null: lists
+  int64_t window;
+  const void* lists;
+  int32_t lists_64, n_lists;
+  int64_t k;
+  // queries and answers
+  const void* q;
+  int64_t q_row, q_head;
+  void* out;
+  int64_t o_row, o_head;
+  float* lse;
+  int64_t n_rows;
+  int32_t n_heads, group, subs, per_unit;  // query heads per KV head; units per KV head; query heads of a unit
+  int32_t units;                           // of a row
+  float scale;                             // in units of log2 e
+  // the split
+  int32_t direct;    // a block per unit
+  int32_t workers;
+  int64_t* marks;    // [workers][2]: the unit that a worker goes on with, the one that it leaves unfinished (-1: none)
+  float* parts;      // [workers][2] partial results of part_floats each
+  int32_t part_floats;
+};
 
-/// A block per (row, head): 128 keys at a time, a thread per key for the scores and per coordinate for the sum.
+// ------------------------------------------------------------------------------------------------ types
 template <typename T>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const AttendArgs a)
+struct Type;
+template <>
+struct Type<float> {
+  static __device__ float up(float v) { return v; }
+  static __device__ float down(float v) { return v; }
+};
+template <>
+struct Type<__half> {
+  static __device__ float up(__half v) { return __half2float(v); }
+  static __device__ __half down(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Type<__nv_bfloat16> {
+  static __device__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+};
+
+__device__ __forceinline__ float exp2_fast(float x)
 {
-  __shared__ float q_s[kPagedMaxDim], p_s[kThreads], red[kThreads / 32];
-  __shared__ int64_t at_s[kThreads], vat_s[kThreads];
-  const int64_t row = blockIdx.x / a.n_heads;
-  const int head    = static_cast<int>(blockIdx.x - row * a.n_heads);
-  const int dim     = static_cast<int>(a.cache.head_dim);
-  const int kv      = static_cast<int>(head / (a.n_heads / a.cache.n_kv_heads));
-  const T* q        = static_cast<const T*>(a.q.data) + row * a.q.row_stride + head * a.q.head_stride;
-  const T* keys     = static_cast<const T*>(a.cache.keys) + kv * a.cache.key_strides[2];
-  const T* values   = static_cast<const T*>(a.cache.values) + kv * a.cache.value_strides[2];
-  for (int i = threadIdx.x; i < dim; i += kThreads) { q_s[i] = up(q[i]); }
-  int64_t begin = 0, end = a.k, seq = row;
-  if (a.lengths) {
-    if (a.table.row_to_sequence) { seq = a.table.row_to_sequence[row]; }
-    end   = a.lengths[row];
-    begin = a.window > 0 && end > a.window ? end - a.window : 0;
-    const int64_t most = a.table.pages_per_sequence * a.cache.page_size;
-    if (end > 0 && (seq < 0 || seq >= a.table.n_sequences)) { end = 0, *a.cache.fault = 1; }
-    if (end > most) { end = most, *a.cache.fault = 1; }
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+/// 16 bytes to shared memory, or 16 zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real)
+{
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait()
+{
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ what a row sees
+struct Span {
+  int64_t begin;  // first token
+  int64_t count;
+  int64_t sequence;
+};
+
+__device__ __forceinline__ Span span_of(const Params& p, int64_t row)
+{
+  if (p.lengths == nullptr) { return {0, p.k, row}; }
+  int64_t end       = p.lengths[row];
+  const int64_t seq = p.row_to_sequence ? p.row_to_sequence[row] : row;
+  if (end <= 0) { return {0, 0, 0}; }
+  const bool stranger = seq < 0 || seq >= p.n_sequences;
+  if (stranger || end > p.most) { *p.fault = 1; }
+  if (stranger) { return {0, 0, 0}; }
+  end                 = min(end, p.most);
+  const int64_t begin = p.window > 0 ? max(int64_t(0), end - p.window) : 0;
+  return {begin, end - begin, seq};
+}
+
+/// One unit's share: tokens [i0, i1) of what its row sees.
+struct Segment {
+  int64_t row;
+  int kv, head, n_heads;  // KV head, first query head, query heads
+  int64_t begin;
+  const int32_t* pages;   // the sequence's row of the table, or
+  const void* list;
+  int64_t i0, i1;
+  int64_t slot;           // of the partial result, -1: this is the whole unit
+};
+
+__device__ __forceinline__ Segment segment_of(const Params& p, int64_t row, const Span& s, int unit)
+{
+  Segment g;
+  g.row     = row;
+  g.kv      = unit / p.subs;
+  const int sub = unit - g.kv * p.subs;
+  g.head    = g.kv * p.group + sub * p.per_unit;
+  g.n_heads = min(p.per_unit, p.group - sub * p.per_unit);
+  g.begin   = s.begin;
+  g.pages   = p.pages + s.sequence * p.page_row;
+  const int64_t list = p.n_lists == 1 ? row : p.n_lists == p.n_heads ? row * p.n_lists + g.head : row * p.n_lists + g.kv;
+  g.list    = p.lists_64 ? static_cast<const void*>(static_cast<const int64_t*>(p.lists) + list * p.k)
+                         : static_cast<const void*>(static_cast<const int32_t*>(p.lists) + list * p.k);
+  return g;
+}
+
+/// Where token i of a segment lies: offsets of its key and value, or false.
+__device__ __forceinline__ bool place_of(const Params& p, const Segment& g, int64_t i, int64_t& k_at, int64_t& v_at)
+{
+  int64_t page;
+  uint32_t place;
+  if (p.lengths) {
+    const auto t    = static_cast<uint32_t>(g.begin + i);
+    const uint32_t n = t / p.page_size;
+    place           = t - n * p.page_size;
+    page            = g.pages[n];
+    if (page < 0 || page >= p.n_pages) {
+      *p.fault = 1;
+      return false;
+    }
+  } else {
+    const int64_t at = p.lists_64 ? static_cast<const int64_t*>(g.list)[i] : static_cast<const int32_t*>(g.list)[i];
+    if (at < 0) { return false; }
+    if (at >= p.n_places) {
+      *p.fault = 1;
+      return false;
+    }
+    if (at >> 32) {
+      page = at / p.page_size;
+    } else {
+      page = static_cast<uint32_t>(at) / p.page_size;
+    }
+    place = static_cast<uint32_t>(at - page * p.page_size);
   }
-  float m = -INFINITY, total = 0.f, acc[2] = {0.f, 0.f};
-  bool any = false;
-  for (int64_t t0 = begin; t0 < end; t0 += kThreads) {
+  k_at = page * p.k_page + place * p.k_token;
+  v_at = page * p.v_page + place * p.v_token;
+  return true;
+}
+
+/// Calls body(segment) for this block's share of the work. A block of kThreads threads calls it as a whole.
+template <typename T, typename F>
+__device__ __forceinline__ void for_segments(const Params& p, F&& body)
+{
+  __shared__ int64_t sums[kWarps];
+  __shared__ int64_t found[2];
+  auto nothing_seen = [&](int64_t row, int head, int n_heads, int first, int step) {
+    for (int h = head; h < head + n_heads; ++h) {
+      T* o = static_cast<T*>(p.out) + row * p.o_row + h * p.o_head;
+      for (int c = first; c < p.dim; c += step) { o[c] = Type<T>::down(0.f); }
+      if (p.lse && first == 0) { p.lse[row * p.n_heads + h] = -INFINITY; }
+    }
+  };
+  if (p.direct) {
+    const int64_t row = blockIdx.x / p.units;
+    const Span s      = span_of(p, row);
+    Segment g         = segment_of(p, row, s, static_cast<int>(blockIdx.x - row * p.units));
+    if (s.count == 0) {
+      nothing_seen(row, g.head, g.n_heads, threadIdx.x, kThreads);
+      return;
+    }
+    g.i0 = 0, g.i1 = s.count, g.slot = -1;
+    body(g);
+    return;
+  }
+
+  // how many steps there are in all: every block counts for itself
+  auto steps_of = [&](int64_t row) { return (span_of(p, row).count + kStep - 1) / kStep; };
+  const int64_t same = p.lengths ? 0 : (p.k + kStep - 1) / kStep;
+  int64_t total = 0, mine = 0;
+  if (!p.lengths) {
+    total = p.n_rows * same;
+  } else if (p.n_rows == 1) {
+    total = steps_of(0);
+  } else {
+    for (int64_t row = threadIdx.x; row < p.n_rows; row += kThreads) {
+      const int64_t n = steps_of(row);
+      mine += n;
+    }
+    for (int o = 16; o > 0; o >>= 1) { mine += __shfl_xor_sync(~0u, mine, o); }
+    if (threadIdx.x % 32 == 0) { sums[threadIdx.x / 32] = mine; }
     __syncthreads();
-    const int64_t t = t0 + threadIdx.x;
-    int64_t page = -1, place = 0;
-    if (t < end) {
-      if (a.lengths) {
-        page  = a.table.pages[seq * a.table.row_stride + t / a.cache.page_size];
-        place = t % a.cache.page_size;
-        if (page < 0 || page >= a.cache.n_pages) { page = -1, *a.cache.fault = 1; }
-      } else {
-        const int64_t i = (row * a.n_lists + head / (a.n_heads / a.n_lists)) * a.k + t;
-        const int64_t p = a.selected_64 ? static_cast<const int64_t*>(a.selected)[i] : static_cast<const int32_t*>(a.selected)[i];
-        if (p >= 0) {
-          page  = p / a.cache.page_size;
-          place = p % a.cache.page_size;
-          if (page >= a.cache.n_pages) { page = -1, *a.cache.fault = 1; }
+    for (int w = 0; w < kWarps; ++w) { total += sums[w]; }
+  }
+  // rows that see nothing have no steps: the blocks share them out
+  if (p.lengths) {
+    for (int64_t row = blockIdx.x; row < p.n_rows; row += gridDim.x) {
+      if (steps_of(row) == 0) { nothing_seen(row, 0, p.n_heads, threadIdx.x, kThreads); }
+    }
+  }
+  total *= p.units;
+  const int64_t workers = min(int64_t(p.workers), total), w = blockIdx.x;
+  if (threadIdx.x == 0) { p.marks[2 * w] = p.marks[2 * w + 1] = -1; }
+  if (w >= workers) { return; }
+  int64_t at        = total * w / workers;
+  const int64_t end = total * (w + 1) / workers;
+
+  // the row of step `at`, and the first step of that row
+  int64_t row = 0, base = 0;
+  if (!p.lengths) {
+    row  = at / (same * p.units);
+    base = row * same * p.units;
+  } else if (p.n_rows > 1) {
+    int64_t before = 0;
+    for (int64_t r0 = 0; r0 < p.n_rows; r0 += kThreads) {
+      const int64_t r = r0 + threadIdx.x;
+      const int64_t n = r < p.n_rows ? steps_of(r) * p.units : 0;
+      int64_t upto    = n;  // inclusive sum over the warp
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(~0u, upto, o);
+        if (threadIdx.x % 32 >= o) { upto += x; }
+      }
+      __syncthreads();
+      if (threadIdx.x % 32 == 31) { sums[threadIdx.x / 32] = upto; }
+      __syncthreads();
+      int64_t first = before;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < threadIdx.x / 32) { first += sums[i]; }
+        before += sums[i];
+      }
+      first += upto - n;
+      if (n > 0 && first <= at && at < first + n) { found[0] = r, found[1] = first; }
+      if (at < before) { break; }
+    }
+    __syncthreads();
+    row = found[0], base = found[1];
+  }
+
+  while (at < end) {
+    const Span s        = span_of(p, row);
+    const int64_t steps = (s.count + kStep - 1) / kStep;
+    if (steps == 0) {
+      ++row;
+      continue;
+    }
+    const auto unit = static_cast<int>((at - base) / steps);
+    const int64_t u0 = base + unit * steps, u1 = u0 + steps, to = min(end, u1);
+    Segment g = segment_of(p, row, s, unit);
+    g.i0      = (at - u0) * kStep;
+    g.i1      = min(s.count, (to - u0) * kStep);
+    // a partial result that begins a unit belongs to the worker's second slot, one that goes on with it to the first
+    g.slot    = at == u0 && to == u1 ? -1 : 2 * w + (at > u0 ? 0 : 1);
+    if (threadIdx.x == 0) {
+      const int64_t id = row * p.units + unit;
+      if (at > u0) { p.marks[2 * w] = id; }
+      if (to < u1) { p.marks[2 * w + 1] = id; }
+    }
+    body(g);
+    at = to;
+    if (at == base + steps * p.units) {
+      base = at;
+      ++row;
+    }
+  }
+}
+
+/// The answer of a unit's query head from its sums, or a partial result: coordinate c of query i.
+template <typename T>
+__device__ __forceinline__ void put_out(const Params& p, const Segment& g, int i, int c, float v)
+{
+  if (g.slot >= 0) {
+    p.parts[g.slot * p.part_floats + 4 * p.per_unit + i * p.dim + c] = v;
+  } else {
+    (static_cast<T*>(p.out) + g.row * p.o_row + (g.head + i) * p.o_head)[c] = Type<T>::down(v);
+  }
+}
+
+/// m, l and whether anything was seen, of query i (once per query).
+__device__ __forceinline__ void put_sums(const Params& p, const Segment& g, int i, float m, float l, bool any)
+{
+  if (g.slot >= 0) {
+    float* to = p.parts + g.slot * p.part_floats + 4 * i;
+    to[0] = m, to[1] = l, to[2] = any ? 1.f : 0.f;
+  } else if (p.lse) {
+    p.lse[g.row * p.n_heads + g.head + i] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ 16-bit types
+// Tensor cores by warp-level products (mma.m16n8k16): with one new token there are 1 to 16 queries per KV head, and tcgen05's
+// smallest tile of 128 rows would be nearly empty. Keys and values take the 16-row side of the product and the
+// queries the 8-column side, so that 8 queries fill it: S^T = K Q^T, then O^T = V^T P^T. The two products of a tile of
+// 16 keys by d = 128 are 8 + 16 instructions for 8 KB read.
+//
+// Weights enter the second product as two 16-bit numbers, the upper part cut off and the rest (p = hi + lo to 2^-16), because a
+// weight rounded once to bfloat16 would add as much error as the rounding of the result. lo is kept positive: zero times an
+// infinite value would be NaN. Weights of float16 are multiplied by 2^12, since float16 has nothing below 2^-24; l carries
+// the factor too, so it cancels.
+constexpr int kKeys   = 16;  // of a tile
+constexpr int kStages = 3;
+
+__device__ __forceinline__ void load_matrix(uint32_t (&a)[4], uint32_t at)
+{
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void load_matrix_t(uint32_t (&a)[4], uint32_t at)
+{
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
+{
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  static constexpr float kRaise = 0.f;  // log2 of the factor on weights
+  static __device__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+  {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  /// (x, y) as two pairs of numbers whose sum they are; x in the lower halves.
+  static __device__ void split(float x, float y, uint32_t& hi, uint32_t& lo)
+  {
+    const uint32_t a = __float_as_uint(x) & 0xffff0000u, b = __float_as_uint(y) & 0xffff0000u;
+    hi = (a >> 16) | b;
+    const __nv_bfloat162 r = __floats2bfloat162_rn(fmaxf(x - __uint_as_float(a), 1.2e-38f), fmaxf(y - __uint_as_float(b), 1.2e-38f));
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <>
+struct Half<__half> {
+  static constexpr float kRaise = 12.f;
+  static __device__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+  {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ void split(float x, float y, uint32_t& hi, uint32_t& lo)
+  {
+    const __half2 h = __halves2half2(__float2half_rz(x), __float2half_rz(y));
+    hi              = *reinterpret_cast<const uint32_t*>(&h);
+    const __half2 r = __floats2half2_rn(fmaxf(x - __low2float(h), 6e-8f), fmaxf(y - __high2float(h), 6e-8f));
+    lo              = *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+
+/// D: the head dimension, padded to what the tiles are built for; NT: groups of eight queries.
+template <int D>
+struct HalfTile {
+  static constexpr int kPitch = D * 2 + 16;  // bytes of a row in shared memory: eight rows start in eight different banks
+  static constexpr int kBytes = kKeys * kPitch;
+  static constexpr int kWarp  = kStages * 2 * kBytes;
+  static constexpr int kAll   = kWarps * kWarp;
+  static constexpr int kLanes = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes that copy a row
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attend_half_kernel(const Params p)
+{
+  using Tile = HalfTile<D>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
+  unsigned char* ring = smem + warp * Tile::kWarp;
+  const uint32_t ring_at = smem_of(ring);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.dim < D) {
+    // the columns behind the last coordinate are multiplied by zeros of the queries: they must hold numbers
+    for (int i = lane * 16; i < Tile::kWarp; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
+    __syncwarp();
+  }
+
+  for_segments<T>(p, [&](const Segment& g) {
+    // the queries, as the 8-column side of the first product
+    uint32_t qf[NT][D / 16][2];
+    {
+      const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int i  = n * 8 + g8;
+        const T* row = q + i * p.q_head;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c = k * 16 + h * 8 + t4 * 2;
+            uint32_t v  = 0;
+            if (i < g.n_heads && c < p.dim) {
+              const auto a = *reinterpret_cast<const uint16_t*>(row + c), b = *reinterpret_cast<const uint16_t*>(row + c + 1);
+              v            = a | (uint32_t(b) << 16);
+            }
+            qf[n][k][h] = v;
+          }
         }
       }
     }
-    float s = -INFINITY;
-    if (page >= 0) {
-      const T* key = keys + page * a.cache.key_strides[0] + place * a.cache.key_strides[1];
-      s            = 0.f;
-      for (int i = 0; i < dim; ++i) { s += q_s[i] * up(key[i]); }
-      s *= a.scale;
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) { o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f; }
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
     }
-    any                = any || __syncthreads_or(page >= 0);
-    at_s[threadIdx.x]  = page;
-    vat_s[threadIdx.x] = page * a.cache.value_strides[0] + place * a.cache.value_strides[1];
-    float top = s;
-    for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, o)); }
-    if (threadIdx.x % 32 == 0) { red[threadIdx.x / 32] = top; }
-    __syncthreads();
-    float next = m;
-    for (float r : red) { next = fmaxf(next, r); }
-    const float base  = next == -INFINITY ? 0.f : next;
-    const float alpha = expf(m - base);
-    m                 = next;
-    const float p     = s != s ? s : expf(s - base);
-    p_s[threadIdx.x]  = p;
-    __syncthreads();
-    total *= alpha, acc[0] *= alpha, acc[1] *= alpha;
-    for (int j = 0; j < kThreads; ++j) {
-      if (at_s[j] < 0) { continue; }
-      total += p_s[j];
-      for (int i = 0; i < 2; ++i) {
-        const int c = threadIdx.x + i * kThreads;
-        if (c < dim) { acc[i] += p_s[j] * up(values[vat_s[j] + c]); }
+
+    const T* keys   = static_cast<const T*>(p.keys) + g.kv * p.k_head;
+    const T* values = static_cast<const T*>(p.values) + g.kv * p.v_head;
+    // tiles of this warp: warp, warp + kWarps, ...
+    const int tiles = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
+    const int n     = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+    // the place of key lane % 16 of the next tile to be copied
+    int64_t k_at = 0, v_at = 0;
+    bool real    = false;
+    auto look_up = [&](int j) {
+      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
+      real            = j < n && i < g.i1 && place_of(p, g, i, k_at, v_at);
+    };
+    uint32_t masks = 0;  // of the tiles in the ring: which keys are real, newest lowest
+    uint32_t older = 0;
+    auto copy = [&](int stage) {
+      constexpr int kRows = 32 / Tile::kLanes;  // rows that the warp copies at once
+      const int chunk = lane % Tile::kLanes, sub = lane / Tile::kLanes;
+      const uint32_t to = ring_at + stage * 2 * Tile::kBytes + chunk * 16;
+      const bool inside = chunk * 8 < p.dim;
+#pragma unroll
+      for (int r = 0; r < kKeys; r += kRows) {
+        const int row    = r + sub;
+        const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
+        const bool ok    = __shfl_sync(~0u, real, row);
+        if (inside) {
+          copy16(to + row * Tile::kPitch, ok ? keys + ka + chunk * 8 : keys, ok);
+          copy16(to + Tile::kBytes + row * Tile::kPitch, ok ? values + va + chunk * 8 : values, ok);
+        }
+      }
+      older = masks >> 16;
+      masks = (masks << 16) | (__ballot_sync(~0u, real) & 0xffffu);
+    };
+    bool any = false;
+    look_up(0);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      copy(s);
+      copy_commit();
+      look_up(s + 1);
+    }
+    int stage = 0;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      copy(stage == 0 ? kStages - 1 : stage - 1);
+      copy_commit();
+      look_up(j + kStages);
+      const uint32_t mask = older & 0xffffu;  // kStages - 1 = 2 tiles were copied behind this one
+      any                 = any || mask != 0;
+      const uint32_t k_tile = ring_at + stage * 2 * Tile::kBytes, v_tile = k_tile + Tile::kBytes;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+
+      float s[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) { s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f; }
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t a[4];
+        load_matrix(a, k_tile + (lane % 16) * Tile::kPitch + (k * 2 + lane / 16) * 16);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) { Half<T>::mma(s[i], a, qf[i][k][0], qf[i][k][1]); }
+      }
+      const bool see0 = mask >> g8 & 1, see1 = mask >> (g8 + 8) & 1;
+      uint32_t hi[NT][2], lo[NT][2];
+      bool grew = false;
+      float alpha[NT][2];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float base[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          s[i][c]     = see0 ? s[i][c] * p.scale : -INFINITY;
+          s[i][c + 2] = see1 ? s[i][c + 2] * p.scale : -INFINITY;
+          float top   = fmaxf(s[i][c], s[i][c + 2]);
+          top         = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+          top         = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+          top         = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          top         = fmaxf(top, m[i][c]);
+          base[c]     = top == -INFINITY ? 0.f : top;
+          alpha[i][c] = exp2_fast(m[i][c] - base[c]);
+          grew        = grew || top > m[i][c];
+          m[i][c]     = top;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) { s[i][c] = exp2_fast(s[i][c] - base[c & 1] + Half<T>::kRaise); }
+        l[i][0] = l[i][0] * alpha[i][0] + (s[i][0] + s[i][2]);
+        l[i][1] = l[i][1] * alpha[i][1] + (s[i][1] + s[i][3]);
+        Half<T>::split(s[i][0], s[i][1], hi[i][0], lo[i][0]);
+        Half<T>::split(s[i][2], s[i][3], hi[i][1], lo[i][1]);
+        hi[i][0] = transpose8x8(hi[i][0]), hi[i][1] = transpose8x8(hi[i][1]);
+        lo[i][0] = transpose8x8(lo[i][0]), lo[i][1] = transpose8x8(lo[i][1]);
+      }
+      if (__any_sync(~0u, grew)) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            o[i][d][0] *= alpha[i][0], o[i][d][1] *= alpha[i][1];
+            o[i][d][2] *= alpha[i][0], o[i][d][3] *= alpha[i][1];
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t a[4];
+        load_matrix_t(a, v_tile + (lane % 8 + (lane / 16) * 8) * Tile::kPitch + (d * 2 + lane / 8 % 2) * 16);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          Half<T>::mma(o[i][d], a, hi[i][0], hi[i][1]);
+          Half<T>::mma(o[i][d], a, lo[i][0], lo[i][1]);
+        }
       }
     }
+    copy_wait<0>();
+    __syncwarp();
+
+    // the warps' results meet in shared memory, each in its own ring
+    constexpr int kRow = D + 4;
+    auto* sums         = reinterpret_cast<float*>(ring);  // [8 NT][kRow]: output, m, l, any
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float* to = sums + (i * 8 + t4 * 2 + c) * kRow;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          to[d * 16 + g8]     = o[i][d][c];
+          to[d * 16 + g8 + 8] = o[i][d][c + 2];
+        }
+        float sum = l[i][c];
+        sum += __shfl_xor_sync(~0u, sum, 4);
+        sum += __shfl_xor_sync(~0u, sum, 8);
+        sum += __shfl_xor_sync(~0u, sum, 16);
+        if (g8 == 0) { to[D] = m[i][c], to[D + 1] = sum, to[D + 2] = any ? 1.f : 0.f; }
+      }
+    }
+    __syncthreads();
+    for (int i = 0; i < g.n_heads; ++i) {
+      float w[kWarps], top = -INFINITY, sum = 0.f, seen = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        w[x] = reinterpret_cast<float*>(smem + x * Tile::kWarp)[i * kRow + D];
+        top  = fmaxf(top, w[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float* from = reinterpret_cast<float*>(smem + x * Tile::kWarp) + i * kRow;
+        w[x]              = top == -INFINITY ? 1.f : exp2_fast(w[x] - top);
+        sum += w[x] * from[D + 1];
+        seen += from[D + 2];
+      }
+      const float scale = g.slot >= 0 ? 1.f : seen > 0.f ? 1.f / sum : 0.f;
+      for (int c = threadIdx.x; c < p.dim; c += kThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) { v += w[x] * reinterpret_cast<float*>(smem + x * Tile::kWarp)[i * kRow + c]; }
+        put_out<T>(p, g, i, c, seen > 0.f ? v * scale : 0.f);
+      }
+      if (threadIdx.x == 0) { put_sums(p, g, i, top - Half<T>::kRaise, sum, seen > 0.f); }
+    }
+    __syncthreads();
+    if (p.dim < D) {
+      for (int i = lane * 16; i < Tile::kWarp; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
+      __syncwarp();
+    }
+  });
+}
+
+// ------------------------------------------------------------------------------------------------ float32
+// No tensor core keeps float32's products, so this is fused multiply-adds: a lane (or two, or four) per key for the scores, with
+// the queries broadcast from shared memory, then a lane per four coordinates for the sum over values.
+template <int D>
+struct FloatTile {
+  static constexpr int kKeys  = D <= 128 ? 16 : 8;
+  static constexpr int kParts = 32 / kKeys;  // lanes of a key
+  static constexpr int kPitch = D * 4 + 16;
+  static constexpr int kBytes = kKeys * kPitch;
+  static constexpr int kStages = 3;
+  static constexpr int kRing  = kStages * 2 * kBytes;
+  static constexpr int kCols  = D / 32;      // coordinates of a lane
+};
+
+/// Q: queries of a unit that the kernel is built for.
+template <int D, int Q>
+struct FloatShared {
+  static constexpr int kWarp = FloatTile<D>::kRing + Q * FloatTile<D>::kKeys * 4;  // ring, weights [Q][keys]
+  static constexpr int kAll  = kWarps * kWarp + Q * D * 4;                         // and the queries [Q][D]
+};
+
+template <int N>
+struct alignas(N < 4 ? N * 4 : 16) Floats {
+  float e[N];
+};
+
+template <int D, int Q>
+__global__ void __launch_bounds__(kThreads) attend_float_kernel(const Params p)
+{
+  using Tile          = FloatTile<D>;
+  constexpr int kKeys = Tile::kKeys, kStages = Tile::kStages, kCols = Tile::kCols;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  unsigned char* ring    = smem + warp * FloatShared<D, Q>::kWarp;
+  const uint32_t ring_at = smem_of(ring);
+  auto* weights          = reinterpret_cast<float*>(ring + Tile::kRing);
+  auto* q_s              = reinterpret_cast<float*>(smem + kWarps * FloatShared<D, Q>::kWarp);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  auto clear = [&] {
+    if (p.dim < D) {
+      for (int i = lane * 16; i < Tile::kRing; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
+      __syncwarp();
+    }
+  };
+  clear();
+
+  for_segments<float>(p, [&](const Segment& g) {
+    const float* q = static_cast<const float*>(p.q) + g.row * p.q_row + g.head * p.q_head;
+    for (int i = threadIdx.x; i < Q * D; i += kThreads) {
+      const int x = i / D, c = i % D;
+      q_s[i] = x < g.n_heads && c < p.dim ? q[x * p.q_head + c] : 0.f;
+    }
+    __syncthreads();
+    float o[Q][kCols], m[Q], l[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) { o[i][c] = 0.f; }
+    }
+    const float* keys   = static_cast<const float*>(p.keys) + g.kv * p.k_head;
+    const float* values = static_cast<const float*>(p.values) + g.kv * p.v_head;
+    const int tiles     = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
+    const int n         = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+    int64_t k_at = 0, v_at = 0;
+    bool real    = false;
+    auto look_up = [&](int j) {
+      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
+      real            = j < n && i < g.i1 && place_of(p, g, i, k_at, v_at);
+    };
+    uint32_t masks[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) { masks[i] = 0; }
+    auto copy = [&](int stage) {
+      constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kRows = 32 / kLanes, kTimes = D / 4 / kLanes;
+      const int sub = lane / kLanes;
+#pragma unroll
+      for (int r = 0; r < kKeys; r += kRows) {
+        const int row    = r + sub;
+        const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
+        const bool ok    = __shfl_sync(~0u, real, row);
+#pragma unroll
+        for (int x = 0; x < kTimes; ++x) {
+          const int chunk = lane % kLanes + x * kLanes;
+          if (chunk * 4 < p.dim) {
+            const uint32_t to = ring_at + stage * 2 * Tile::kBytes + row * Tile::kPitch + chunk * 16;
+            copy16(to, ok ? keys + ka + chunk * 4 : keys, ok);
+            copy16(to + Tile::kBytes, ok ? values + va + chunk * 4 : values, ok);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = kStages - 1; i > 0; --i) { masks[i] = masks[i - 1]; }
+      masks[0] = __ballot_sync(~0u, real);
+    };
+    bool any = false;
+    look_up(0);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      copy(s);
+      copy_commit();
+      look_up(s + 1);
+    }
+    int stage = 0;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      copy(stage == 0 ? kStages - 1 : stage - 1);
+      copy_commit();
+      look_up(j + kStages);
+      const uint32_t mask = masks[kStages - 1];
+      any                 = any || mask != 0;
+      const unsigned char* k_tile = ring + stage * 2 * Tile::kBytes;
+      const unsigned char* v_tile = k_tile + Tile::kBytes;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+
+      const int key = lane % kKeys, part = lane / kKeys;
+      float s[Q];
+#pragma unroll
+      for (int i = 0; i < Q; ++i) { s[i] = 0.f; }
+#pragma unroll 4
+      for (int c = part * 4; c < D; c += Tile::kParts * 4) {
+        const float4 k = *reinterpret_cast<const float4*>(k_tile + key * Tile::kPitch + c * 4);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(q_s + i * D + c);
+          s[i] += x.x * k.x + x.y * k.y + x.z * k.z + x.w * k.w;
+        }
+      }
+      const bool see = mask >> key & 1;
+      float alpha[Q];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+#pragma unroll
+        for (int x = kKeys; x < 32; x <<= 1) { s[i] += __shfl_xor_sync(~0u, s[i], x); }
+        s[i]      = see ? s[i] * p.scale : -INFINITY;
+        float top = s[i];
+#pragma unroll
+        for (int x = 1; x < kKeys; x <<= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, x)); }
+        top              = fmaxf(top, m[i]);
+        const float base = top == -INFINITY ? 0.f : top;
+        alpha[i]         = exp2_fast(m[i] - base);
+        grew             = grew || top > m[i];
+        m[i]             = top;
+        const float w    = exp2_fast(s[i] - base);
+        l[i]             = l[i] * alpha[i] + (part == 0 ? w : 0.f);
+        if (part == 0) { weights[i * kKeys + key] = w; }
+      }
+      __syncwarp();
+      if (grew) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) { o[i][c] *= alpha[i]; }
+        }
+      }
+#pragma unroll 2
+      for (int k = 0; k < kKeys; k += 4) {
+        Floats<kCols> v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          v[x] = *reinterpret_cast<const Floats<kCols>*>(v_tile + (k + x) * Tile::kPitch + lane * kCols * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          const float4 w = *reinterpret_cast<const float4*>(weights + i * kKeys + k);
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            o[i][c] += w.x * v[0].e[c] + w.y * v[1].e[c] + w.z * v[2].e[c] + w.w * v[3].e[c];
+          }
+        }
+      }
+      __syncwarp();
+    }
+    copy_wait<0>();
+    __syncwarp();
+
+    constexpr int kRow = D + 4;
+    auto* sums         = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) { sums[i * kRow + lane * kCols + c] = o[i][c]; }
+      float sum = l[i];
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) { sum += __shfl_xor_sync(~0u, sum, x); }
+      if (lane == 0) { sums[i * kRow + D] = m[i], sums[i * kRow + D + 1] = sum, sums[i * kRow + D + 2] = any ? 1.f : 0.f; }
+    }
+    __syncthreads();
+    constexpr int kStride = FloatShared<D, Q>::kWarp;
+    for (int i = 0; i < g.n_heads; ++i) {
+      float w[kWarps], top = -INFINITY, sum = 0.f, seen = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        w[x] = reinterpret_cast<float*>(smem + x * kStride)[i * kRow + D];
+        top  = fmaxf(top, w[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float* from = reinterpret_cast<float*>(smem + x * kStride) + i * kRow;
+        w[x]              = top == -INFINITY ? 1.f : exp2_fast(w[x] - top);
+        sum += w[x] * from[D + 1];
+        seen += from[D + 2];
+      }
+      const float scale = g.slot >= 0 ? 1.f : seen > 0.f ? 1.f / sum : 0.f;
+      for (int c = threadIdx.x; c < p.dim; c += kThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) { v += w[x] * reinterpret_cast<float*>(smem + x * kStride)[i * kRow + c]; }
+        put_out<float>(p, g, i, c, seen > 0.f ? v * scale : 0.f);
+      }
+      if (threadIdx.x == 0) { put_sums(p, g, i, top, sum, seen > 0.f); }
+    }
+    __syncthreads();
+    clear();
+  });
+}
+
+// ------------------------------------------------------------------------------------------------ joining the shares
+// Block (w, i): if worker w left a unit unfinished that it had begun, joins that unit's partial results for query i. They lie in
+// w's second slot and in the first slots of the workers behind it that went on with the unit.
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
+{
+  extern __shared__ float weight[];  // [workers]
+  __shared__ float red[2][kJoinThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int w = blockIdx.x, i = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int64_t id = p.marks[2 * w + 1];
+  if (id < 0 || p.marks[2 * w] == id) { return; }
+  const int64_t row = id / p.units;
+  const Segment g   = segment_of(p, row, Span{0, 0, 0}, static_cast<int>(id - row * p.units));
+  if (i >= g.n_heads) { return; }
+  int n = 1;
+  for (int x0 = w + 1;; x0 += kJoinThreads) {
+    const int x     = x0 + static_cast<int>(threadIdx.x);
+    const int count = __syncthreads_count(x < p.workers && p.marks[2 * x] == id);
+    n += count;
+    if (count < kJoinThreads) { break; }
   }
-  T* out = static_cast<T*>(a.out.data) + row * a.out.row_stride + head * a.out.head_stride;
-  for (int i = 0; i < 2; ++i) {
-    const int c = threadIdx.x + i * kThreads;
-    if (c < dim) { put(out + c, any ? acc[i] / total : 0.f); }
+  auto part = [&](int x) { return p.parts + (x == 0 ? 2 * int64_t(w) + 1 : 2 * int64_t(w + x)) * p.part_floats; };
+  float top = -INFINITY;
+  for (int x = threadIdx.x; x < n; x += kJoinThreads) { top = fmaxf(top, part(x)[4 * i]); }
+  for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, o)); }
+  if (lane == 0) { red[0][warp] = top; }
+  __syncthreads();
+  for (float r : red[0]) { top = fmaxf(top, r); }
+  __syncthreads();
+  float sum = 0.f, seen = 0.f;
+  for (int x = threadIdx.x; x < n; x += kJoinThreads) {
+    const float* from = part(x) + 4 * i;
+    const float f     = top == -INFINITY ? 1.f : exp2_fast(from[0] - top);
+    weight[x]         = f;
+    sum += f * from[1];
+    seen += from[2];
   }
-  if (a.lse && threadIdx.x == 0) { a.lse[row * a.n_heads + head] = any ? m + logf(total) : -INFINITY; }
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(~0u, sum, o);
+    seen += __shfl_xor_sync(~0u, seen, o);
+  }
+  if (lane == 0) { red[0][warp] = sum, red[1][warp] = seen; }
+  __syncthreads();
+  sum = seen = 0.f;
+  for (int x = 0; x < kJoinThreads / 32; ++x) { sum += red[0][x], seen += red[1][x]; }
+  for (int c = threadIdx.x; c < p.dim; c += kJoinThreads) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int x = 0; x < n; ++x) { v += weight[x] * part(x)[4 * p.per_unit + i * p.dim + c]; }
+    (static_cast<T*>(p.out) + row * p.o_row + (g.head + i) * p.o_head)[c] = Type<T>::down(seen > 0.f ? v / sum : 0.f);
+  }
+  if (p.lse && threadIdx.x == 0) { p.lse[row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
+}
+
+// ------------------------------------------------------------------------------------------------ launch
+/// Units whose rows see at most so many tokens, as far as the host can tell, get a block each.
+constexpr int64_t kDirectTokens = 512;
+
+struct Plan {
+  int32_t per_unit, subs, units;
+  int direct;
+  int64_t blocks;
+  int part_floats;
+  size_t bytes;
+};
+
+Plan plan_of(const AttendArgs& a, int sm_count)
+{
+  Plan n;
+  const bool half = a.cache.dtype != kPagedF32;
+  const int dim   = static_cast<int>(a.cache.head_dim);
+  const int group = static_cast<int>(a.n_heads / a.cache.n_kv_heads);
+  // a list per query head is a unit of one query; otherwise the heads that share a KV head are taken together
+  const bool alone = a.n_lists == a.n_heads && a.n_lists != a.cache.n_kv_heads;
+  n.per_unit       = alone ? 1 : std::min(group, half ? 16 : 8);
+  n.subs           = (group + n.per_unit - 1) / n.per_unit;
+  n.units          = static_cast<int32_t>(a.cache.n_kv_heads) * n.subs;
+  int64_t most     = a.n_lists > 0 ? a.k : a.table.pages_per_sequence * a.cache.page_size;
+  if (a.n_lists == 0 && a.window > 0) { most = std::min(most, a.window); }
+  const int64_t units = a.n_rows * n.units;
+  n.direct            = most <= kDirectTokens;
+  const int resident  = sm_count * (half && dim <= 128 ? 2 : !half && dim <= 64 ? 2 : 1);
+  n.blocks            = n.direct ? units : std::min<int64_t>(resident, units * ((most + kStep - 1) / kStep));
+  n.part_floats       = n.per_unit * (dim + 4);
+  n.bytes             = n.direct ? 0 : static_cast<size_t>(n.blocks) * 2 * (8 + sizeof(float) * n.part_floats);
+  return n;
+}
+
+template <typename Kernel>
+void launch(Kernel kernel, int smem, const Params& p, int64_t blocks, cudaStream_t s)
+{
+  if (smem > 32 * 1024) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
+  kernel<<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(p);
+}
+
+template <typename T, int D>
+void launch_half(const Params& p, int64_t blocks, cudaStream_t s)
+{
+  if (p.per_unit <= 8) {
+    launch(attend_half_kernel<T, D, 1>, HalfTile<D>::kAll, p, blocks, s);
+  } else {
+    launch(attend_half_kernel<T, D, 2>, HalfTile<D>::kAll, p, blocks, s);
+  }
+}
+
+template <typename T>
+void launch_half(const Params& p, int64_t blocks, cudaStream_t s)
+{
+  if (p.dim <= 64) {
+    launch_half<T, 64>(p, blocks, s);
+  } else if (p.dim <= 96) {
+    launch_half<T, 96>(p, blocks, s);
+  } else if (p.dim <= 128) {
+    launch_half<T, 128>(p, blocks, s);
+  } else if (p.dim <= 192) {
+    launch_half<T, 192>(p, blocks, s);
+  } else {
+    launch_half<T, 256>(p, blocks, s);
+  }
+}
+
+template <int D>
+void launch_float(const Params& p, int64_t blocks, cudaStream_t s)
+{
+  if (p.per_unit == 1) {
+    launch(attend_float_kernel<D, 1>, FloatShared<D, 1>::kAll, p, blocks, s);
+  } else if (p.per_unit <= 4) {
+    launch(attend_float_kernel<D, 4>, FloatShared<D, 4>::kAll, p, blocks, s);
+  } else {
+    launch(attend_float_kernel<D, 8>, FloatShared<D, 8>::kAll, p, blocks, s);
+  }
+}
+
+template <typename T>
+void launch_join(const Params& p, cudaStream_t s)
+{
+  cudaLaunchConfig_t c{};
+  c.gridDim          = dim3(static_cast<unsigned>(p.workers), static_cast<unsigned>(p.per_unit));
+  c.blockDim         = dim3(kJoinThreads);
+  c.dynamicSmemBytes = sizeof(float) * static_cast<size_t>(p.workers);
+  c.stream           = s;
+  cudaLaunchAttribute early{};
+  early.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs                                          = &early;
+  c.numAttrs                                       = 1;
+  cudaLaunchKernelEx(&c, join_kernel<T>, p);
 }
 
 }  // namespace
 
-size_t paged_attend_workspace(const AttendArgs&, int) { return 0; }
+size_t paged_attend_workspace(const AttendArgs& a, int sm_count) { return plan_of(a, sm_count).bytes; }
 
-void launch_paged_attend(const AttendArgs& a, int, cudaStream_t s)
+void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
 {
-  const auto grid = static_cast<unsigned>(a.n_rows * a.n_heads);
+  const Plan n = plan_of(a, sm_count);
+  Params p{};
+  p.keys            = a.cache.keys;
+  p.values          = a.cache.values;
+  p.k_page          = a.cache.key_strides[0];
+  p.k_token         = a.cache.key_strides[1];
+  p.k_head          = a.cache.key_strides[2];
+  p.v_page          = a.cache.value_strides[0];
+  p.v_token         = a.cache.value_strides[1];
+  p.v_head          = a.cache.value_strides[2];
+  p.n_places        = a.cache.n_pages * a.cache.page_size;
+  p.n_pages         = static_cast<int32_t>(a.cache.n_pages);
+  p.page_size       = static_cast<uint32_t>(a.cache.page_size);
+  p.dim             = static_cast<int32_t>(a.cache.head_dim);
+  p.fault           = a.cache.fault;
+  p.pages           = a.table.pages;
+  p.page_row        = a.table.row_stride;
+  p.n_sequences     = a.table.n_sequences;
+  p.most            = a.table.pages_per_sequence * a.cache.page_size;
+  p.row_to_sequence = a.table.row_to_sequence;
+  p.lengths         = a.lengths;
+  p.window          = a.window;
+  p.lists           = a.selected;
+  p.lists_64        = a.selected_64;
+  p.n_lists         = static_cast<int32_t>(a.n_lists);
+  p.k               = a.k;
+  p.q               = a.q.data;
+  p.q_row           = a.q.row_stride;
+  p.q_head          = a.q.head_stride;
+  p.out             = a.out.data;
+  p.o_row           = a.out.row_stride;
+  p.o_head          = a.out.head_stride;
+  p.lse             = a.lse;
+  p.n_rows          = a.n_rows;
+  p.n_heads         = static_cast<int32_t>(a.n_heads);
+  p.group           = static_cast<int32_t>(a.n_heads / a.cache.n_kv_heads);
+  p.subs            = n.subs;
+  p.per_unit        = n.per_unit;
+  p.units           = n.units;
+  p.scale           = a.scale * kLog2e;
+  p.direct          = n.direct;
+  p.workers         = static_cast<int32_t>(n.blocks);
+  p.part_floats     = n.part_floats;
+  p.parts           = static_cast<float*>(a.workspace);
+  p.marks           = n.direct ? nullptr : reinterpret_cast<int64_t*>(p.parts + 2 * n.blocks * n.part_floats);
   if (a.cache.dtype == kPagedF32) {
-    attend_kernel<float><<<grid, kThreads, 0, s>>>(a);
+    if (p.dim <= 64) {
+      launch_float<64>(p, n.blocks, s);
+    } else if (p.dim <= 128) {
+      launch_float<128>(p, n.blocks, s);
+    } else {
+      launch_float<256>(p, n.blocks, s);
+    }
+    if (!n.direct) { launch_join<float>(p, s); }
   } else if (a.cache.dtype == kPagedF16) {
-    attend_kernel<__half><<<grid, kThreads, 0, s>>>(a);
+    launch_half<__half>(p, n.blocks, s);
+    if (!n.direct) { launch_join<__half>(p, s); }
   } else {
-    attend_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+    launch_half<__nv_bfloat16>(p, n.blocks, s);
+    if (!n.direct) { launch_join<__nv_bfloat16>(p, s); }
   }
 }
 
