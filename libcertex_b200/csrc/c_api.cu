@@ -625,6 +625,7 @@ const certexB200PagedCache_t& checked_cache(const certexB200PagedCache_t* c)
   bool fine          = reinterpret_cast<uintptr_t>(c->keys) % 16 == 0 && reinterpret_cast<uintptr_t>(c->values) % 16 == 0;
   for (int i = 0; i < 3; ++i) { fine = fine && c->key_strides[i] * size % 16 == 0 && c->value_strides[i] * size % 16 == 0; }
   CERTEX_EXPECTS(fine, "certex: keys, values and the strides of a paged cache must be multiples of 16 bytes");
+  CERTEX_EXPECTS(paged_within_reach(*c), "certex: the strides of this cache are negative, or too fine for its size");
   return *c;
 }
 

@@ -43,6 +43,8 @@ struct AttendArgs {
   float* lse;              // [n_rows, n_heads] or null
   void* workspace;
 };
+/// Whether the kernels' 32-bit offsets, in units that the cache's strides are multiples of, reach all of the cache.
+bool paged_within_reach(const certexB200PagedCache_t& cache);
 size_t paged_attend_workspace(const AttendArgs& a, int sm_count);
 void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s);
 

@@ -18,11 +18,11 @@
 //    a cut divides leaves a partial result (m, l, output) per share, which a second, small kernel joins in the order of the
 //    shares: results do not depend on timing. It is launched while the first still runs and waits for it.
 //    Calls whose units are known to be short take a block per unit and one launch.
-//  * Loads are asynchronous copies (cp.async) into a ring of kStages tiles of kKeys keys that belongs to one warp: no
-//    barrier between warps until a unit ends. The table's entries for a tile are fetched one step before its copies.
+//  * A warp works by itself on tiles of 16 keys (every fourth of its block's): no barrier until a unit ends, and the loads of
+//    the next tile are in flight while one is computed. The table's entries for a tile are fetched one tile before its loads.
 //
-// Copies of rows that are not to be seen are zero-filled and their scores set to -infinity, so nothing that lies there (NaN,
-// infinity, another sequence's tokens) has an effect.
+// Rows that are not to be seen have scores of -infinity and values of zero, so nothing that lies there (NaN, infinity,
+// another sequence's tokens) has an effect.
 #include "paged.cuh"
 
 #include <cuda_bf16.h>
@@ -36,6 +36,7 @@ namespace {
 constexpr int kWarps   = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStep    = 64;  // tokens of a step of the work split
+constexpr int kLead    = 2;   // steps that a unit's beginning and end count for: fetching its first tiles, joining the warps
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2   = 0.6931471805599453f;
 
@@ -43,8 +44,12 @@ constexpr float kLn2   = 0.6931471805599453f;
 struct Params {
   const void* keys;
   const void* values;
-  int64_t k_page, k_token, k_head, v_page, v_token, v_head;  // elements
-  int64_t n_places;                                            // n_pages * page_size
+  // strides of pages and tokens in units of 2^unit_shift bytes, of heads in elements
+  uint32_t k_page, k_token, v_page, v_token;
+  int64_t k_head, v_head;
+  int32_t unit_shift;
+  int32_t page_shift;  // log2 of page_size, -1: no power of two
+  int64_t n_places;    // n_pages * page_size
   int32_t n_pages;
   uint32_t page_size;
   int32_t dim;
@@ -165,37 +170,40 @@ __device__ __forceinline__ Segment segment_of(const Params& p, int64_t row, cons
   return g;
 }
 
-/// Where token i of a segment lies: offsets of its key and value, or false.
-__device__ __forceinline__ bool place_of(const Params& p, const Segment& g, int64_t i, int64_t& k_at, int64_t& v_at)
+/// Where a key and its value lie, in units from the first key and value of their head; kNowhere for one that is not seen.
+struct Place {
+  uint32_t k, v;
+};
+constexpr uint32_t kNowhere = ~0u;
+
+/// The place of token i of a segment.
+__device__ __forceinline__ Place place_of(const Params& p, const Segment& g, int64_t i)
 {
-  int64_t page;
-  uint32_t place;
+  uint32_t page, place;
   if (p.lengths) {
-    const auto t    = static_cast<uint32_t>(g.begin + i);
-    const uint32_t n = t / p.page_size;
-    place           = t - n * p.page_size;
-    page            = g.pages[n];
-    if (page < 0 || page >= p.n_pages) {
+    const auto t = static_cast<uint32_t>(g.begin + i);
+    const uint32_t n = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+    place        = t - n * p.page_size;
+    page         = static_cast<uint32_t>(g.pages[n]);
+    if (page >= static_cast<uint32_t>(p.n_pages)) {  // negative entries too
       *p.fault = 1;
-      return false;
+      return {kNowhere, kNowhere};
     }
   } else {
     const int64_t at = p.lists_64 ? static_cast<const int64_t*>(g.list)[i] : static_cast<const int32_t*>(g.list)[i];
-    if (at < 0) { return false; }
+    if (at < 0) { return {kNowhere, kNowhere}; }
     if (at >= p.n_places) {
       *p.fault = 1;
-      return false;
+      return {kNowhere, kNowhere};
     }
-    if (at >> 32) {
-      page = at / p.page_size;
+    if (p.page_shift >= 0) {
+      page = static_cast<uint32_t>(at >> p.page_shift);
     } else {
-      page = static_cast<uint32_t>(at) / p.page_size;
+      page = at >> 32 ? static_cast<uint32_t>(at / p.page_size) : static_cast<uint32_t>(at) / p.page_size;
     }
-    place = static_cast<uint32_t>(at - page * p.page_size);
+    place = static_cast<uint32_t>(at) - page * p.page_size;
   }
-  k_at = page * p.k_page + place * p.k_token;
-  v_at = page * p.v_page + place * p.v_token;
-  return true;
+  return {page * p.k_page + place * p.k_token, page * p.v_page + place * p.v_token};
 }
 
 /// Calls body(segment) for this block's share of the work. A block of kThreads threads calls it as a whole.
@@ -225,8 +233,9 @@ __device__ __forceinline__ void for_segments(const Params& p, F&& body)
   }
 
   // how many steps there are in all: every block counts for itself
-  auto steps_of = [&](int64_t row) { return (span_of(p, row).count + kStep - 1) / kStep; };
-  const int64_t same = p.lengths ? 0 : (p.k + kStep - 1) / kStep;
+  auto steps_for = [&](int64_t count) { return count > 0 ? (count + kStep - 1) / kStep + kLead : 0; };
+  auto steps_of  = [&](int64_t row) { return steps_for(span_of(p, row).count); };
+  const int64_t same = p.lengths ? 0 : steps_for(p.k);
   int64_t total = 0, mine = 0;
   if (!p.lengths) {
     total = p.n_rows * same;
@@ -288,24 +297,27 @@ __device__ __forceinline__ void for_segments(const Params& p, F&& body)
 
   while (at < end) {
     const Span s        = span_of(p, row);
-    const int64_t steps = (s.count + kStep - 1) / kStep;
+    const int64_t steps = steps_for(s.count);
     if (steps == 0) {
       ++row;
       continue;
     }
-    const auto unit = static_cast<int>((at - base) / steps);
-    const int64_t u0 = base + unit * steps, u1 = u0 + steps, to = min(end, u1);
+    const auto unit  = static_cast<int>((at - base) / steps);
+    const int64_t u0 = base + unit * steps, to = min(end, u0 + steps);
     Segment g = segment_of(p, row, s, unit);
-    g.i0      = (at - u0) * kStep;
-    g.i1      = min(s.count, (to - u0) * kStep);
-    // a partial result that begins a unit belongs to the worker's second slot, one that goes on with it to the first
-    g.slot    = at == u0 && to == u1 ? -1 : 2 * w + (at > u0 ? 0 : 1);
-    if (threadIdx.x == 0) {
-      const int64_t id = row * p.units + unit;
-      if (at > u0) { p.marks[2 * w] = id; }
-      if (to < u1) { p.marks[2 * w + 1] = id; }
+    g.i0      = max(int64_t(0), at - u0 - kLead) * kStep;
+    g.i1      = min(s.count, max(int64_t(0), to - u0 - kLead) * kStep);
+    if (g.i0 < g.i1) {  // (a share may end within a unit's lead)
+      const bool begins = g.i0 == 0, ends = g.i1 == s.count;
+      // a partial result that begins a unit belongs to the worker's second slot, one that goes on with it to the first
+      g.slot = begins && ends ? -1 : 2 * w + (begins ? 1 : 0);
+      if (threadIdx.x == 0) {
+        const int64_t id = row * p.units + unit;
+        if (!begins) { p.marks[2 * w] = id; }
+        if (!ends) { p.marks[2 * w + 1] = id; }
+      }
+      body(g);
     }
-    body(g);
     at = to;
     if (at == base + steps * p.units) {
       base = at;
@@ -408,18 +420,339 @@ struct Half<__half> {
   }
 };
 
-/// D: the head dimension, padded to what the tiles are built for; NT: groups of eight queries.
-template <int D>
+/// What the block's warps found of a segment meets in shared memory (`sums`: a warp's [queries][D + 4] floats: output, m, l, seen;
+/// `pitch` floats between warps) and goes out. m is relative to weights that were raised by 2^raise.
+template <typename T, int D>
+__device__ __forceinline__ void finish_segment(const Params& p, const Segment& g, const float* sums, int pitch, float raise)
+{
+  constexpr int kRow = D + 4;
+  __syncthreads();
+  for (int i = 0; i < g.n_heads; ++i) {
+    float w[kWarps], top = -INFINITY, sum = 0.f, seen = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+      w[x] = sums[x * pitch + i * kRow + D];
+      top  = fmaxf(top, w[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+      const float* from = sums + x * pitch + i * kRow;
+      w[x]              = top == -INFINITY ? 1.f : exp2_fast(w[x] - top);
+      sum += w[x] * from[D + 1];
+      seen += from[D + 2];
+    }
+    const float scale = g.slot >= 0 ? 1.f : 1.f / sum;
+    for (int c = threadIdx.x; c < p.dim; c += kThreads) {
+      float v = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) { v += w[x] * sums[x * pitch + i * kRow + c]; }
+      put_out<T>(p, g, i, c, seen > 0.f ? v * scale : 0.f);
+    }
+    if (threadIdx.x == 0) { put_sums(p, g, i, top - raise, sum, seen > 0.f); }
+  }
+  __syncthreads();
+}
+
+/// The softmax of a tile's scores s (16 keys x 8 queries, as the first product leaves them), one group of eight queries:
+/// scores become weights as the second product's operand, m and l go on. Returns whether m grew (in this thread's queries).
+template <typename T>
+__device__ __forceinline__ bool soften(float (&s)[4], float scale, bool see0, bool see1, float (&m)[2], float (&l)[2], float (&alpha)[2],
+                                       uint32_t (&hi)[2], uint32_t (&lo)[2])
+{
+  float base[2];
+  bool grew = false;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    s[c]      = see0 ? s[c] * scale : -INFINITY;
+    s[c + 2]  = see1 ? s[c + 2] * scale : -INFINITY;
+    float top = fmaxf(s[c], s[c + 2]);
+    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+    top       = fmaxf(top, m[c]);
+    base[c]   = top == -INFINITY ? 0.f : top;
+    alpha[c]  = exp2_fast(m[c] - base[c]);
+    grew      = grew || top > m[c];
+    m[c]      = top;
+    base[c] -= Half<T>::kRaise;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) { s[c] = exp2_fast(s[c] - base[c & 1]); }
+  l[0] = l[0] * alpha[0] + (s[0] + s[2]);
+  l[1] = l[1] * alpha[1] + (s[1] + s[3]);
+  Half<T>::split(s[0], s[1], hi[0], lo[0]);
+  Half<T>::split(s[2], s[3], hi[1], lo[1]);
+  // from keys by lanes to queries by lanes
+  hi[0] = transpose8x8(hi[0]), hi[1] = transpose8x8(hi[1]);
+  lo[0] = transpose8x8(lo[0]), lo[1] = transpose8x8(lo[1]);
+  return grew;
+}
+
+/// The sum over the lanes that hold different keys of the same query.
+__device__ __forceinline__ float sum_over_keys(float v)
+{
+  v += __shfl_xor_sync(~0u, v, 4);
+  v += __shfl_xor_sync(~0u, v, 8);
+  return v + __shfl_xor_sync(~0u, v, 16);
+}
+
+// Heads of up to 128 coordinates: operands come straight from global memory into the registers of the product that uses
+// them. A product over coordinates may take them in any order, as long as keys and queries agree, so lane t of a
+// key's four lanes takes 16 bytes in a row for two steps of the product; and the second product's rows, the
+// coordinates of the result, may be any eight coordinates, so lane g of a value's eight lanes takes 16 bytes in a row for
+// four products. What is left is to pair the values of neighbouring keys, one byte permutation per register.
+// Against copies into shared memory and ldmatrix this takes 250 instructions per tile instead of 470.
+
+/// N * 4 bytes that are read once.
+template <int N>
+__device__ __forceinline__ void read_once(uint32_t (&r)[N], const char* at)
+{
+  static_assert(N == 1 || N == 2 || N == 4, "");
+  if constexpr (N == 4) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(at));
+  } else if constexpr (N == 2) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(at));
+  } else {
+    asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(r[0]) : "l"(at));
+  }
+}
+
+/// A lane's share of a row's coordinates in blocks: 8 * E coordinates where every lane of eight (or 4 * E, of four) takes E.
+template <int N64, int N32, int N16>
+struct RowPart {
+  uint32_t b64[N64 ? N64 : 1][4], b32[N32 ? N32 : 1][2], b16[N16 ? N16 : 1][1];
+};
+
+template <typename T, int D, int NT, bool PAD>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attend_direct_kernel(const Params p)
+{
+  constexpr int kK32 = D / 32, kK16 = D % 32 / 16;                  // keys: blocks of 32 and 16 coordinates
+  constexpr int kV64 = D / 64, kV32 = D % 64 / 32, kV16 = D % 32 / 16;  // values: of 64, 32 and 16
+  constexpr int kSteps = 2 * kK32 + kK16, kTiles = 4 * kV64 + 2 * kV32 + kV16;
+  extern __shared__ __align__(16) float sums[];  // [warps][8 NT][D + 4]
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  for_segments<T>(p, [&](const Segment& g) {
+    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(T) + t4 * 16;
+    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(T) + g8 * 16;
+    const int tiles    = static_cast<int>((g.i1 - g.i0 + 15) / 16);
+    const int n        = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+
+    // where key lane % 16 of tile j lies
+    auto look_up = [&](int j) {
+      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * 16 + lane % 16;
+      return j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
+    };
+    Place now = look_up(0), next = look_up(1);
+
+    // the queries, as the 8-column side of the first product
+    uint32_t qf[NT][kSteps][2];
+    {
+      const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        const int i  = x * 8 + g8;
+        const T* row = q + i * p.q_head;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c = k < 2 * kK32 ? k / 2 * 32 + t4 * 8 + k % 2 * 4 + h * 2 : kK32 * 32 + t4 * 4 + h * 2;
+            uint32_t v  = 0;
+            if (i < g.n_heads && (!PAD || c < p.dim)) {
+              const auto a = *reinterpret_cast<const uint16_t*>(row + c), b = *reinterpret_cast<const uint16_t*>(row + c + 1);
+              v            = a | (uint32_t(b) << 16);
+            }
+            qf[x][k][h] = v;
+          }
+        }
+      }
+    }
+    float o[NT][kTiles][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) { o[x][d][0] = o[x][d][1] = o[x][d][2] = o[x][d][3] = 0.f; }
+      m[x][0] = m[x][1] = -INFINITY;
+      l[x][0] = l[x][1] = 0.f;
+    }
+
+    uint32_t kr[2][kK32 + kK16][4];  // keys g8 and g8 + 8
+    RowPart<kV64, kV32, kV16> vr[4];  // values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+    auto at_of = [&](uint32_t place) { return static_cast<uint64_t>(place == kNowhere ? 0 : place) << p.unit_shift; };
+    auto load_keys = [&](const uint32_t (&place)[2]) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const char* at = keys + at_of(place[r]);
+#pragma unroll
+        for (int b = 0; b < kK32; ++b) {
+          if (!PAD || b * 32 + t4 * 8 < p.dim) { read_once<4>(kr[r][b], at + b * 64); }
+        }
+        if constexpr (kK16 > 0) {
+          uint32_t two[2];
+          read_once<2>(two, at + kK32 * 64 - t4 * 8);
+          kr[r][kK32][0] = two[0], kr[r][kK32][1] = two[1];
+        }
+      }
+    };
+    auto load_values = [&](const uint32_t (&place)[4]) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const char* at = values + at_of(place[r]);
+#pragma unroll
+        for (int b = 0; b < kV64; ++b) {
+          if (!PAD || b * 64 + g8 * 8 < p.dim) { read_once<4>(vr[r].b64[b], at + b * 128); }
+        }
+        if constexpr (kV32 > 0) { read_once<2>(vr[r].b32[0], at + kV64 * 128 - g8 * 8); }
+        if constexpr (kV16 > 0) { read_once<1>(vr[r].b16[0], at + kV64 * 128 + kV32 * 64 - g8 * 12); }
+      }
+    };
+    auto keys_of = [&](const Place& x, uint32_t (&place)[2]) {
+      place[0] = __shfl_sync(~0u, x.k, g8);
+      place[1] = __shfl_sync(~0u, x.k, g8 + 8);
+    };
+    auto values_of = [&](const Place& x, uint32_t (&place)[4]) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) { place[r] = __shfl_sync(~0u, x.v, t4 * 2 + (r & 1) + (r & 2) * 4); }
+    };
+    // a register of two neighbouring keys' values at one coordinate
+    auto pair = [](uint32_t a, uint32_t b, int odd) { return __byte_perm(a, b, odd ? 0x7632 : 0x5410); };
+
+    if (PAD) {
+      // what lies behind the last coordinate is never loaded, and must be a number
+#pragma unroll
+      for (int b = 0; b < kK32; ++b) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) { kr[0][b][x] = kr[1][b][x] = 0; }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int b = 0; b < kV64; ++b) { vr[r].b64[b][0] = vr[r].b64[b][1] = vr[r].b64[b][2] = vr[r].b64[b][3] = 0; }
+      }
+    }
+    uint32_t kp[2], vp[4];
+    bool any = false;
+    if (n > 0) {
+      keys_of(now, kp);
+      values_of(now, vp);
+      load_keys(kp);
+      load_values(vp);
+    }
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      float s[NT][4];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) { s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f; }
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int b = k / 2, h = k % 2 * 2;
+        const uint32_t a[4] = {kr[0][b][h], kr[1][b][h], kr[0][b][h + 1], kr[1][b][h + 1]};
+#pragma unroll
+        for (int x = 0; x < NT; ++x) { Half<T>::mma(s[x], a, qf[x][k][0], qf[x][k][1]); }
+      }
+      const bool see0 = kp[0] != kNowhere, see1 = kp[1] != kNowhere;
+      any             = any || see0 || see1;
+      // every key of the tile is seen, or the values of those that are not become zeros
+      const bool full = __all_sync(~0u, see0 && see1);
+      if (!full) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (vp[r] == kNowhere) {
+#pragma unroll
+            for (int b = 0; b < kV64; ++b) { vr[r].b64[b][0] = vr[r].b64[b][1] = vr[r].b64[b][2] = vr[r].b64[b][3] = 0; }
+            vr[r].b32[0][0] = vr[r].b32[0][1] = vr[r].b16[0][0] = 0;
+          }
+        }
+      }
+      if (j + 1 < n) {
+        keys_of(next, kp);
+        load_keys(kp);
+      }
+      values_of(next, vp);
+      next = look_up(j + 2);
+
+      uint32_t hi[NT][2], lo[NT][2];
+      float alpha[NT][2];
+      bool grew = false;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) { grew |= soften<T>(s[x], p.scale, see0, see1, m[x], l[x], alpha[x], hi[x], lo[x]); }
+      if (__any_sync(~0u, grew)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d) {
+            o[x][d][0] *= alpha[x][0], o[x][d][1] *= alpha[x][1];
+            o[x][d][2] *= alpha[x][0], o[x][d][3] *= alpha[x][1];
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) {
+        uint32_t a[4];
+        if (d < 4 * kV64) {
+          const int b = d / 4, i = d % 4, h = i % 2;
+          a[0] = pair(vr[0].b64[b][i / 2], vr[1].b64[b][i / 2], h), a[1] = pair(vr[0].b64[b][i / 2 + 2], vr[1].b64[b][i / 2 + 2], h);
+          a[2] = pair(vr[2].b64[b][i / 2], vr[3].b64[b][i / 2], h), a[3] = pair(vr[2].b64[b][i / 2 + 2], vr[3].b64[b][i / 2 + 2], h);
+        } else if (d < 4 * kV64 + 2 * kV32) {
+          const int h = d % 2;
+          a[0] = pair(vr[0].b32[0][0], vr[1].b32[0][0], h), a[1] = pair(vr[0].b32[0][1], vr[1].b32[0][1], h);
+          a[2] = pair(vr[2].b32[0][0], vr[3].b32[0][0], h), a[3] = pair(vr[2].b32[0][1], vr[3].b32[0][1], h);
+        } else {
+          a[0] = pair(vr[0].b16[0][0], vr[1].b16[0][0], 0), a[1] = pair(vr[0].b16[0][0], vr[1].b16[0][0], 1);
+          a[2] = pair(vr[2].b16[0][0], vr[3].b16[0][0], 0), a[3] = pair(vr[2].b16[0][0], vr[3].b16[0][0], 1);
+        }
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          Half<T>::mma(o[x][d], a, hi[x][0], hi[x][1]);
+          Half<T>::mma(o[x][d], a, lo[x][0], lo[x][1]);
+        }
+      }
+      if (j + 1 < n) { load_values(vp); }
+    }
+
+    constexpr int kRow = D + 4, kPitch = 8 * NT * kRow;
+    any = __any_sync(~0u, any);
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float* to = sums + warp * kPitch + (x * 8 + t4 * 2 + c) * kRow;
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+          // the coordinates of rows g8 and g8 + 8 of product d
+          int at, step;
+          if (d < 4 * kV64) {
+            at = d / 4 * 64 + g8 * 8 + d % 4, step = 4;
+          } else if (d < 4 * kV64 + 2 * kV32) {
+            at = kV64 * 64 + g8 * 4 + d % 2, step = 2;
+          } else {
+            at = kV64 * 64 + kV32 * 32 + g8 * 2, step = 1;
+          }
+          to[at]        = o[x][d][c];
+          to[at + step] = o[x][d][c + 2];
+        }
+        const float sum = sum_over_keys(l[x][c]);
+        if (g8 == 0) { to[D] = m[x][c], to[D + 1] = sum, to[D + 2] = any ? 1.f : 0.f; }
+      }
+    }
+    finish_segment<T, D>(p, g, sums, kPitch, Half<T>::kRaise);
+  });
+}
+
+// Wider heads do not fit the registers that way: their tiles are copied into a ring in shared memory that belongs to a warp.
+template <int D>  // the head dimension, padded to what the tiles are built for
 struct HalfTile {
   static constexpr int kPitch = D * 2 + 16;  // bytes of a row in shared memory: eight rows start in eight different banks
   static constexpr int kBytes = kKeys * kPitch;
   static constexpr int kWarp  = kStages * 2 * kBytes;
   static constexpr int kAll   = kWarps * kWarp;
-  static constexpr int kLanes = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes that copy a row
+  static constexpr int kLanes = 32;           // lanes that copy a row
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attend_half_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads) attend_ring_kernel(const Params p)
 {
   using Tile = HalfTile<D>;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -466,17 +799,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attend_half_kernel
       l[n][0] = l[n][1] = 0.f;
     }
 
-    const T* keys   = static_cast<const T*>(p.keys) + g.kv * p.k_head;
-    const T* values = static_cast<const T*>(p.values) + g.kv * p.v_head;
+    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(T);
+    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(T);
     // tiles of this warp: warp, warp + kWarps, ...
     const int tiles = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
     const int n     = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
     // the place of key lane % 16 of the next tile to be copied
-    int64_t k_at = 0, v_at = 0;
-    bool real    = false;
+    Place at{kNowhere, kNowhere};
     auto look_up = [&](int j) {
       const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
-      real            = j < n && i < g.i1 && place_of(p, g, i, k_at, v_at);
+      at              = j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
     };
     uint32_t masks = 0;  // of the tiles in the ring: which keys are real, newest lowest
     uint32_t older = 0;
@@ -487,16 +819,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attend_half_kernel
       const bool inside = chunk * 8 < p.dim;
 #pragma unroll
       for (int r = 0; r < kKeys; r += kRows) {
-        const int row    = r + sub;
-        const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
-        const bool ok    = __shfl_sync(~0u, real, row);
+        const int row     = r + sub;
+        const uint32_t ka = __shfl_sync(~0u, at.k, row), va = __shfl_sync(~0u, at.v, row);
+        const bool ok     = ka != kNowhere;
         if (inside) {
-          copy16(to + row * Tile::kPitch, ok ? keys + ka + chunk * 8 : keys, ok);
-          copy16(to + Tile::kBytes + row * Tile::kPitch, ok ? values + va + chunk * 8 : values, ok);
+          copy16(to + row * Tile::kPitch, keys + (ok ? static_cast<uint64_t>(ka) << p.unit_shift : 0) + chunk * 16, ok);
+          copy16(to + Tile::kBytes + row * Tile::kPitch, values + (ok ? static_cast<uint64_t>(va) << p.unit_shift : 0) + chunk * 16, ok);
         }
       }
       older = masks >> 16;
-      masks = (masks << 16) | (__ballot_sync(~0u, real) & 0xffffu);
+      masks = (masks << 16) | (__ballot_sync(~0u, at.k != kNowhere) & 0xffffu);
     };
     bool any = false;
     look_up(0);
@@ -534,31 +866,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attend_half_kernel
       bool grew = false;
       float alpha[NT][2];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float base[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          s[i][c]     = see0 ? s[i][c] * p.scale : -INFINITY;
-          s[i][c + 2] = see1 ? s[i][c + 2] * p.scale : -INFINITY;
-          float top   = fmaxf(s[i][c], s[i][c + 2]);
-          top         = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-          top         = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-          top         = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-          top         = fmaxf(top, m[i][c]);
-          base[c]     = top == -INFINITY ? 0.f : top;
-          alpha[i][c] = exp2_fast(m[i][c] - base[c]);
-          grew        = grew || top > m[i][c];
-          m[i][c]     = top;
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) { s[i][c] = exp2_fast(s[i][c] - base[c & 1] + Half<T>::kRaise); }
-        l[i][0] = l[i][0] * alpha[i][0] + (s[i][0] + s[i][2]);
-        l[i][1] = l[i][1] * alpha[i][1] + (s[i][1] + s[i][3]);
-        Half<T>::split(s[i][0], s[i][1], hi[i][0], lo[i][0]);
-        Half<T>::split(s[i][2], s[i][3], hi[i][1], lo[i][1]);
-        hi[i][0] = transpose8x8(hi[i][0]), hi[i][1] = transpose8x8(hi[i][1]);
-        lo[i][0] = transpose8x8(lo[i][0]), lo[i][1] = transpose8x8(lo[i][1]);
-      }
+      for (int i = 0; i < NT; ++i) { grew |= soften<T>(s[i], p.scale, see0, see1, m[i], l[i], alpha[i], hi[i], lo[i]); }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -596,38 +904,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1) attend_half_kernel
           to[d * 16 + g8]     = o[i][d][c];
           to[d * 16 + g8 + 8] = o[i][d][c + 2];
         }
-        float sum = l[i][c];
-        sum += __shfl_xor_sync(~0u, sum, 4);
-        sum += __shfl_xor_sync(~0u, sum, 8);
-        sum += __shfl_xor_sync(~0u, sum, 16);
+        const float sum = sum_over_keys(l[i][c]);
         if (g8 == 0) { to[D] = m[i][c], to[D + 1] = sum, to[D + 2] = any ? 1.f : 0.f; }
       }
     }
-    __syncthreads();
-    for (int i = 0; i < g.n_heads; ++i) {
-      float w[kWarps], top = -INFINITY, sum = 0.f, seen = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        w[x] = reinterpret_cast<float*>(smem + x * Tile::kWarp)[i * kRow + D];
-        top  = fmaxf(top, w[x]);
-      }
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float* from = reinterpret_cast<float*>(smem + x * Tile::kWarp) + i * kRow;
-        w[x]              = top == -INFINITY ? 1.f : exp2_fast(w[x] - top);
-        sum += w[x] * from[D + 1];
-        seen += from[D + 2];
-      }
-      const float scale = g.slot >= 0 ? 1.f : seen > 0.f ? 1.f / sum : 0.f;
-      for (int c = threadIdx.x; c < p.dim; c += kThreads) {
-        float v = 0.f;
-#pragma unroll
-        for (int x = 0; x < kWarps; ++x) { v += w[x] * reinterpret_cast<float*>(smem + x * Tile::kWarp)[i * kRow + c]; }
-        put_out<T>(p, g, i, c, seen > 0.f ? v * scale : 0.f);
-      }
-      if (threadIdx.x == 0) { put_sums(p, g, i, top - Half<T>::kRaise, sum, seen > 0.f); }
-    }
-    __syncthreads();
+    finish_segment<T, D>(p, g, reinterpret_cast<const float*>(smem), Tile::kWarp / 4, Half<T>::kRaise);
     if (p.dim < D) {
       for (int i = lane * 16; i < Tile::kWarp; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
       __syncwarp();
@@ -695,15 +976,14 @@ __global__ void __launch_bounds__(kThreads) attend_float_kernel(const Params p)
 #pragma unroll
       for (int c = 0; c < kCols; ++c) { o[i][c] = 0.f; }
     }
-    const float* keys   = static_cast<const float*>(p.keys) + g.kv * p.k_head;
-    const float* values = static_cast<const float*>(p.values) + g.kv * p.v_head;
-    const int tiles     = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
+    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(float);
+    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(float);
+    const int tiles    = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
     const int n         = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-    int64_t k_at = 0, v_at = 0;
-    bool real    = false;
+    Place at{kNowhere, kNowhere};
     auto look_up = [&](int j) {
       const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
-      real            = j < n && i < g.i1 && place_of(p, g, i, k_at, v_at);
+      at              = j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
     };
     uint32_t masks[kStages];
 #pragma unroll
@@ -713,22 +993,22 @@ __global__ void __launch_bounds__(kThreads) attend_float_kernel(const Params p)
       const int sub = lane / kLanes;
 #pragma unroll
       for (int r = 0; r < kKeys; r += kRows) {
-        const int row    = r + sub;
-        const int64_t ka = __shfl_sync(~0u, k_at, row), va = __shfl_sync(~0u, v_at, row);
-        const bool ok    = __shfl_sync(~0u, real, row);
+        const int row     = r + sub;
+        const uint32_t ka = __shfl_sync(~0u, at.k, row), va = __shfl_sync(~0u, at.v, row);
+        const bool ok     = ka != kNowhere;
 #pragma unroll
         for (int x = 0; x < kTimes; ++x) {
           const int chunk = lane % kLanes + x * kLanes;
           if (chunk * 4 < p.dim) {
             const uint32_t to = ring_at + stage * 2 * Tile::kBytes + row * Tile::kPitch + chunk * 16;
-            copy16(to, ok ? keys + ka + chunk * 4 : keys, ok);
-            copy16(to + Tile::kBytes, ok ? values + va + chunk * 4 : values, ok);
+            copy16(to, keys + (ok ? static_cast<uint64_t>(ka) << p.unit_shift : 0) + chunk * 16, ok);
+            copy16(to + Tile::kBytes, values + (ok ? static_cast<uint64_t>(va) << p.unit_shift : 0) + chunk * 16, ok);
           }
         }
       }
 #pragma unroll
       for (int i = kStages - 1; i > 0; --i) { masks[i] = masks[i - 1]; }
-      masks[0] = __ballot_sync(~0u, real);
+      masks[0] = __ballot_sync(~0u, at.k != kNowhere);
     };
     bool any = false;
     look_up(0);
@@ -825,32 +1105,7 @@ __global__ void __launch_bounds__(kThreads) attend_float_kernel(const Params p)
       for (int x = 1; x < 32; x <<= 1) { sum += __shfl_xor_sync(~0u, sum, x); }
       if (lane == 0) { sums[i * kRow + D] = m[i], sums[i * kRow + D + 1] = sum, sums[i * kRow + D + 2] = any ? 1.f : 0.f; }
     }
-    __syncthreads();
-    constexpr int kStride = FloatShared<D, Q>::kWarp;
-    for (int i = 0; i < g.n_heads; ++i) {
-      float w[kWarps], top = -INFINITY, sum = 0.f, seen = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        w[x] = reinterpret_cast<float*>(smem + x * kStride)[i * kRow + D];
-        top  = fmaxf(top, w[x]);
-      }
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float* from = reinterpret_cast<float*>(smem + x * kStride) + i * kRow;
-        w[x]              = top == -INFINITY ? 1.f : exp2_fast(w[x] - top);
-        sum += w[x] * from[D + 1];
-        seen += from[D + 2];
-      }
-      const float scale = g.slot >= 0 ? 1.f : seen > 0.f ? 1.f / sum : 0.f;
-      for (int c = threadIdx.x; c < p.dim; c += kThreads) {
-        float v = 0.f;
-#pragma unroll
-        for (int x = 0; x < kWarps; ++x) { v += w[x] * reinterpret_cast<float*>(smem + x * kStride)[i * kRow + c]; }
-        put_out<float>(p, g, i, c, seen > 0.f ? v * scale : 0.f);
-      }
-      if (threadIdx.x == 0) { put_sums(p, g, i, top, sum, seen > 0.f); }
-    }
-    __syncthreads();
+    finish_segment<float, D>(p, g, reinterpret_cast<const float*>(smem), FloatShared<D, Q>::kWarp / 4, 0.f);
     clear();
   });
 }
@@ -939,11 +1194,21 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   if (a.n_lists == 0 && a.window > 0) { most = std::min(most, a.window); }
   const int64_t units = a.n_rows * n.units;
   n.direct            = most <= kDirectTokens;
-  const int resident  = sm_count * (half && dim <= 128 ? 2 : !half && dim <= 64 ? 2 : 1);
-  n.blocks            = n.direct ? units : std::min<int64_t>(resident, units * ((most + kStep - 1) / kStep));
+  const int resident  = sm_count * (half ? (dim > 128 ? 1 : n.per_unit <= 8 ? 3 : 2) : dim <= 64 ? 2 : 1);
+  n.blocks            = n.direct ? units : std::min<int64_t>(resident, units * ((most + kStep - 1) / kStep + kLead));
   n.part_floats       = n.per_unit * (dim + 4);
   n.bytes             = n.direct ? 0 : static_cast<size_t>(n.blocks) * 2 * (8 + sizeof(float) * n.part_floats);
   return n;
+}
+
+/// The largest power of two that divides the strides of pages and tokens in bytes: with 256-byte rows, 32 bits of them reach
+/// 1 TB.
+int unit_shift(const certexB200PagedCache_t& c)
+{
+  const int size = paged_type_size(static_cast<int>(c.dtype));
+  uint64_t all   = 0;
+  for (int i = 0; i < 2; ++i) { all |= static_cast<uint64_t>(c.key_strides[i] * size) | static_cast<uint64_t>(c.value_strides[i] * size); }
+  return all == 0 ? 4 : __builtin_ctzll(all);
 }
 
 template <typename Kernel>
@@ -953,29 +1218,44 @@ void launch(Kernel kernel, int smem, const Params& p, int64_t blocks, cudaStream
   kernel<<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(p);
 }
 
+template <typename T, int D, bool PAD>
+void launch_direct(const Params& p, int64_t blocks, cudaStream_t s)
+{
+  constexpr int kSums = kWarps * 8 * (D + 4) * 4;
+  if (p.per_unit <= 8) {
+    launch(attend_direct_kernel<T, D, 1, PAD>, kSums, p, blocks, s);
+  } else {
+    launch(attend_direct_kernel<T, D, 2, PAD>, 2 * kSums, p, blocks, s);
+  }
+}
+
 template <typename T, int D>
-void launch_half(const Params& p, int64_t blocks, cudaStream_t s)
+void launch_ring(const Params& p, int64_t blocks, cudaStream_t s)
 {
   if (p.per_unit <= 8) {
-    launch(attend_half_kernel<T, D, 1>, HalfTile<D>::kAll, p, blocks, s);
+    launch(attend_ring_kernel<T, D, 1>, HalfTile<D>::kAll, p, blocks, s);
   } else {
-    launch(attend_half_kernel<T, D, 2>, HalfTile<D>::kAll, p, blocks, s);
+    launch(attend_ring_kernel<T, D, 2>, HalfTile<D>::kAll, p, blocks, s);
   }
 }
 
 template <typename T>
 void launch_half(const Params& p, int64_t blocks, cudaStream_t s)
 {
-  if (p.dim <= 64) {
-    launch_half<T, 64>(p, blocks, s);
-  } else if (p.dim <= 96) {
-    launch_half<T, 96>(p, blocks, s);
-  } else if (p.dim <= 128) {
-    launch_half<T, 128>(p, blocks, s);
+  switch (p.dim) {
+    case 64: return launch_direct<T, 64, false>(p, blocks, s);
+    case 80: return launch_direct<T, 80, false>(p, blocks, s);
+    case 96: return launch_direct<T, 96, false>(p, blocks, s);
+    case 128: return launch_direct<T, 128, false>(p, blocks, s);
+  }
+  if (p.dim < 64) {
+    launch_direct<T, 64, true>(p, blocks, s);
+  } else if (p.dim < 128) {
+    launch_direct<T, 128, true>(p, blocks, s);
   } else if (p.dim <= 192) {
-    launch_half<T, 192>(p, blocks, s);
+    launch_ring<T, 192>(p, blocks, s);
   } else {
-    launch_half<T, 256>(p, blocks, s);
+    launch_ring<T, 256>(p, blocks, s);
   }
 }
 
@@ -1009,6 +1289,18 @@ void launch_join(const Params& p, cudaStream_t s)
 
 }  // namespace
 
+bool paged_within_reach(const certexB200PagedCache_t& c)
+{
+  const int size  = paged_type_size(static_cast<int>(c.dtype));
+  const int shift = unit_shift(c);
+  for (const int64_t* s : {c.key_strides, c.value_strides}) {
+    if (s[0] < 0 || s[1] < 0) { return false; }
+    const double far = static_cast<double>(c.n_pages - 1) * s[0] + static_cast<double>(c.page_size - 1) * s[1];
+    if (far * size / (1ull << shift) >= 4294967295.0) { return false; }
+  }
+  return true;
+}
+
 size_t paged_attend_workspace(const AttendArgs& a, int sm_count) { return plan_of(a, sm_count).bytes; }
 
 void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
@@ -1017,15 +1309,20 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   Params p{};
   p.keys            = a.cache.keys;
   p.values          = a.cache.values;
-  p.k_page          = a.cache.key_strides[0];
-  p.k_token         = a.cache.key_strides[1];
+  p.unit_shift      = unit_shift(a.cache);
+  auto units        = [&](int64_t stride) {
+    return static_cast<uint32_t>(stride * paged_type_size(static_cast<int>(a.cache.dtype)) >> p.unit_shift);
+  };
+  p.k_page          = units(a.cache.key_strides[0]);
+  p.k_token         = units(a.cache.key_strides[1]);
   p.k_head          = a.cache.key_strides[2];
-  p.v_page          = a.cache.value_strides[0];
-  p.v_token         = a.cache.value_strides[1];
+  p.v_page          = units(a.cache.value_strides[0]);
+  p.v_token         = units(a.cache.value_strides[1]);
   p.v_head          = a.cache.value_strides[2];
   p.n_places        = a.cache.n_pages * a.cache.page_size;
   p.n_pages         = static_cast<int32_t>(a.cache.n_pages);
   p.page_size       = static_cast<uint32_t>(a.cache.page_size);
+  p.page_shift      = (a.cache.page_size & (a.cache.page_size - 1)) == 0 ? __builtin_ctzll(a.cache.page_size) : -1;
   p.dim             = static_cast<int32_t>(a.cache.head_dim);
   p.fault           = a.cache.fault;
   p.pages           = a.table.pages;
