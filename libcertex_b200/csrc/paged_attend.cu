@@ -77,7 +77,7 @@ struct Params {
   // the split
   int32_t direct;    // a block per unit
   int32_t workers;
-  int64_t* marks;    // [workers][2]: the unit that a worker goes on with, the one that it leaves unfinished (-1: none)
+  int64_t* marks;    // [workers][2]: a unit that a worker begins and leaves unfinished, and the shares that it has (0: none)
   float* parts;      // [workers][2] partial results of part_floats each
   int32_t part_floats;
 };
@@ -259,7 +259,7 @@ __device__ __forceinline__ void for_segments(const Params& p, F&& body)
   }
   total *= p.units;
   const int64_t workers = min(int64_t(p.workers), total), w = blockIdx.x;
-  if (threadIdx.x == 0) { p.marks[2 * w] = p.marks[2 * w + 1] = -1; }
+  if (threadIdx.x == 0) { p.marks[2 * w + 1] = 0; }
   if (w >= workers) { return; }
   int64_t at        = total * w / workers;
   const int64_t end = total * (w + 1) / workers;
@@ -311,10 +311,10 @@ __device__ __forceinline__ void for_segments(const Params& p, F&& body)
       const bool begins = g.i0 == 0, ends = g.i1 == s.count;
       // a partial result that begins a unit belongs to the worker's second slot, one that goes on with it to the first
       g.slot = begins && ends ? -1 : 2 * w + (begins ? 1 : 0);
-      if (threadIdx.x == 0) {
-        const int64_t id = row * p.units + unit;
-        if (!begins) { p.marks[2 * w] = id; }
-        if (!ends) { p.marks[2 * w + 1] = id; }
+      if (begins && !ends && threadIdx.x == 0) {
+        // step x is in the share of worker ((x + 1) * workers - 1) / total
+        p.marks[2 * w]     = row * p.units + unit;
+        p.marks[2 * w + 1] = ((u0 + steps) * workers - 1) / total - w + 1;
       }
       body(g);
     }
@@ -1112,57 +1112,67 @@ __global__ void __launch_bounds__(kThreads) attend_float_kernel(const Params p)
 
 // ------------------------------------------------------------------------------------------------ joining the shares
 // Block (w, i): if worker w left a unit unfinished that it had begun, joins that unit's partial results for query i. They lie in
-// w's second slot and in the first slots of the workers behind it that went on with the unit.
+// w's second slot and in the first slots of the workers behind it. A chain of three reads (mark, sums, outputs) is all its time,
+// so every thread reads at once what it needs: one share's sums, then four coordinates of every eighth share.
 constexpr int kJoinThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
 {
   extern __shared__ float weight[];  // [workers]
-  __shared__ float red[2][kJoinThreads / 32];
+  __shared__ float red[3][kJoinThreads / 32];
+  __shared__ float4 outs[kJoinThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int w = blockIdx.x, i = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t id = p.marks[2 * w + 1];
-  if (id < 0 || p.marks[2 * w] == id) { return; }
+  const int64_t id = p.marks[2 * w];
+  const int n      = static_cast<int>(p.marks[2 * w + 1]);
+  if (n == 0) { return; }
   const int64_t row = id / p.units;
   const Segment g   = segment_of(p, row, Span{0, 0, 0}, static_cast<int>(id - row * p.units));
   if (i >= g.n_heads) { return; }
-  int n = 1;
-  for (int x0 = w + 1;; x0 += kJoinThreads) {
-    const int x     = x0 + static_cast<int>(threadIdx.x);
-    const int count = __syncthreads_count(x < p.workers && p.marks[2 * x] == id);
-    n += count;
-    if (count < kJoinThreads) { break; }
-  }
   auto part = [&](int x) { return p.parts + (x == 0 ? 2 * int64_t(w) + 1 : 2 * int64_t(w + x)) * p.part_floats; };
+  // the largest m of all, then the weights, the sum and whether anything was seen
   float top = -INFINITY;
-  for (int x = threadIdx.x; x < n; x += kJoinThreads) { top = fmaxf(top, part(x)[4 * i]); }
+  for (int x = threadIdx.x; x < n; x += kJoinThreads) {
+    weight[x] = part(x)[4 * i];
+    top       = fmaxf(top, weight[x]);
+  }
   for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, o)); }
   if (lane == 0) { red[0][warp] = top; }
   __syncthreads();
   for (float r : red[0]) { top = fmaxf(top, r); }
-  __syncthreads();
   float sum = 0.f, seen = 0.f;
   for (int x = threadIdx.x; x < n; x += kJoinThreads) {
     const float* from = part(x) + 4 * i;
-    const float f     = top == -INFINITY ? 1.f : exp2_fast(from[0] - top);
-    weight[x]         = f;
-    sum += f * from[1];
+    weight[x]         = top == -INFINITY ? 1.f : exp2_fast(weight[x] - top);
+    sum += weight[x] * from[1];
     seen += from[2];
   }
   for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(~0u, sum, o);
     seen += __shfl_xor_sync(~0u, seen, o);
   }
-  if (lane == 0) { red[0][warp] = sum, red[1][warp] = seen; }
+  if (lane == 0) { red[1][warp] = sum, red[2][warp] = seen; }
   __syncthreads();
   sum = seen = 0.f;
-  for (int x = 0; x < kJoinThreads / 32; ++x) { sum += red[0][x], seen += red[1][x]; }
-  for (int c = threadIdx.x; c < p.dim; c += kJoinThreads) {
-    float v = 0.f;
+  for (int x = 0; x < kJoinThreads / 32; ++x) { sum += red[1][x], seen += red[2][x]; }
+  const int lanes = p.dim <= 128 ? 32 : 64, groups = kJoinThreads / lanes;
+  const int c = threadIdx.x % lanes * 4, first = threadIdx.x / lanes;
+  float4 v{0.f, 0.f, 0.f, 0.f};
+  if (c < p.dim) {
 #pragma unroll 8
-    for (int x = 0; x < n; ++x) { v += weight[x] * part(x)[4 * p.per_unit + i * p.dim + c]; }
-    (static_cast<T*>(p.out) + row * p.o_row + (g.head + i) * p.o_head)[c] = Type<T>::down(seen > 0.f ? v / sum : 0.f);
+    for (int x = first; x < n; x += groups) {
+      const float4 o = *reinterpret_cast<const float4*>(part(x) + 4 * p.per_unit + i * p.dim + c);
+      const float f  = weight[x];
+      v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
+    }
+  }
+  outs[threadIdx.x] = v;
+  __syncthreads();
+  for (int x = threadIdx.x; x < p.dim; x += kJoinThreads) {
+    float r = 0.f;
+    for (int y = 0; y < groups; ++y) { r += reinterpret_cast<const float*>(outs + y * lanes)[x]; }
+    (static_cast<T*>(p.out) + row * p.o_row + (g.head + i) * p.o_head)[x] = Type<T>::down(seen > 0.f ? r / sum : 0.f);
   }
   if (p.lse && threadIdx.x == 0) { p.lse[row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
 }
