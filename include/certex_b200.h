@@ -392,9 +392,10 @@ CERTEX_B200_EXPORT cuvsError_t certexB200PagedAppend(cuvsResources_t res, const 
                                                      int64_t n_q_heads, const void* positions, int32_t positions_64);
 
 /** Bytes of device memory that an attention of these sizes wants as its workspace (16-byte aligned; it belongs to one call at
- *  a time). n_lists: 0 for certexB200PagedAttend; k: its pages_per_sequence * page_size, or the length of a list. */
+ *  a time). n_lists: 0 for certexB200PagedAttend, with k = its pages_per_sequence * page_size; else k is the length of a list
+ *  and window 0. */
 CERTEX_B200_EXPORT cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedCache_t* cache, int64_t n_rows,
-                                                        int64_t n_heads, int64_t n_lists, int64_t k, size_t* bytes);
+                                                        int64_t n_heads, int64_t n_lists, int64_t k, int64_t window, size_t* bytes);
 
 /** out[i, h] = the values that row i sees, weighed by the softmax of scale * <q[i, h], key> over KV head h / (n_heads /
  *  n_kv_heads). Row i sees the first lengths[i] tokens of its sequence, of those the last `window` if window > 0; a row that

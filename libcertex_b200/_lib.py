@@ -206,7 +206,7 @@ def lib():
                 i32, f32, sz = ctypes.c_int32, ctypes.c_float, ctypes.c_size_t
                 L.certexB200Rotate.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, vp, i32, i32]
                 L.certexB200PagedAppend.argtypes = [vp] * 8 + [i64, i64, vp, i32]
-                L.certexB200PagedWorkspace.argtypes = [vp, vp, i64, i64, i64, i64, P(sz)]
+                L.certexB200PagedWorkspace.argtypes = [vp, vp, i64, i64, i64, i64, i64, P(sz)]
                 L.certexB200PagedAttend.argtypes = [vp, vp, vp, vp, i64, vp, vp, i64, i64, f32, vp, vp, sz]
                 L.certexB200PagedAttendSelected.argtypes = [vp, vp, vp, i32, i64, i64, vp, vp, i64, i64, f32, vp, vp, sz]
                 L.certexB200ScreenTrace.argtypes = [vp, ctypes.c_int32]
@@ -256,16 +256,25 @@ class Tensor:
         return ctypes.byref(self.m)
 
 
-def resources():
-    """The resources handle of the calling thread for the current CUDA device, bound to torch's current stream."""
-    dev = torch.cuda.current_device()
-    cache = getattr(_tls, "res", None)
-    if cache is None:
-        cache = _tls.res = {}
-    if dev not in cache:
+try:
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # what current_stream() asks, without an object around the answer
+except AttributeError:
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
+
+
+def resources(dev=None):
+    """The resources handle of the calling thread for the current CUDA device (`dev`, where the caller knows it), bound to
+    torch's current stream."""
+    if dev is None:
+        dev = torch.cuda.current_device()
+    try:
+        h = _tls.res[dev]
+    except (AttributeError, KeyError):
+        if getattr(_tls, "res", None) is None:
+            _tls.res = {}
         h = ctypes.c_void_p()
         check(lib().cuvsResourcesCreate(ctypes.byref(h)))
-        cache[dev] = h
-    h = cache[dev]
-    check(lib().cuvsStreamSet(h, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        _tls.res[dev] = h
+    check(_lib.cuvsStreamSet(h, _raw_stream(dev)))
     return h

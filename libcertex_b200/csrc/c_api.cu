@@ -711,10 +711,10 @@ cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCach
 }
 
 cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedCache_t* cache, int64_t n_rows, int64_t n_heads,
-                                     int64_t n_lists, int64_t k, size_t* bytes)
+                                     int64_t n_lists, int64_t k, int64_t window, size_t* bytes)
 {
   return translate([=] {
-    CERTEX_EXPECTS(bytes != nullptr && n_rows >= 0 && n_lists >= 0 && k >= 0, "certex: null argument");
+    CERTEX_EXPECTS(bytes != nullptr && n_rows >= 0 && n_lists >= 0 && k >= 0 && window >= 0, "certex: null argument");
     AttendArgs a{};
     a.cache = checked_cache(cache);
     CERTEX_EXPECTS(n_heads >= 1 && n_heads % a.cache.n_kv_heads == 0, "certex: the query heads must be a multiple of the KV heads");
@@ -722,6 +722,7 @@ cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedC
     a.n_heads                  = n_heads;
     a.n_lists                  = n_lists;
     a.k                        = k;
+    a.window                   = window;
     a.table.pages_per_sequence = n_lists > 0 ? 0 : (k + a.cache.page_size - 1) / a.cache.page_size;
     *bytes                     = n_rows > 0 ? paged_attend_workspace(a, as_res(res).sm_count) : 0;
   });

@@ -1224,7 +1224,7 @@ int unit_shift(const certexB200PagedCache_t& c)
 template <typename Kernel>
 void launch(Kernel kernel, int smem, const Params& p, int64_t blocks, cudaStream_t s)
 {
-  if (smem > 32 * 1024) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
+  if (smem > 40 * 1024) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
   kernel<<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(p);
 }
 

@@ -24,23 +24,28 @@
 namespace certex_b200 {
 namespace {
 
-template <typename T>
-struct Convert;
-template <>
-struct Convert<float> {
-  static __device__ float up(float v) { return v; }
-  static __device__ float down(float v) { return v; }
-};
-template <>
-struct Convert<__half> {
-  static __device__ float up(__half v) { return __half2float(v); }
-  static __device__ __half down(float v) { return __float2half_rn(v); }
-};
-template <>
-struct Convert<__nv_bfloat16> {
-  static __device__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-  static __device__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
-};
+/// Two neighbouring 16-bit values as floats and back, and single ones.
+__device__ __forceinline__ float2 up2(uint32_t w, __half)
+{
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 up2(uint32_t w, __nv_bfloat16) { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
+__device__ __forceinline__ uint32_t down2(float x, float y, __half)
+{
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t down2(float x, float y, __nv_bfloat16)
+{
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float up(float v) { return v; }
+__device__ __forceinline__ float up(__half v) { return __half2float(v); }
+__device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float down(float v, float) { return v; }
+__device__ __forceinline__ __half down(float v, __half) { return __float2half_rn(v); }
+__device__ __forceinline__ __nv_bfloat16 down(float v, __nv_bfloat16) { return __float2bfloat16_rn(v); }
 
 /// V elements that move as one access (V * sizeof(T) is 16, or V is 1).
 template <typename T, int V>
@@ -92,16 +97,50 @@ __device__ __forceinline__ void turn_sincos(uint64_t turn, float& s, float& c)
   }
 }
 
+/// The V pairs of a unit's vectors x and y turned by (c, s): pair i is (x[i], y[i]), or when interleaved the elements 2i and
+/// 2i + 1 of both vectors in a row.
+template <typename T, int V, bool INTERLEAVED>
+__device__ __forceinline__ void turn_unit(Pack<T, V>& x, Pack<T, V>& y, const float (&c)[V], const float (&s)[V])
+{
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    auto* xw = reinterpret_cast<uint32_t*>(&x);
+    auto* yw = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 u = up2(xw[i], T{}), w = up2(yw[i], T{});
+      if constexpr (INTERLEAVED) {
+        constexpr int H = V / 2;
+        xw[i] = down2(u.x * c[i] - u.y * s[i], u.y * c[i] + u.x * s[i], T{});
+        yw[i] = down2(w.x * c[H + i] - w.y * s[H + i], w.y * c[H + i] + w.x * s[H + i], T{});
+      } else {
+        xw[i] = down2(u.x * c[2 * i] - w.x * s[2 * i], u.y * c[2 * i + 1] - w.y * s[2 * i + 1], T{});
+        yw[i] = down2(w.x * c[2 * i] + u.x * s[2 * i], w.y * c[2 * i + 1] + u.y * s[2 * i + 1], T{});
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      T& e0 = INTERLEAVED ? (2 * i < V ? x.e[(2 * i) % V] : y.e[(2 * i) % V]) : x.e[i];
+      T& e1 = INTERLEAVED ? (2 * i + 1 < V ? x.e[(2 * i + 1) % V] : y.e[(2 * i + 1) % V]) : y.e[i];
+      const float u = up(e0), w = up(e1);
+      e0 = down(u * c[i] - w * s[i], T{});
+      e1 = down(w * c[i] + u * s[i], T{});
+    }
+  }
+}
+
+// Four blocks of 256 threads on an SM with two heads' 64 bytes in flight per thread: 64 KB in flight. With four heads in flight
+// in 159 registers there was room for one block, and turning 32 768 rows of 32 heads took 143 us.
 template <typename T, int V, bool INTERLEAVED, int HEADS>
-__global__ void __launch_bounds__(256) turn_rows_kernel(const TurnArgs<T> a)
+__global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
 {
   constexpr bool kExact = sizeof(T) == 4;
   const int units       = a.dim / (2 * V);  // of a head
   int chunks            = 0;
   for (int i = 0; i < a.n_sec; ++i) { chunks += a.sec[i].chunks; }
   const int64_t item = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t per  = int64_t(chunks) * units;
-  const int64_t row  = item / per;
+  const int per      = chunks * units;
+  const int64_t row  = item >> 31 ? item / per : static_cast<uint32_t>(item) / static_cast<uint32_t>(per);
   if (row >= a.n_rows) { return; }
   const int in_row = static_cast<int>(item - row * per);
   int chunk        = in_row / units;
@@ -148,35 +187,27 @@ __global__ void __launch_bounds__(256) turn_rows_kernel(const TurnArgs<T> a)
   const T* from     = sec.src + row * sec.src_row + int64_t(first) * sec.src_head;
   T* dst            = sec.dst + to + int64_t(first) * sec.dst_head;
   const int n       = min(HEADS, sec.heads - first);
-  constexpr int kAt = HEADS < 4 ? HEADS : 4;  // heads whose loads are in flight together
+  constexpr int kAt = HEADS < 2 ? HEADS : 2;  // heads whose loads are in flight together
 #pragma unroll 1
-  for (int h0 = 0; h0 < n; h0 += kAt) {
+  for (int h = 0; h < n; h += kAt) {
     P x[kAt], y[kAt];
 #pragma unroll
     for (int j = 0; j < kAt; ++j) {
-      if (h0 + j < n) {
-        x[j] = *reinterpret_cast<const P*>(from + (h0 + j) * sec.src_head + lo);
-        y[j] = *reinterpret_cast<const P*>(from + (h0 + j) * sec.src_head + hi);
+      if (h + j < n) {
+        x[j] = *reinterpret_cast<const P*>(from + j * sec.src_head + lo);
+        y[j] = *reinterpret_cast<const P*>(from + j * sec.src_head + hi);
       }
     }
 #pragma unroll
     for (int j = 0; j < kAt; ++j) {
-      if (h0 + j < n) {
-        if (turn) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            // pair i: (x[i], y[i]), or when interleaved the elements 2i and 2i + 1 of both vectors in a row
-            T& e0 = INTERLEAVED ? (2 * i < V ? x[j].e[(2 * i) % V] : y[j].e[(2 * i) % V]) : x[j].e[i];
-            T& e1 = INTERLEAVED ? (2 * i + 1 < V ? x[j].e[(2 * i + 1) % V] : y[j].e[(2 * i + 1) % V]) : y[j].e[i];
-            const float u = Convert<T>::up(e0), w = Convert<T>::up(e1);
-            e0 = Convert<T>::down(u * c[i] - w * s[i]);
-            e1 = Convert<T>::down(w * c[i] + u * s[i]);
-          }
-        }
-        *reinterpret_cast<P*>(dst + (h0 + j) * sec.dst_head + lo) = x[j];
-        *reinterpret_cast<P*>(dst + (h0 + j) * sec.dst_head + hi) = y[j];
+      if (h + j < n) {
+        if (turn) { turn_unit<T, V, INTERLEAVED>(x[j], y[j], c, s); }
+        *reinterpret_cast<P*>(dst + j * sec.dst_head + lo) = x[j];
+        *reinterpret_cast<P*>(dst + j * sec.dst_head + hi) = y[j];
       }
     }
+    from += kAt * sec.src_head;
+    dst += kAt * sec.dst_head;
   }
 }
 

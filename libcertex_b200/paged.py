@@ -36,11 +36,18 @@ _MOST_DIM = 256
 _TURN = Fraction("6.283185307179586476925286766559005768394")
 
 
+def _fail(message):
+    raise ValueError(message)
+
+
+# The checks below stand in front of kernels of a few microseconds: messages are made only when one fails.
 def _check_rows(x, what, heads=None, dim=None):
     """A CUDA tensor (n, heads, dim) whose last axis is dense, as the kernels read it."""
-    _need(isinstance(x, torch.Tensor) and x.is_cuda, f"{what} must be a CUDA tensor")
-    _need(x.ndim == 3 and (heads is None or x.shape[1] == heads) and (dim is None or x.shape[2] == dim),
-          f"{what} must have shape (n, {heads or 'heads'}, {dim or 'head_dim'}), not {tuple(x.shape)}")
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        _fail(f"{what} must be a CUDA tensor")
+    shape = x.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
+        _fail(f"{what} must have shape (n, {heads or 'heads'}, {dim or 'head_dim'}), not {tuple(shape)}")
     if x.is_neg():
         x = x.resolve_neg()
     return x if x.stride(2) == 1 else x.contiguous()
@@ -48,15 +55,23 @@ def _check_rows(x, what, heads=None, dim=None):
 
 def _check_index(t, what, shape, device, wide=False):
     """An index tensor of this shape: int32 (or int64 if `wide`), dense."""
-    _need(isinstance(t, torch.Tensor) and t.device == device, f"{what} must be a tensor on {device}")
-    _need(t.dtype is torch.int32 or (wide and t.dtype is torch.int64),
-          f"{what} must be {'int32 or int64' if wide else 'int32'}, not {t.dtype}")
-    _need(t.shape == shape, f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        _fail(f"{what} must be a tensor on {device}")
+    if t.dtype is not torch.int32 and not (wide and t.dtype is torch.int64):
+        _fail(f"{what} must be {'int32 or int64' if wide else 'int32'}, not {t.dtype}")
+    if t.shape != shape:
+        _fail(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _new_like(x):
+    """A dense tensor of x's shape."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _packed(x):
-    return _ROWS.pack(x.data_ptr(), x.stride(0), x.stride(1))
+    s = x.stride()
+    return _ROWS.pack(x.data_ptr(), s[0], s[1])
 
 
 def _span(x):
@@ -79,15 +94,22 @@ def _check_out(out, x, in_place):
 
 
 def _no_gradient(*tensors):
-    _need(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors),
-          "no gradient flows through a paged cache: call it under torch.no_grad()")
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            _fail("no gradient flows through a paged cache: call it under torch.no_grad()")
+
+
+try:
+    _current_device = torch._C._cuda_getDevice  # torch.cuda.current_device() without asking whether CUDA is initialised
+except AttributeError:
+    _current_device = torch.cuda.current_device
 
 
 def _on_device(method):
     """Runs a call with the device of its first tensor current: kernels, streams and handles are the current device's."""
 
     def call(self, x, *args, **kwargs):
-        if isinstance(x, torch.Tensor) and x.is_cuda and x.device.index != torch.cuda.current_device():
+        if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() != _current_device():
             with torch.cuda.device(x.device):
                 return method(self, x, *args, **kwargs)
         return method(self, x, *args, **kwargs)
@@ -148,6 +170,8 @@ class Rotary:
         # what one position adds to an angle, as a fraction of a turn in units of 2**-64
         turns = [round(Fraction(f) / _TURN * 2**64) % 2**64 for f in w]
         self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device=device)
+        self.device = self._turns.device
+        self._index = self._turns.get_device()
         self._plan = _ROTARY.pack(self._turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.magnitude)
 
     @_on_device
@@ -155,19 +179,21 @@ class Rotary:
         """x (n, heads, head_dim) float32, float16 or bfloat16, its rows turned by positions (n,) int32 or int64, which may be
         negative; inverse=True turns back. Differentiable in x. out: where to write, x itself allowed; without a gradient."""
         x = _check_rows(x, "x", dim=self.head_dim)
-        _need(x.dtype in _KIND, f"rows are float32, float16 or bfloat16, not {x.dtype}")
-        _need(x.device == self._turns.device, f"this rotation lives on {self._turns.device}, the rows on {x.device}")
+        if x.dtype not in _KIND:
+            _fail(f"rows are float32, float16 or bfloat16, not {x.dtype}")
+        if x.device != self.device:
+            _fail(f"this rotation lives on {self.device}, the rows on {x.device}")
         positions = _check_index(positions, "positions", (x.shape[0],), x.device, wide=True)
-        if torch.is_grad_enabled() and x.requires_grad:
+        if x.requires_grad and torch.is_grad_enabled():
             _need(out is None, "out takes no gradient: call without it, or under torch.no_grad()")
             return _Turn.apply(x, positions, self, bool(inverse))
         return self._turn(x, positions, inverse, out)
 
     def _turn(self, x, positions, inverse, out):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else _check_out(out, x, True)
+        y = _new_like(x) if out is None else _check_out(out, x, True)
         n, heads, dim = x.shape
         if n and heads:
-            L.check(L.lib().certexB200Rotate(L.resources(), self._plan, _packed(x), _packed(y), n, heads, dim, _KIND[x.dtype],
+            L.check(L.lib().certexB200Rotate(L.resources(self._index), self._plan, _packed(x), _packed(y), n, heads, dim, _KIND[x.dtype],
                                              positions.data_ptr(), positions.dtype is torch.int64, bool(inverse)))
         return y
 
@@ -234,6 +260,8 @@ class PagedCache:
         for t in (keys, values):
             _need(t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s * size % 16 == 0 for s in t.stride()[:3]),
                   "keys and values need a dense last axis and strides of whole 16 bytes")
+        self._index = keys.get_device()
+        self._needs = {}  # sizes of a call -> bytes of its workspace
         self._fault = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._args = _CACHE.pack(keys.data_ptr(), values.data_ptr(),
                                  *(t.stride(i) for t in (keys, values) for i in (0, token, head)), self.n_pages,
@@ -248,21 +276,24 @@ class PagedCache:
 
     def _rows(self, x, what, heads=None):
         x = _check_rows(x, what, heads, self.head_dim)
-        _need(x.dtype is self.dtype and x.device == self.device,
-              f"{what} must be {self.dtype} on {self.device} like the cache, not {x.dtype} on {x.device}")
+        if x.dtype is not self.dtype or x.device != self.device:
+            _fail(f"{what} must be {self.dtype} on {self.device} like the cache, not {x.dtype} on {x.device}")
         return x
 
     def _table(self, page_table, row_to_batch, n):
-        _need(isinstance(page_table, torch.Tensor) and page_table.device == self.device and page_table.dtype is torch.int32
-              and page_table.ndim == 2, f"the page table must be an int32 tensor (sequences, pages) on {self.device}")
+        if (not isinstance(page_table, torch.Tensor) or page_table.device != self.device or page_table.dtype is not torch.int32
+                or page_table.ndim != 2):
+            _fail(f"the page table must be an int32 tensor (sequences, pages) on {self.device}")
         if page_table.stride(1) != 1:
             page_table = page_table.contiguous()
+        sequences, pages = page_table.shape
+        rows = 0
         if row_to_batch is not None:
             row_to_batch = _check_index(row_to_batch, "row_to_batch", (n,), self.device)
-        else:
-            _need(page_table.shape[0] == n, f"{n} rows and a table of {page_table.shape[0]} sequences: give row_to_batch")
-        rows = 0 if row_to_batch is None else row_to_batch.data_ptr()
-        args = _TABLE.pack(page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], rows)
+            rows = row_to_batch.data_ptr()
+        elif sequences != n:
+            _fail(f"{n} rows and a table of {sequences} sequences: give row_to_batch")
+        args = _TABLE.pack(page_table.data_ptr(), page_table.stride(0), sequences, pages, rows)
         return args, (page_table, row_to_batch)  # what must live until the launch
 
     @_on_device
@@ -274,20 +305,22 @@ class PagedCache:
         _no_gradient(k, v, q)
         k, v = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
         n = k.shape[0]
-        _need(v.shape[0] == n, f"{n} keys and {v.shape[0]} values")
+        if v.shape[0] != n:
+            _fail(f"{n} keys and {v.shape[0]} values")
         positions = _check_index(positions, "positions", (n,), self.device, wide=True)
         table, alive = self._table(page_table, row_to_batch, n)
         heads, q_in, q_to, turned = 0, None, None, None
         if q is not None:
             _need(self.rotary is not None, "queries come along to be turned, but this cache has no rotation")
             q = self._rows(q, "q")
-            _need(q.shape[0] == n, f"{n} keys and {q.shape[0]} queries")
-            turned = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            if q.shape[0] != n:
+                _fail(f"{n} keys and {q.shape[0]} queries")
+            turned = _new_like(q)
             heads = q.shape[1]
             if heads:
                 q_in, q_to = _packed(q), _packed(turned)
         if n:
-            L.check(L.lib().certexB200PagedAppend(L.resources(), self._args, self.rotary._plan if self.rotary else None, table,
+            L.check(L.lib().certexB200PagedAppend(L.resources(self._index), self._args, self.rotary._plan if self.rotary else None, table,
                                                   _packed(k), _packed(v), q_in, q_to, n, heads, positions.data_ptr(),
                                                   positions.dtype is torch.int64))
         return turned
@@ -297,19 +330,30 @@ class PagedCache:
         _no_gradient(q)
         q = self._rows(q, "q")
         n, heads, dim = q.shape
-        _need(heads >= 1 and heads % self.n_kv_heads == 0, f"{heads} query heads are no multiple of {self.n_kv_heads} KV heads")
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else _check_out(out, q, False)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        if heads < 1 or heads % self.n_kv_heads:
+            _fail(f"{heads} query heads are no multiple of {self.n_kv_heads} KV heads")
+        out = _new_like(q) if out is None else _check_out(out, q, False)
+        lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
         scale = dim ** -0.5 if scale is None else float(scale)
-        _need(math.isfinite(scale), "the scale must be finite")
+        if not math.isfinite(scale):
+            _fail("the scale must be finite")
         return q, out, lse, scale
 
-    def _workspace(self, n, heads, lists, k):
-        """Memory for the partial results of one call: of the stream's allocator, so that calls on other streams and in
-        captured graphs have their own."""
-        need = L.ctypes.c_size_t()
-        L.check(L.lib().certexB200PagedWorkspace(L.resources(), self._args, n, heads, lists, k, L.ctypes.byref(need)))
-        return torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
+    def _workspace(self, n, heads, lists, k, window):
+        """(tensor or None, its address, its bytes): memory for the partial results of one call, of the stream's allocator, so
+        that calls on other streams and in captured graphs have their own."""
+        sizes = (n, heads, lists, k, window)
+        need = self._needs.get(sizes)
+        if need is None:
+            size = L.ctypes.c_size_t()
+            L.check(L.lib().certexB200PagedWorkspace(L.resources(), self._args, *sizes, L.ctypes.byref(size)))
+            if len(self._needs) > 1000:
+                self._needs.clear()
+            need = self._needs[sizes] = size.value
+        if not need:
+            return None, None, 0
+        w = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return w, w.data_ptr(), need
 
     @_on_device
     def attend(self, q, page_table, lengths, row_to_batch=None, scale=None, window=None, return_lse=False, out=None):
@@ -320,15 +364,16 @@ class PagedCache:
         one sequence (drafted tokens) name it in row_to_batch and have their own lengths."""
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
-        _need(window is None or window >= 1, "window must be positive")
+        if window is None:
+            window = 0
+        elif window < 1:
+            _fail("window must be positive")
         lengths = _check_index(lengths, "lengths", (n,), self.device)
         table, alive = self._table(page_table, row_to_batch, n)
         if n:
-            w = self._workspace(n, heads, 0, page_table.shape[1] * self.page_size)
-            L.check(L.lib().certexB200PagedAttend(L.resources(), self._args, table, lengths.data_ptr(), int(window or 0),
-                                                  _packed(q), _packed(out), n, heads, scale,
-                                                  None if lse is None else lse.data_ptr(), None if w is None else w.data_ptr(),
-                                                  0 if w is None else w.numel()))
+            w, at, size = self._workspace(n, heads, 0, page_table.shape[1] * self.page_size, window)
+            L.check(L.lib().certexB200PagedAttend(L.resources(self._index), self._args, table, lengths.data_ptr(), window, _packed(q),
+                                                  _packed(out), n, heads, scale, None if lse is None else lse.data_ptr(), at, size))
         return (out, lse) if return_lse else out
 
     @_on_device
@@ -338,15 +383,14 @@ class PagedCache:
         negative ones are left out, one that is named twice counts twice."""
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
-        _need(isinstance(selected, torch.Tensor) and selected.ndim == 3 and selected.shape[0] == n
-              and selected.shape[1] in (heads, self.n_kv_heads, 1),
-              f"selected must have shape ({n}, {heads}, k), ({n}, {self.n_kv_heads}, k) or ({n}, 1, k)")
+        if (not isinstance(selected, torch.Tensor) or selected.ndim != 3 or selected.shape[0] != n
+                or selected.shape[1] not in (heads, self.n_kv_heads, 1)):
+            _fail(f"selected must have shape ({n}, {heads}, k), ({n}, {self.n_kv_heads}, k) or ({n}, 1, k)")
         selected = _check_index(selected, "selected", selected.shape, self.device, wide=True)
         lists, k = selected.shape[1:]
         if n:
-            w = self._workspace(n, heads, lists, k)
-            L.check(L.lib().certexB200PagedAttendSelected(L.resources(), self._args, selected.data_ptr(),
+            w, at, size = self._workspace(n, heads, lists, k, 0)
+            L.check(L.lib().certexB200PagedAttendSelected(L.resources(self._index), self._args, selected.data_ptr(),
                                                           selected.dtype is torch.int64, lists, k, _packed(q), _packed(out), n,
-                                                          heads, scale, None if lse is None else lse.data_ptr(),
-                                                          None if w is None else w.data_ptr(), 0 if w is None else w.numel()))
+                                                          heads, scale, None if lse is None else lse.data_ptr(), at, size))
         return (out, lse) if return_lse else out

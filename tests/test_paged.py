@@ -138,7 +138,7 @@ def test_the_library_refuses_what_it_cannot_read(built_library):
         assert call() == 0 and text in L.cuvsGetLastErrorText(), (text, L.cuvsGetLastErrorText())
     assert attend(n=0) == 1 and append(n=0) == 1 and rotate(n=0) == 1  # nothing to do needs nothing
     need = ctypes.c_size_t()
-    assert L.certexB200PagedWorkspace(None, _cache_args(dim=9), 1, 1, 0, 1, ctypes.byref(need)) == 0
+    assert L.certexB200PagedWorkspace(None, _cache_args(dim=9), 1, 1, 0, 1, 0, ctypes.byref(need)) == 0
 
 
 def test_packed_structures_have_the_headers_sizes(built_library, tmp_path):
@@ -190,7 +190,7 @@ def test_refusals():
     q.requires_grad_(False)
     lib, need = _lib.lib(), ctypes.c_size_t()
     big = torch.zeros((1, 4096), dtype=torch.int32, device="cuda")
-    _lib.check(lib.certexB200PagedWorkspace(_lib.resources(), cache._args, 1, 4, 0, 8192, ctypes.byref(need)))
+    _lib.check(lib.certexB200PagedWorkspace(_lib.resources(), cache._args, 1, 4, 0, 8192, 0, ctypes.byref(need)))
     if need.value:  # a workspace that is too small
         table = paged._TABLE.pack(big.data_ptr(), 4096, 1, 4096, 0)
         rows = paged._packed(q)
