@@ -917,196 +917,268 @@ __global__ void __launch_bounds__(kThreads) attend_ring_kernel(const Params p)
 }
 
 // ------------------------------------------------------------------------------------------------ float32
-// No tensor core keeps float32's products, so this is fused multiply-adds: a lane (or two, or four) per key for the scores, with
-// the queries broadcast from shared memory, then a lane per four coordinates for the sum over values.
-template <int D>
-struct FloatTile {
-  static constexpr int kKeys  = D <= 128 ? 16 : 8;
-  static constexpr int kParts = 32 / kKeys;  // lanes of a key
-  static constexpr int kPitch = D * 4 + 16;
-  static constexpr int kBytes = kKeys * kPitch;
-  static constexpr int kStages = 3;
-  static constexpr int kRing  = kStages * 2 * kBytes;
-  static constexpr int kCols  = D / 32;      // coordinates of a lane
-};
-
-/// Q: queries of a unit that the kernel is built for.
-template <int D, int Q>
-struct FloatShared {
-  static constexpr int kWarp = FloatTile<D>::kRing + Q * FloatTile<D>::kKeys * 4;  // ring, weights [Q][keys]
-  static constexpr int kAll  = kWarps * kWarp + Q * D * 4;                         // and the queries [Q][D]
-};
-
-template <int N>
-struct alignas(N < 4 ? N * 4 : 16) Floats {
-  float e[N];
-};
-
-template <int D, int Q>
-__global__ void __launch_bounds__(kThreads) attend_float_kernel(const Params p)
+// No tensor core keeps float32's products, so this is fused multiply-adds, two at a time (fma.f32x2). Keys lie in registers like
+// above, four lanes per key with 16 bytes in a row each; the queries come from shared memory, one read for both keys of a lane.
+// The four lanes' parts of a score are added while the queries are dealt out to them. For the second product a lane owns four
+// coordinates of every value, and the weights come from shared memory. 830 instructions per tile of 16 KB (8 queries, d = 128).
+__device__ __forceinline__ void fma2(float2& d, float2 a, float2 b)
 {
-  using Tile          = FloatTile<D>;
-  constexpr int kKeys = Tile::kKeys, kStages = Tile::kStages, kCols = Tile::kCols;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  unsigned char* ring    = smem + warp * FloatShared<D, Q>::kWarp;
-  const uint32_t ring_at = smem_of(ring);
-  auto* weights          = reinterpret_cast<float*>(ring + Tile::kRing);
-  auto* q_s              = reinterpret_cast<float*>(smem + kWarps * FloatShared<D, Q>::kWarp);
+  auto& x = reinterpret_cast<unsigned long long&>(d);
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(x) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+}
+
+template <int D, int Q>
+struct FloatTile {
+  static constexpr int kPer    = D <= 128 ? 2 : 1;      // keys of a lane
+  static constexpr int kKeys   = 8 * kPer;              // of a tile
+  static constexpr int kChunks = D / 16;                // 16-byte parts of a key that a lane holds
+  static constexpr int kRows   = D <= 64 ? 2 : 1;       // values that the warp reads at once
+  static constexpr int kWide   = D <= 128 ? 1 : D / 128;  // 16-byte parts of a value that a lane holds
+  static constexpr int kOwn    = Q >= 4 ? Q / 4 : 1;    // queries whose softmax a lane does
+  static constexpr int kWeights = 2 * Q * kKeys + (Q < 4 ? 4 : Q);  // floats of a warp: weights, twice each for fma2, and factors
+  static constexpr int kSums   = Q * (D + 4);           // of a warp: what it found
+  static constexpr int kBytes  = 4 * (Q * D + kWarps * (kWeights + kSums));
+};
+
+/// D: the head dimension, padded; Q: queries of a unit, padded to 1, 4 or 8.
+template <int D, int Q>
+__global__ void __launch_bounds__(kThreads, 2) attend_float_kernel(const Params p)
+{
+  using Tile = FloatTile<D, Q>;
+  constexpr int kPer = Tile::kPer, kKeys = Tile::kKeys, kChunks = Tile::kChunks, kRows = Tile::kRows, kWide = Tile::kWide, kOwn = Tile::kOwn;
+  extern __shared__ __align__(16) float shared[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
+  float* q_s     = shared;                                            // [Q][D]
+  float* weights = q_s + Q * D + warp * Tile::kWeights;               // [Q][keys][2]
+  float* factors = weights + 2 * Q * kKeys;                           // [Q]
+  float* sums    = q_s + Q * D + kWarps * Tile::kWeights;             // [warps][Q][D + 4]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  auto clear = [&] {
-    if (p.dim < D) {
-      for (int i = lane * 16; i < Tile::kRing; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
-      __syncwarp();
-    }
-  };
-  clear();
 
   for_segments<float>(p, [&](const Segment& g) {
+    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(float) + t4 * 16;
+    const int column   = D <= 64 ? lane % 16 * 4 : lane * 4;  // the lane's first coordinate of a value
+    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(float) + column * 4;
+    const int tiles    = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
+    const int n        = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+    auto look_up       = [&](int j) {
+      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
+      return j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
+    };
+    Place now = look_up(0), next = look_up(1);
     const float* q = static_cast<const float*>(p.q) + g.row * p.q_row + g.head * p.q_head;
     for (int i = threadIdx.x; i < Q * D; i += kThreads) {
       const int x = i / D, c = i % D;
       q_s[i] = x < g.n_heads && c < p.dim ? q[x * p.q_head + c] : 0.f;
     }
     __syncthreads();
-    float o[Q][kCols], m[Q], l[Q];
+
+    float4 kr[kPer][kChunks], vr[kKeys / kRows][kWide];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) { kr[x][c] = float4{0.f, 0.f, 0.f, 0.f}; }
+    }
+#pragma unroll
+    for (int x = 0; x < kKeys / kRows; ++x) {
+#pragma unroll
+      for (int c = 0; c < kWide; ++c) { vr[x][c] = float4{0.f, 0.f, 0.f, 0.f}; }
+    }
+    auto at_of     = [&](uint32_t place) { return static_cast<uint64_t>(place == kNowhere ? 0 : place) << p.unit_shift; };
+    auto load_keys = [&](const Place& at) {
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        const char* from = keys + at_of(__shfl_sync(~0u, at.k, g8 + 8 * x));
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          if (c * 16 + t4 * 4 < p.dim) { read_once<4>(reinterpret_cast<uint32_t(&)[4]>(kr[x][c]), from + c * 64); }
+        }
+      }
+    };
+    auto load_values = [&](const Place& at) {
+#pragma unroll
+      for (int x = 0; x < kKeys / kRows; ++x) {
+        const char* from = values + at_of(__shfl_sync(~0u, at.v, x * kRows + (kRows == 2 ? lane / 16 : 0)));
+#pragma unroll
+        for (int c = 0; c < kWide; ++c) {
+          if (column + c * 128 < p.dim) { read_once<4>(reinterpret_cast<uint32_t(&)[4]>(vr[x][c]), from + c * 512); }
+        }
+      }
+    };
+
+    float2 o[Q][kWide][2];
+    float m[kOwn], l[kOwn];
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-      m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) { o[i][c] = 0.f; }
+      for (int c = 0; c < kWide; ++c) { o[i][c][0] = o[i][c][1] = float2{0.f, 0.f}; }
     }
-    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(float);
-    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(float);
-    const int tiles    = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
-    const int n         = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-    Place at{kNowhere, kNowhere};
-    auto look_up = [&](int j) {
-      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
-      at              = j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
-    };
-    uint32_t masks[kStages];
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) { masks[i] = 0; }
-    auto copy = [&](int stage) {
-      constexpr int kLanes = D / 4 < 32 ? D / 4 : 32, kRows = 32 / kLanes, kTimes = D / 4 / kLanes;
-      const int sub = lane / kLanes;
-#pragma unroll
-      for (int r = 0; r < kKeys; r += kRows) {
-        const int row     = r + sub;
-        const uint32_t ka = __shfl_sync(~0u, at.k, row), va = __shfl_sync(~0u, at.v, row);
-        const bool ok     = ka != kNowhere;
-#pragma unroll
-        for (int x = 0; x < kTimes; ++x) {
-          const int chunk = lane % kLanes + x * kLanes;
-          if (chunk * 4 < p.dim) {
-            const uint32_t to = ring_at + stage * 2 * Tile::kBytes + row * Tile::kPitch + chunk * 16;
-            copy16(to, keys + (ok ? static_cast<uint64_t>(ka) << p.unit_shift : 0) + chunk * 16, ok);
-            copy16(to + Tile::kBytes, values + (ok ? static_cast<uint64_t>(va) << p.unit_shift : 0) + chunk * 16, ok);
-          }
-        }
-      }
-#pragma unroll
-      for (int i = kStages - 1; i > 0; --i) { masks[i] = masks[i - 1]; }
-      masks[0] = __ballot_sync(~0u, at.k != kNowhere);
-    };
+    for (int i = 0; i < kOwn; ++i) { m[i] = -INFINITY, l[i] = 0.f; }
     bool any = false;
-    look_up(0);
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      copy(s);
-      copy_commit();
-      look_up(s + 1);
+    if (n > 0) {
+      load_keys(now);
+      load_values(now);
     }
-    int stage = 0;
+    uint32_t seen = __ballot_sync(~0u, now.k != kNowhere);  // bit i: key i of the tile
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
-      copy_wait<kStages - 2>();
-      __syncwarp();
-      copy(stage == 0 ? kStages - 1 : stage - 1);
-      copy_commit();
-      look_up(j + kStages);
-      const uint32_t mask = masks[kStages - 1];
-      any                 = any || mask != 0;
-      const unsigned char* k_tile = ring + stage * 2 * Tile::kBytes;
-      const unsigned char* v_tile = k_tile + Tile::kBytes;
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-
-      const int key = lane % kKeys, part = lane / kKeys;
-      float s[Q];
-#pragma unroll
-      for (int i = 0; i < Q; ++i) { s[i] = 0.f; }
-#pragma unroll 4
-      for (int c = part * 4; c < D; c += Tile::kParts * 4) {
-        const float4 k = *reinterpret_cast<const float4*>(k_tile + key * Tile::kPitch + c * 4);
+      float s[Q][kPer];
+      {
+        float2 sum[Q][kPer];
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-          const float4 x = *reinterpret_cast<const float4*>(q_s + i * D + c);
-          s[i] += x.x * k.x + x.y * k.y + x.z * k.z + x.w * k.w;
+#pragma unroll
+          for (int x = 0; x < kPer; ++x) { sum[i][x] = float2{0.f, 0.f}; }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+          for (int i = 0; i < Q; ++i) {
+            const float4 w = *reinterpret_cast<const float4*>(q_s + i * D + c * 16 + t4 * 4);
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) {
+              fma2(sum[i][x], float2{w.x, w.y}, float2{kr[x][c].x, kr[x][c].y});
+              fma2(sum[i][x], float2{w.z, w.w}, float2{kr[x][c].z, kr[x][c].w});
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+#pragma unroll
+          for (int x = 0; x < kPer; ++x) { s[i][x] = sum[i][x].x + sum[i][x].y; }
         }
       }
-      const bool see = mask >> key & 1;
-      float alpha[Q];
-      bool grew = false;
+      const uint32_t mask = seen;
+      any                 = any || (mask & ((1u << kKeys) - 1)) != 0;
+      if (j + 1 < n) { load_keys(next); }
+      seen = __ballot_sync(~0u, next.k != kNowhere);
+      now  = next;
+      next = look_up(j + 2);
+
+      // the four lanes of a key add their parts; with four queries or more each ends with its own queries
+      if constexpr (Q >= 4) {
 #pragma unroll
-      for (int i = 0; i < Q; ++i) {
+        for (int x = 0; x < kPer; ++x) {
 #pragma unroll
-        for (int x = kKeys; x < 32; x <<= 1) { s[i] += __shfl_xor_sync(~0u, s[i], x); }
-        s[i]      = see ? s[i] * p.scale : -INFINITY;
-        float top = s[i];
+          for (int i = 0; i < Q / 2; ++i) {
+            const float mine = t4 & 2 ? s[i + Q / 2][x] : s[i][x], other = t4 & 2 ? s[i][x] : s[i + Q / 2][x];
+            s[i][x] = mine + __shfl_xor_sync(~0u, other, 2);
+          }
 #pragma unroll
-        for (int x = 1; x < kKeys; x <<= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, x)); }
+          for (int i = 0; i < Q / 4; ++i) {
+            const float mine = t4 & 1 ? s[i + Q / 4][x] : s[i][x], other = t4 & 1 ? s[i][x] : s[i + Q / 4][x];
+            s[i][x] = mine + __shfl_xor_sync(~0u, other, 1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          s[0][x] += __shfl_xor_sync(~0u, s[0][x], 2);
+          s[0][x] += __shfl_xor_sync(~0u, s[0][x], 1);
+        }
+      }
+      const int own = Q >= 4 ? t4 * kOwn : 0;  // the lane's first query
+      bool grew     = false;
+      float alpha[kOwn];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          s[i][x] = mask >> (g8 + 8 * x) & 1 ? s[i][x] * p.scale : -INFINITY;
+          top     = fmaxf(top, s[i][x]);
+        }
+        top              = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+        top              = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+        top              = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
         top              = fmaxf(top, m[i]);
         const float base = top == -INFINITY ? 0.f : top;
         alpha[i]         = exp2_fast(m[i] - base);
         grew             = grew || top > m[i];
         m[i]             = top;
-        const float w    = exp2_fast(s[i] - base);
-        l[i]             = l[i] * alpha[i] + (part == 0 ? w : 0.f);
-        if (part == 0) { weights[i * kKeys + key] = w; }
-      }
-      __syncwarp();
-      if (grew) {
+        l[i] *= alpha[i];
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) { o[i][c] *= alpha[i]; }
+        for (int x = 0; x < kPer; ++x) {
+          const float w = exp2_fast(s[i][x] - base);
+          l[i] += w;
+          if (Q >= 4 || t4 == 0) { *reinterpret_cast<float2*>(weights + 2 * ((own + i) * kKeys + g8 + 8 * x)) = float2{w, w}; }
         }
       }
-#pragma unroll 2
-      for (int k = 0; k < kKeys; k += 4) {
-        Floats<kCols> v[4];
+      if (__any_sync(~0u, grew)) {
+        if (g8 == 0) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          v[x] = *reinterpret_cast<const Floats<kCols>*>(v_tile + (k + x) * Tile::kPitch + lane * kCols * 4);
+          for (int i = 0; i < kOwn; ++i) { factors[own + i] = alpha[i]; }
         }
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
-          const float4 w = *reinterpret_cast<const float4*>(weights + i * kKeys + k);
+          const float f = factors[i];
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            o[i][c] += w.x * v[0].e[c] + w.y * v[1].e[c] + w.z * v[2].e[c] + w.w * v[3].e[c];
+          for (int c = 0; c < kWide; ++c) {
+            o[i][c][0].x *= f, o[i][c][0].y *= f;
+            o[i][c][1].x *= f, o[i][c][1].y *= f;
           }
         }
       }
       __syncwarp();
+      if ((mask & ((1u << kKeys) - 1)) != (1u << kKeys) - 1) {
+#pragma unroll
+        for (int x = 0; x < kKeys / kRows; ++x) {
+          if (!(mask >> (x * kRows + (kRows == 2 ? lane / 16 : 0)) & 1)) {
+#pragma unroll
+            for (int c = 0; c < kWide; ++c) { vr[x][c] = float4{0.f, 0.f, 0.f, 0.f}; }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+#pragma unroll
+        for (int x = 0; x < kKeys / kRows; x += 2) {
+          // the weights of two values of the lane
+          float2 w[2];
+          if constexpr (kRows == 1) {
+            const float4 both = *reinterpret_cast<const float4*>(weights + 2 * (i * kKeys + x));
+            w[0] = float2{both.x, both.y}, w[1] = float2{both.z, both.w};
+          } else {
+            w[0] = *reinterpret_cast<const float2*>(weights + 2 * (i * kKeys + x * 2 + lane / 16));
+            w[1] = *reinterpret_cast<const float2*>(weights + 2 * (i * kKeys + x * 2 + 2 + lane / 16));
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int c = 0; c < kWide; ++c) {
+              fma2(o[i][c][0], w[y], float2{vr[x + y][c].x, vr[x + y][c].y});
+              fma2(o[i][c][1], w[y], float2{vr[x + y][c].z, vr[x + y][c].w});
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (j + 1 < n) { load_values(now); }
     }
-    copy_wait<0>();
-    __syncwarp();
 
-    constexpr int kRow = D + 4;
-    auto* sums         = reinterpret_cast<float*>(ring);
+    float* mine = sums + warp * Tile::kSums;
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) { sums[i * kRow + lane * kCols + c] = o[i][c]; }
-      float sum = l[i];
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) { sum += __shfl_xor_sync(~0u, sum, x); }
-      if (lane == 0) { sums[i * kRow + D] = m[i], sums[i * kRow + D + 1] = sum, sums[i * kRow + D + 2] = any ? 1.f : 0.f; }
+      for (int c = 0; c < kWide; ++c) {
+        float4 v{o[i][c][0].x, o[i][c][0].y, o[i][c][1].x, o[i][c][1].y};
+        if constexpr (kRows == 2) {
+          v.x += __shfl_xor_sync(~0u, v.x, 16), v.y += __shfl_xor_sync(~0u, v.y, 16);
+          v.z += __shfl_xor_sync(~0u, v.z, 16), v.w += __shfl_xor_sync(~0u, v.w, 16);
+        }
+        if (column + c * 128 < D) { *reinterpret_cast<float4*>(mine + i * (D + 4) + column + c * 128) = v; }
+      }
     }
-    finish_segment<float, D>(p, g, reinterpret_cast<const float*>(smem), FloatShared<D, Q>::kWarp / 4, 0.f);
-    clear();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const float sum = sum_over_keys(l[i]);
+      if (g8 == 0 && (Q >= 4 || t4 == 0)) {
+        float* to = mine + ((Q >= 4 ? t4 * kOwn : 0) + i) * (D + 4) + D;
+        to[0] = m[i], to[1] = sum, to[2] = any ? 1.f : 0.f;
+      }
+    }
+    finish_segment<float, D>(p, g, sums, Tile::kSums, 0.f);
   });
 }
 
@@ -1204,7 +1276,7 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   if (a.n_lists == 0 && a.window > 0) { most = std::min(most, a.window); }
   const int64_t units = a.n_rows * n.units;
   n.direct            = most <= kDirectTokens;
-  const int resident  = sm_count * (half ? (dim > 128 ? 1 : n.per_unit <= 8 ? 3 : 2) : dim <= 64 ? 2 : 1);
+  const int resident  = sm_count * (half ? (dim > 128 ? 1 : n.per_unit <= 8 ? 3 : 2) : 2);
   n.blocks            = n.direct ? units : std::min<int64_t>(resident, units * ((most + kStep - 1) / kStep + kLead));
   n.part_floats       = n.per_unit * (dim + 4);
   n.bytes             = n.direct ? 0 : static_cast<size_t>(n.blocks) * 2 * (8 + sizeof(float) * n.part_floats);
@@ -1273,11 +1345,11 @@ template <int D>
 void launch_float(const Params& p, int64_t blocks, cudaStream_t s)
 {
   if (p.per_unit == 1) {
-    launch(attend_float_kernel<D, 1>, FloatShared<D, 1>::kAll, p, blocks, s);
+    launch(attend_float_kernel<D, 1>, FloatTile<D, 1>::kBytes, p, blocks, s);
   } else if (p.per_unit <= 4) {
-    launch(attend_float_kernel<D, 4>, FloatShared<D, 4>::kAll, p, blocks, s);
+    launch(attend_float_kernel<D, 4>, FloatTile<D, 4>::kBytes, p, blocks, s);
   } else {
-    launch(attend_float_kernel<D, 8>, FloatShared<D, 8>::kAll, p, blocks, s);
+    launch(attend_float_kernel<D, 8>, FloatTile<D, 8>::kBytes, p, blocks, s);
   }
 }
 
@@ -1368,6 +1440,8 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   if (a.cache.dtype == kPagedF32) {
     if (p.dim <= 64) {
       launch_float<64>(p, n.blocks, s);
+    } else if (p.dim <= 96) {
+      launch_float<96>(p, n.blocks, s);
     } else if (p.dim <= 128) {
       launch_float<128>(p, n.blocks, s);
     } else {
