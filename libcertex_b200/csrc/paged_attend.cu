@@ -77,7 +77,12 @@ struct Params {
   // the split
   int32_t direct;    // a block per unit
   int32_t workers;
-  int64_t* marks;    // [workers][2]: a unit that a worker begins and leaves unfinished, and the shares that it has (0: none)
+  // what the second kernel needs to know, [workers][2]: the unit that a worker begins and leaves unfinished, and how many shares
+  // it has (0: there is none); or if the call has no more units than workers (by_unit), [units][2]: the worker that begins
+  // it, and how many shares it has (0: no more than that)
+  int64_t* marks;
+  int32_t by_unit;
+  int32_t join_lanes;  // threads of a joining block that share a partial result, with four coordinates each
   float* parts;      // [workers][2] partial results of part_floats each
   int32_t part_floats;
 };
@@ -254,12 +259,17 @@ __device__ __forceinline__ void for_segments(const Params& p, F&& body)
   // rows that see nothing have no steps: the blocks share them out
   if (p.lengths) {
     for (int64_t row = blockIdx.x; row < p.n_rows; row += gridDim.x) {
-      if (steps_of(row) == 0) { nothing_seen(row, 0, p.n_heads, threadIdx.x, kThreads); }
+      if (steps_of(row) == 0) {
+        nothing_seen(row, 0, p.n_heads, threadIdx.x, kThreads);
+        if (p.by_unit) {
+          for (int u = threadIdx.x; u < p.units; u += kThreads) { p.marks[2 * (row * p.units + u) + 1] = 0; }
+        }
+      }
     }
   }
   total *= p.units;
   const int64_t workers = min(int64_t(p.workers), total), w = blockIdx.x;
-  if (threadIdx.x == 0) { p.marks[2 * w + 1] = 0; }
+  if (!p.by_unit && threadIdx.x == 0) { p.marks[2 * w + 1] = 0; }
   if (w >= workers) { return; }
   int64_t at        = total * w / workers;
   const int64_t end = total * (w + 1) / workers;
@@ -311,10 +321,12 @@ __device__ __forceinline__ void for_segments(const Params& p, F&& body)
       const bool begins = g.i0 == 0, ends = g.i1 == s.count;
       // a partial result that begins a unit belongs to the worker's second slot, one that goes on with it to the first
       g.slot = begins && ends ? -1 : 2 * w + (begins ? 1 : 0);
-      if (begins && !ends && threadIdx.x == 0) {
+      if (begins && (!ends || p.by_unit) && threadIdx.x == 0) {
+        const int64_t id = row * p.units + unit;
+        int64_t* mark    = p.marks + 2 * (p.by_unit ? id : w);
+        mark[0]          = p.by_unit ? w : id;
         // step x is in the share of worker ((x + 1) * workers - 1) / total
-        p.marks[2 * w]     = row * p.units + unit;
-        p.marks[2 * w + 1] = ((u0 + steps) * workers - 1) / total - w + 1;
+        mark[1] = ends ? 0 : ((u0 + steps) * workers - 1) / total - w + 1;
       }
       body(g);
     }
@@ -1183,8 +1195,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_float_kernel(const Params 
 }
 
 // ------------------------------------------------------------------------------------------------ joining the shares
-// Block (w, i): if worker w left a unit unfinished that it had begun, joins that unit's partial results for query i. They lie in
-// w's second slot and in the first slots of the workers behind it. A chain of three reads (mark, sums, outputs) is all its time,
+// Block (x, i, z): joins the partial results of the unit that worker x left unfinished, or of unit x, for query i and coordinates
+// 4 * join_lanes * z on. They lie in the second slot of the worker w that began the unit and in the first slots of those behind it. A chain of three reads (mark, sums, outputs) is all its time,
 // so every thread reads at once what it needs: one share's sums, then four coordinates of every eighth share.
 constexpr int kJoinThreads = 256;
 
@@ -1195,10 +1207,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
   __shared__ float red[3][kJoinThreads / 32];
   __shared__ float4 outs[kJoinThreads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int w = blockIdx.x, i = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t id = p.marks[2 * w];
-  const int n      = static_cast<int>(p.marks[2 * w + 1]);
+  const int i = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int n = static_cast<int>(p.marks[2 * blockIdx.x + 1]);
   if (n == 0) { return; }
+  const int64_t mark = p.marks[2 * blockIdx.x];
+  const int64_t id   = p.by_unit ? blockIdx.x : mark;
+  const int w        = static_cast<int>(p.by_unit ? mark : blockIdx.x);
   const int64_t row = id / p.units;
   const Segment g   = segment_of(p, row, Span{0, 0, 0}, static_cast<int>(id - row * p.units));
   if (i >= g.n_heads) { return; }
@@ -1228,8 +1242,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
   __syncthreads();
   sum = seen = 0.f;
   for (int x = 0; x < kJoinThreads / 32; ++x) { sum += red[1][x], seen += red[2][x]; }
-  const int lanes = p.dim <= 128 ? 32 : 64, groups = kJoinThreads / lanes;
-  const int c = threadIdx.x % lanes * 4, first = threadIdx.x / lanes;
+  const int lanes = p.join_lanes, groups = kJoinThreads / lanes, from_c = blockIdx.z * lanes * 4;
+  const int c = from_c + threadIdx.x % lanes * 4, first = threadIdx.x / lanes;
   float4 v{0.f, 0.f, 0.f, 0.f};
   if (c < p.dim) {
 #pragma unroll 8
@@ -1241,12 +1255,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
   }
   outs[threadIdx.x] = v;
   __syncthreads();
-  for (int x = threadIdx.x; x < p.dim; x += kJoinThreads) {
+  for (int x = threadIdx.x; x < min(lanes * 4, p.dim - from_c); x += kJoinThreads) {
     float r = 0.f;
     for (int y = 0; y < groups; ++y) { r += reinterpret_cast<const float*>(outs + y * lanes)[x]; }
-    (static_cast<T*>(p.out) + row * p.o_row + (g.head + i) * p.o_head)[x] = Type<T>::down(seen > 0.f ? r / sum : 0.f);
+    (static_cast<T*>(p.out) + row * p.o_row + (g.head + i) * p.o_head)[from_c + x] = Type<T>::down(seen > 0.f ? r / sum : 0.f);
   }
-  if (p.lse && threadIdx.x == 0) { p.lse[row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
+  if (p.lse && threadIdx.x == 0 && blockIdx.z == 0) { p.lse[row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
 }
 
 // ------------------------------------------------------------------------------------------------ launch
@@ -1257,7 +1271,7 @@ struct Plan {
   int32_t per_unit, subs, units;
   int direct;
   int64_t blocks;
-  int part_floats;
+  int part_floats, by_unit;
   size_t bytes;
 };
 
@@ -1280,6 +1294,7 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   n.blocks            = n.direct ? units : std::min<int64_t>(resident, units * ((most + kStep - 1) / kStep + kLead));
   n.part_floats       = n.per_unit * (dim + 4);
   n.bytes             = n.direct ? 0 : static_cast<size_t>(n.blocks) * 2 * (8 + sizeof(float) * n.part_floats);
+  n.by_unit           = units <= n.blocks;
   return n;
 }
 
@@ -1357,7 +1372,8 @@ template <typename T>
 void launch_join(const Params& p, cudaStream_t s)
 {
   cudaLaunchConfig_t c{};
-  c.gridDim          = dim3(static_cast<unsigned>(p.workers), static_cast<unsigned>(p.per_unit));
+  const auto joined  = static_cast<unsigned>(p.by_unit ? p.n_rows * p.units : p.workers);
+  c.gridDim          = dim3(joined, static_cast<unsigned>(p.per_unit), static_cast<unsigned>((p.dim + p.join_lanes * 4 - 1) / (p.join_lanes * 4)));
   c.blockDim         = dim3(kJoinThreads);
   c.dynamicSmemBytes = sizeof(float) * static_cast<size_t>(p.workers);
   c.stream           = s;
@@ -1434,6 +1450,9 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.scale           = a.scale * kLog2e;
   p.direct          = n.direct;
   p.workers         = static_cast<int32_t>(n.blocks);
+  p.by_unit         = n.by_unit;
+  // few units have many shares each: more blocks for each of them
+  p.join_lanes      = a.n_rows * n.units * n.per_unit <= sm_count ? 8 : p.dim <= 128 ? 32 : 64;
   p.part_floats     = n.part_floats;
   p.parts           = static_cast<float*>(a.workspace);
   p.marks           = n.direct ? nullptr : reinterpret_cast<int64_t*>(p.parts + 2 * n.blocks * n.part_floats);
