@@ -1,5 +1,5 @@
 // The operators of a decoding step over a paged cache of keys and values: rotation by position, append, attention of new
-// tokens over the cache and over selected positions of it. Definitions in rotate.cu and paged_attend.cu; the arguments are
+// tokens over the cache and over selected positions of it. Definitions in rotate.cu and paged_attend*.cu; the arguments are
 // checked by the entry points in c_api.cu.
 #pragma once
 

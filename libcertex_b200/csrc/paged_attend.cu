@@ -1,1277 +1,23 @@
-// Attention of new tokens over a paged cache of keys and values: over the first keys of a sequence
-// (certexB200PagedAttend) or over selected positions of the cache (certexB200PagedAttendSelected).
-//
-//   s_j = scale <q, k_j>,  out = sum_j exp(s_j) v_j / sum_j exp(s_j),  lse = log sum_j exp(s_j)
-//
-// over the positions j that the row may see; a row that sees none gets zeros and -infinity.
-//
-// What bounds it: every key and value is read once from HBM, for at most a few dozen operations per byte (two products for
-// each query head that shares the KV head). So the work is a stream of rows of 2 d bytes from addresses that the page table or
-// the list of positions names, and everything else has to fit beside it:
-//
-//  * One pass. Scores, the running maximum m, the running sum l and the output stay in registers in float32;
-//    when m grows, l and the output are multiplied by exp2(m_old - m_new). Scores are kept in units of log2 e, so that a
-//    weight is one multiply-add and one exp2.
-//  * The stream is split evenly. The tokens that all rows of the call see, in steps of kStep, are one sequence of work that
-//    is cut into equal shares, a share per resident block ("worker"), wherever the cuts fall: 1 row of 131 072 keys and 64
-//    rows of 1 to 8192 keys load the GPU alike, and lengths are read on the device only. A row and KV head ("unit") that
-//    a cut divides leaves a partial result (m, l, output) per share, which a second, small kernel joins in the order of the
-//    shares: results do not depend on timing. It is launched while the first still runs and waits for it.
-//    Calls whose units are known to be short take a block per unit and one launch.
-//  * A warp works by itself on tiles of 16 keys (every fourth of its block's): no barrier until a unit ends, and the loads of
-//    the next tile are in flight while one is computed. The table's entries for a tile are fetched one tile before its loads.
-//
-// Rows that are not to be seen have scores of -infinity and values of zero, so nothing that lies there (NaN, infinity,
-// another sequence's tokens) has an effect.
-#include "paged.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+// How the attention over a paged cache is split over the GPU, and its launch. The kernels are in paged_attend.cuh, a file per type
+// compiles them.
+#include "paged_attend.cuh"
 
 #include <algorithm>
 
 namespace certex_b200 {
 namespace {
 
-constexpr int kWarps   = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kStep    = 64;  // tokens of a step of the work split
-constexpr int kLead    = 2;   // steps that a unit's beginning and end count for: fetching its first tiles, joining the warps
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2   = 0.6931471805599453f;
-
-/// What the kernels need, in the sizes that they compute with.
-struct Params {
-  const void* keys;
-  const void* values;
-  // strides of pages and tokens in units of 2^unit_shift bytes, of heads in elements
-  uint32_t k_page, k_token, v_page, v_token;
-  int64_t k_head, v_head;
-  int32_t unit_shift;
-  int32_t page_shift;  // log2 of page_size, -1: no power of two
-  int64_t n_places;    // n_pages * page_size
-  int32_t n_pages;
-  uint32_t page_size;
-  int32_t dim;
-  int32_t* fault;
-  // what a row sees
-  const int32_t* pages;
-  int64_t page_row;
-  int64_t n_sequences, most;  // most: tokens that the table can hold
-  const int32_t* row_to_sequence;
-  const int32_t* lengths;     // null: lists
-  int64_t window;
-  const void* lists;
-  int32_t lists_64, n_lists;
-  int64_t k;
-  // queries and answers
-  const void* q;
-  int64_t q_row, q_head;
-  void* out;
-  int64_t o_row, o_head;
-  float* lse;
-  int64_t n_rows;
-  int32_t n_heads, group, subs, per_unit;  // query heads per KV head; units per KV head; query heads of a unit
-  int32_t units;                           // of a row
-  float scale;                             // in units of log2 e
-  // the split
-  int32_t direct;    // a block per unit
-  int32_t workers;
-  // what the second kernel needs to know, [workers][2]: the unit that a worker begins and leaves unfinished, and how many shares
-  // it has (0: there is none); or if the call has no more units than workers (by_unit), [units][2]: the worker that begins
-  // it, and how many shares it has (0: no more than that)
-  int64_t* marks;
-  int32_t by_unit;
-  int32_t join_lanes;  // threads of a joining block that share a partial result, with four coordinates each
-  float* parts;      // [workers][2] partial results of part_floats each
-  int32_t part_floats;
-};
-
-// ------------------------------------------------------------------------------------------------ types
-template <typename T>
-struct Type;
-template <>
-struct Type<float> {
-  static __device__ float up(float v) { return v; }
-  static __device__ float down(float v) { return v; }
-};
-template <>
-struct Type<__half> {
-  static __device__ float up(__half v) { return __half2float(v); }
-  static __device__ __half down(float v) { return __float2half_rn(v); }
-};
-template <>
-struct Type<__nv_bfloat16> {
-  static __device__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-  static __device__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
-};
-
-__device__ __forceinline__ float exp2_fast(float x)
-{
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-/// 16 bytes to shared memory, or 16 zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real)
-{
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait()
-{
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// ------------------------------------------------------------------------------------------------ what a row sees
-struct Span {
-  int64_t begin;  // first token
-  int64_t count;
-  int64_t sequence;
-};
-
-__device__ __forceinline__ Span span_of(const Params& p, int64_t row)
-{
-  if (p.lengths == nullptr) { return {0, p.k, row}; }
-  int64_t end       = p.lengths[row];
-  const int64_t seq = p.row_to_sequence ? p.row_to_sequence[row] : row;
-  if (end <= 0) { return {0, 0, 0}; }
-  const bool stranger = seq < 0 || seq >= p.n_sequences;
-  if (stranger || end > p.most) { *p.fault = 1; }
-  if (stranger) { return {0, 0, 0}; }
-  end                 = min(end, p.most);
-  const int64_t begin = p.window > 0 ? max(int64_t(0), end - p.window) : 0;
-  return {begin, end - begin, seq};
-}
-
-/// One unit's share: tokens [i0, i1) of what its row sees.
-struct Segment {
-  int64_t row;
-  int kv, head, n_heads;  // KV head, first query head, query heads
-  int64_t begin;
-  const int32_t* pages;   // the sequence's row of the table, or
-  const void* list;
-  int64_t i0, i1;
-  int64_t slot;           // of the partial result, -1: this is the whole unit
-};
-
-__device__ __forceinline__ Segment segment_of(const Params& p, int64_t row, const Span& s, int unit)
-{
-  Segment g;
-  g.row     = row;
-  g.kv      = unit / p.subs;
-  const int sub = unit - g.kv * p.subs;
-  g.head    = g.kv * p.group + sub * p.per_unit;
-  g.n_heads = min(p.per_unit, p.group - sub * p.per_unit);
-  g.begin   = s.begin;
-  g.pages   = p.pages + s.sequence * p.page_row;
-  const int64_t list = p.n_lists == 1 ? row : p.n_lists == p.n_heads ? row * p.n_lists + g.head : row * p.n_lists + g.kv;
-  g.list    = p.lists_64 ? static_cast<const void*>(static_cast<const int64_t*>(p.lists) + list * p.k)
-                         : static_cast<const void*>(static_cast<const int32_t*>(p.lists) + list * p.k);
-  return g;
-}
-
-/// Where a key and its value lie, in units from the first key and value of their head; kNowhere for one that is not seen.
-struct Place {
-  uint32_t k, v;
-};
-constexpr uint32_t kNowhere = ~0u;
-
-/// The place of token i of a segment.
-__device__ __forceinline__ Place place_of(const Params& p, const Segment& g, int64_t i)
-{
-  uint32_t page, place;
-  if (p.lengths) {
-    const auto t = static_cast<uint32_t>(g.begin + i);
-    const uint32_t n = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-    place        = t - n * p.page_size;
-    page         = static_cast<uint32_t>(g.pages[n]);
-    if (page >= static_cast<uint32_t>(p.n_pages)) {  // negative entries too
-      *p.fault = 1;
-      return {kNowhere, kNowhere};
-    }
-  } else {
-    const int64_t at = p.lists_64 ? static_cast<const int64_t*>(g.list)[i] : static_cast<const int32_t*>(g.list)[i];
-    if (at < 0) { return {kNowhere, kNowhere}; }
-    if (at >= p.n_places) {
-      *p.fault = 1;
-      return {kNowhere, kNowhere};
-    }
-    if (p.page_shift >= 0) {
-      page = static_cast<uint32_t>(at >> p.page_shift);
-    } else {
-      page = at >> 32 ? static_cast<uint32_t>(at / p.page_size) : static_cast<uint32_t>(at) / p.page_size;
-    }
-    place = static_cast<uint32_t>(at) - page * p.page_size;
-  }
-  return {page * p.k_page + place * p.k_token, page * p.v_page + place * p.v_token};
-}
-
-/// Calls body(segment) for this block's share of the work. A block of kThreads threads calls it as a whole.
-template <typename T, typename F>
-__device__ __forceinline__ void for_segments(const Params& p, F&& body)
-{
-  __shared__ int64_t sums[kWarps];
-  __shared__ int64_t found[2];
-  auto nothing_seen = [&](int64_t row, int head, int n_heads, int first, int step) {
-    for (int h = head; h < head + n_heads; ++h) {
-      T* o = static_cast<T*>(p.out) + row * p.o_row + h * p.o_head;
-      for (int c = first; c < p.dim; c += step) { o[c] = Type<T>::down(0.f); }
-      if (p.lse && first == 0) { p.lse[row * p.n_heads + h] = -INFINITY; }
-    }
-  };
-  if (p.direct) {
-    const int64_t row = blockIdx.x / p.units;
-    const Span s      = span_of(p, row);
-    Segment g         = segment_of(p, row, s, static_cast<int>(blockIdx.x - row * p.units));
-    if (s.count == 0) {
-      nothing_seen(row, g.head, g.n_heads, threadIdx.x, kThreads);
-      return;
-    }
-    g.i0 = 0, g.i1 = s.count, g.slot = -1;
-    body(g);
-    return;
-  }
-
-  // how many steps there are in all: every block counts for itself
-  auto steps_for = [&](int64_t count) { return count > 0 ? (count + kStep - 1) / kStep + kLead : 0; };
-  auto steps_of  = [&](int64_t row) { return steps_for(span_of(p, row).count); };
-  const int64_t same = p.lengths ? 0 : steps_for(p.k);
-  int64_t total = 0, mine = 0;
-  if (!p.lengths) {
-    total = p.n_rows * same;
-  } else if (p.n_rows == 1) {
-    total = steps_of(0);
-  } else {
-    for (int64_t row = threadIdx.x; row < p.n_rows; row += kThreads) {
-      const int64_t n = steps_of(row);
-      mine += n;
-    }
-    for (int o = 16; o > 0; o >>= 1) { mine += __shfl_xor_sync(~0u, mine, o); }
-    if (threadIdx.x % 32 == 0) { sums[threadIdx.x / 32] = mine; }
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) { total += sums[w]; }
-  }
-  // rows that see nothing have no steps: the blocks share them out
-  if (p.lengths) {
-    for (int64_t row = blockIdx.x; row < p.n_rows; row += gridDim.x) {
-      if (steps_of(row) == 0) {
-        nothing_seen(row, 0, p.n_heads, threadIdx.x, kThreads);
-        if (p.by_unit) {
-          for (int u = threadIdx.x; u < p.units; u += kThreads) { p.marks[2 * (row * p.units + u) + 1] = 0; }
-        }
-      }
-    }
-  }
-  total *= p.units;
-  const int64_t workers = min(int64_t(p.workers), total), w = blockIdx.x;
-  if (!p.by_unit && threadIdx.x == 0) { p.marks[2 * w + 1] = 0; }
-  if (w >= workers) { return; }
-  int64_t at        = total * w / workers;
-  const int64_t end = total * (w + 1) / workers;
-
-  // the row of step `at`, and the first step of that row
-  int64_t row = 0, base = 0;
-  if (!p.lengths) {
-    row  = at / (same * p.units);
-    base = row * same * p.units;
-  } else if (p.n_rows > 1) {
-    int64_t before = 0;
-    for (int64_t r0 = 0; r0 < p.n_rows; r0 += kThreads) {
-      const int64_t r = r0 + threadIdx.x;
-      const int64_t n = r < p.n_rows ? steps_of(r) * p.units : 0;
-      int64_t upto    = n;  // inclusive sum over the warp
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(~0u, upto, o);
-        if (threadIdx.x % 32 >= o) { upto += x; }
-      }
-      __syncthreads();
-      if (threadIdx.x % 32 == 31) { sums[threadIdx.x / 32] = upto; }
-      __syncthreads();
-      int64_t first = before;
-      for (int i = 0; i < kWarps; ++i) {
-        if (i < threadIdx.x / 32) { first += sums[i]; }
-        before += sums[i];
-      }
-      first += upto - n;
-      if (n > 0 && first <= at && at < first + n) { found[0] = r, found[1] = first; }
-      if (at < before) { break; }
-    }
-    __syncthreads();
-    row = found[0], base = found[1];
-  }
-
-  while (at < end) {
-    const Span s        = span_of(p, row);
-    const int64_t steps = steps_for(s.count);
-    if (steps == 0) {
-      ++row;
-      continue;
-    }
-    const auto unit  = static_cast<int>((at - base) / steps);
-    const int64_t u0 = base + unit * steps, to = min(end, u0 + steps);
-    Segment g = segment_of(p, row, s, unit);
-    g.i0      = max(int64_t(0), at - u0 - kLead) * kStep;
-    g.i1      = min(s.count, max(int64_t(0), to - u0 - kLead) * kStep);
-    if (g.i0 < g.i1) {  // (a share may end within a unit's lead)
-      const bool begins = g.i0 == 0, ends = g.i1 == s.count;
-      // a partial result that begins a unit belongs to the worker's second slot, one that goes on with it to the first
-      g.slot = begins && ends ? -1 : 2 * w + (begins ? 1 : 0);
-      if (begins && (!ends || p.by_unit) && threadIdx.x == 0) {
-        const int64_t id = row * p.units + unit;
-        int64_t* mark    = p.marks + 2 * (p.by_unit ? id : w);
-        mark[0]          = p.by_unit ? w : id;
-        // step x is in the share of worker ((x + 1) * workers - 1) / total
-        mark[1] = ends ? 0 : ((u0 + steps) * workers - 1) / total - w + 1;
-      }
-      body(g);
-    }
-    at = to;
-    if (at == base + steps * p.units) {
-      base = at;
-      ++row;
-    }
-  }
-}
-
-/// The answer of a unit's query head from its sums, or a partial result: coordinate c of query i.
-template <typename T>
-__device__ __forceinline__ void put_out(const Params& p, const Segment& g, int i, int c, float v)
-{
-  if (g.slot >= 0) {
-    p.parts[g.slot * p.part_floats + 4 * p.per_unit + i * p.dim + c] = v;
-  } else {
-    (static_cast<T*>(p.out) + g.row * p.o_row + (g.head + i) * p.o_head)[c] = Type<T>::down(v);
-  }
-}
-
-/// m, l and whether anything was seen, of query i (once per query).
-__device__ __forceinline__ void put_sums(const Params& p, const Segment& g, int i, float m, float l, bool any)
-{
-  if (g.slot >= 0) {
-    float* to = p.parts + g.slot * p.part_floats + 4 * i;
-    to[0] = m, to[1] = l, to[2] = any ? 1.f : 0.f;
-  } else if (p.lse) {
-    p.lse[g.row * p.n_heads + g.head + i] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
-  }
-}
-
-// ------------------------------------------------------------------------------------------------ 16-bit types
-// Tensor cores by warp-level products (mma.m16n8k16): with one new token there are 1 to 16 queries per KV head, and tcgen05's
-// smallest tile of 128 rows would be nearly empty. Keys and values take the 16-row side of the product and the
-// queries the 8-column side, so that 8 queries fill it: S^T = K Q^T, then O^T = V^T P^T. The two products of a tile of
-// 16 keys by d = 128 are 8 + 16 instructions for 8 KB read.
-//
-// Weights enter the second product as two 16-bit numbers, the upper part cut off and the rest (p = hi + lo to 2^-16), because a
-// weight rounded once to bfloat16 would add as much error as the rounding of the result. lo is kept positive: zero times an
-// infinite value would be NaN. Weights of float16 are multiplied by 2^12, since float16 has nothing below 2^-24; l carries
-// the factor too, so it cancels.
-constexpr int kKeys   = 16;  // of a tile
-constexpr int kStages = 3;
-
-__device__ __forceinline__ void load_matrix(uint32_t (&a)[4], uint32_t at)
-{
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-               : "r"(at)
-               : "memory");
-}
-__device__ __forceinline__ void load_matrix_t(uint32_t (&a)[4], uint32_t at)
-{
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-               : "r"(at)
-               : "memory");
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
-{
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-
-template <typename T>
-struct Half;
-template <>
-struct Half<__nv_bfloat16> {
-  static constexpr float kRaise = 0.f;  // log2 of the factor on weights
-  static __device__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-  {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  /// (x, y) as two pairs of numbers whose sum they are; x in the lower halves.
-  static __device__ void split(float x, float y, uint32_t& hi, uint32_t& lo)
-  {
-    const uint32_t a = __float_as_uint(x) & 0xffff0000u, b = __float_as_uint(y) & 0xffff0000u;
-    hi = (a >> 16) | b;
-    const __nv_bfloat162 r = __floats2bfloat162_rn(fmaxf(x - __uint_as_float(a), 1.2e-38f), fmaxf(y - __uint_as_float(b), 1.2e-38f));
-    lo = *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-template <>
-struct Half<__half> {
-  static constexpr float kRaise = 12.f;
-  static __device__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-  {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ void split(float x, float y, uint32_t& hi, uint32_t& lo)
-  {
-    const __half2 h = __halves2half2(__float2half_rz(x), __float2half_rz(y));
-    hi              = *reinterpret_cast<const uint32_t*>(&h);
-    const __half2 r = __floats2half2_rn(fmaxf(x - __low2float(h), 6e-8f), fmaxf(y - __high2float(h), 6e-8f));
-    lo              = *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-
-/// What the block's warps found of a segment meets in shared memory (`sums`: a warp's [queries][D + 4] floats: output, m, l, seen;
-/// `pitch` floats between warps) and goes out. m is relative to weights that were raised by 2^raise.
-template <typename T, int D>
-__device__ __forceinline__ void finish_segment(const Params& p, const Segment& g, const float* sums, int pitch, float raise)
-{
-  constexpr int kRow = D + 4;
-  __syncthreads();
-  for (int i = 0; i < g.n_heads; ++i) {
-    float w[kWarps], top = -INFINITY, sum = 0.f, seen = 0.f;
-#pragma unroll
-    for (int x = 0; x < kWarps; ++x) {
-      w[x] = sums[x * pitch + i * kRow + D];
-      top  = fmaxf(top, w[x]);
-    }
-#pragma unroll
-    for (int x = 0; x < kWarps; ++x) {
-      const float* from = sums + x * pitch + i * kRow;
-      w[x]              = top == -INFINITY ? 1.f : exp2_fast(w[x] - top);
-      sum += w[x] * from[D + 1];
-      seen += from[D + 2];
-    }
-    const float scale = g.slot >= 0 ? 1.f : 1.f / sum;
-    for (int c = threadIdx.x; c < p.dim; c += kThreads) {
-      float v = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) { v += w[x] * sums[x * pitch + i * kRow + c]; }
-      put_out<T>(p, g, i, c, seen > 0.f ? v * scale : 0.f);
-    }
-    if (threadIdx.x == 0) { put_sums(p, g, i, top - raise, sum, seen > 0.f); }
-  }
-  __syncthreads();
-}
-
-/// The softmax of a tile's scores s (16 keys x 8 queries, as the first product leaves them), one group of eight queries:
-/// scores become weights as the second product's operand, m and l go on. Returns whether m grew (in this thread's queries).
-template <typename T>
-__device__ __forceinline__ bool soften(float (&s)[4], float scale, bool see0, bool see1, float (&m)[2], float (&l)[2], float (&alpha)[2],
-                                       uint32_t (&hi)[2], uint32_t (&lo)[2])
-{
-  float base[2];
-  bool grew = false;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    s[c]      = see0 ? s[c] * scale : -INFINITY;
-    s[c + 2]  = see1 ? s[c + 2] * scale : -INFINITY;
-    float top = fmaxf(s[c], s[c + 2]);
-    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-    top       = fmaxf(top, m[c]);
-    base[c]   = top == -INFINITY ? 0.f : top;
-    alpha[c]  = exp2_fast(m[c] - base[c]);
-    grew      = grew || top > m[c];
-    m[c]      = top;
-    base[c] -= Half<T>::kRaise;
-  }
-#pragma unroll
-  for (int c = 0; c < 4; ++c) { s[c] = exp2_fast(s[c] - base[c & 1]); }
-  l[0] = l[0] * alpha[0] + (s[0] + s[2]);
-  l[1] = l[1] * alpha[1] + (s[1] + s[3]);
-  Half<T>::split(s[0], s[1], hi[0], lo[0]);
-  Half<T>::split(s[2], s[3], hi[1], lo[1]);
-  // from keys by lanes to queries by lanes
-  hi[0] = transpose8x8(hi[0]), hi[1] = transpose8x8(hi[1]);
-  lo[0] = transpose8x8(lo[0]), lo[1] = transpose8x8(lo[1]);
-  return grew;
-}
-
-/// The sum over the lanes that hold different keys of the same query.
-__device__ __forceinline__ float sum_over_keys(float v)
-{
-  v += __shfl_xor_sync(~0u, v, 4);
-  v += __shfl_xor_sync(~0u, v, 8);
-  return v + __shfl_xor_sync(~0u, v, 16);
-}
-
-// Heads of up to 128 coordinates: operands come straight from global memory into the registers of the product that uses
-// them. A product over coordinates may take them in any order, as long as keys and queries agree, so lane t of a
-// key's four lanes takes 16 bytes in a row for two steps of the product; and the second product's rows, the
-// coordinates of the result, may be any eight coordinates, so lane g of a value's eight lanes takes 16 bytes in a row for
-// four products. What is left is to pair the values of neighbouring keys, one byte permutation per register.
-// Against copies into shared memory and ldmatrix this takes 250 instructions per tile instead of 470.
-
-/// N * 4 bytes that are read once.
-template <int N>
-__device__ __forceinline__ void read_once(uint32_t (&r)[N], const char* at)
-{
-  static_assert(N == 1 || N == 2 || N == 4, "");
-  if constexpr (N == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(at));
-  } else if constexpr (N == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(at));
-  } else {
-    asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(r[0]) : "l"(at));
-  }
-}
-
-/// A lane's share of a row's coordinates in blocks: 8 * E coordinates where every lane of eight (or 4 * E, of four) takes E.
-template <int N64, int N32, int N16>
-struct RowPart {
-  uint32_t b64[N64 ? N64 : 1][4], b32[N32 ? N32 : 1][2], b16[N16 ? N16 : 1][1];
-};
-
-template <typename T, int D, int NT, bool PAD>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attend_direct_kernel(const Params p)
-{
-  constexpr int kK32 = D / 32, kK16 = D % 32 / 16;                  // keys: blocks of 32 and 16 coordinates
-  constexpr int kV64 = D / 64, kV32 = D % 64 / 32, kV16 = D % 32 / 16;  // values: of 64, 32 and 16
-  constexpr int kSteps = 2 * kK32 + kK16, kTiles = 4 * kV64 + 2 * kV32 + kV16;
-  extern __shared__ __align__(16) float sums[];  // [warps][8 NT][D + 4]
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  for_segments<T>(p, [&](const Segment& g) {
-    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(T) + t4 * 16;
-    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(T) + g8 * 16;
-    const int tiles    = static_cast<int>((g.i1 - g.i0 + 15) / 16);
-    const int n        = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-
-    // where key lane % 16 of tile j lies
-    auto look_up = [&](int j) {
-      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * 16 + lane % 16;
-      return j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
-    };
-    Place now = look_up(0), next = look_up(1);
-
-    // the queries, as the 8-column side of the first product
-    uint32_t qf[NT][kSteps][2];
-    {
-      const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
-#pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        const int i  = x * 8 + g8;
-        const T* row = q + i * p.q_head;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c = k < 2 * kK32 ? k / 2 * 32 + t4 * 8 + k % 2 * 4 + h * 2 : kK32 * 32 + t4 * 4 + h * 2;
-            uint32_t v  = 0;
-            if (i < g.n_heads && (!PAD || c < p.dim)) {
-              const auto a = *reinterpret_cast<const uint16_t*>(row + c), b = *reinterpret_cast<const uint16_t*>(row + c + 1);
-              v            = a | (uint32_t(b) << 16);
-            }
-            qf[x][k][h] = v;
-          }
-        }
-      }
-    }
-    float o[NT][kTiles][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-#pragma unroll
-      for (int d = 0; d < kTiles; ++d) { o[x][d][0] = o[x][d][1] = o[x][d][2] = o[x][d][3] = 0.f; }
-      m[x][0] = m[x][1] = -INFINITY;
-      l[x][0] = l[x][1] = 0.f;
-    }
-
-    uint32_t kr[2][kK32 + kK16][4];  // keys g8 and g8 + 8
-    RowPart<kV64, kV32, kV16> vr[4];  // values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
-    auto at_of = [&](uint32_t place) { return static_cast<uint64_t>(place == kNowhere ? 0 : place) << p.unit_shift; };
-    auto load_keys = [&](const uint32_t (&place)[2]) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const char* at = keys + at_of(place[r]);
-#pragma unroll
-        for (int b = 0; b < kK32; ++b) {
-          if (!PAD || b * 32 + t4 * 8 < p.dim) { read_once<4>(kr[r][b], at + b * 64); }
-        }
-        if constexpr (kK16 > 0) {
-          uint32_t two[2];
-          read_once<2>(two, at + kK32 * 64 - t4 * 8);
-          kr[r][kK32][0] = two[0], kr[r][kK32][1] = two[1];
-        }
-      }
-    };
-    auto load_values = [&](const uint32_t (&place)[4]) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const char* at = values + at_of(place[r]);
-#pragma unroll
-        for (int b = 0; b < kV64; ++b) {
-          if (!PAD || b * 64 + g8 * 8 < p.dim) { read_once<4>(vr[r].b64[b], at + b * 128); }
-        }
-        if constexpr (kV32 > 0) { read_once<2>(vr[r].b32[0], at + kV64 * 128 - g8 * 8); }
-        if constexpr (kV16 > 0) { read_once<1>(vr[r].b16[0], at + kV64 * 128 + kV32 * 64 - g8 * 12); }
-      }
-    };
-    auto keys_of = [&](const Place& x, uint32_t (&place)[2]) {
-      place[0] = __shfl_sync(~0u, x.k, g8);
-      place[1] = __shfl_sync(~0u, x.k, g8 + 8);
-    };
-    auto values_of = [&](const Place& x, uint32_t (&place)[4]) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) { place[r] = __shfl_sync(~0u, x.v, t4 * 2 + (r & 1) + (r & 2) * 4); }
-    };
-    // a register of two neighbouring keys' values at one coordinate
-    auto pair = [](uint32_t a, uint32_t b, int odd) { return __byte_perm(a, b, odd ? 0x7632 : 0x5410); };
-
-    if (PAD) {
-      // what lies behind the last coordinate is never loaded, and must be a number
-#pragma unroll
-      for (int b = 0; b < kK32; ++b) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) { kr[0][b][x] = kr[1][b][x] = 0; }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int b = 0; b < kV64; ++b) { vr[r].b64[b][0] = vr[r].b64[b][1] = vr[r].b64[b][2] = vr[r].b64[b][3] = 0; }
-      }
-    }
-    uint32_t kp[2], vp[4];
-    bool any = false;
-    if (n > 0) {
-      keys_of(now, kp);
-      values_of(now, vp);
-      load_keys(kp);
-      load_values(vp);
-    }
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      float s[NT][4];
-#pragma unroll
-      for (int x = 0; x < NT; ++x) { s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f; }
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const int b = k / 2, h = k % 2 * 2;
-        const uint32_t a[4] = {kr[0][b][h], kr[1][b][h], kr[0][b][h + 1], kr[1][b][h + 1]};
-#pragma unroll
-        for (int x = 0; x < NT; ++x) { Half<T>::mma(s[x], a, qf[x][k][0], qf[x][k][1]); }
-      }
-      const bool see0 = kp[0] != kNowhere, see1 = kp[1] != kNowhere;
-      any             = any || see0 || see1;
-      // every key of the tile is seen, or the values of those that are not become zeros
-      const bool full = __all_sync(~0u, see0 && see1);
-      if (!full) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (vp[r] == kNowhere) {
-#pragma unroll
-            for (int b = 0; b < kV64; ++b) { vr[r].b64[b][0] = vr[r].b64[b][1] = vr[r].b64[b][2] = vr[r].b64[b][3] = 0; }
-            vr[r].b32[0][0] = vr[r].b32[0][1] = vr[r].b16[0][0] = 0;
-          }
-        }
-      }
-      if (j + 1 < n) {
-        keys_of(next, kp);
-        load_keys(kp);
-      }
-      values_of(next, vp);
-      next = look_up(j + 2);
-
-      uint32_t hi[NT][2], lo[NT][2];
-      float alpha[NT][2];
-      bool grew = false;
-#pragma unroll
-      for (int x = 0; x < NT; ++x) { grew |= soften<T>(s[x], p.scale, see0, see1, m[x], l[x], alpha[x], hi[x], lo[x]); }
-      if (__any_sync(~0u, grew)) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-#pragma unroll
-          for (int d = 0; d < kTiles; ++d) {
-            o[x][d][0] *= alpha[x][0], o[x][d][1] *= alpha[x][1];
-            o[x][d][2] *= alpha[x][0], o[x][d][3] *= alpha[x][1];
-          }
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < kTiles; ++d) {
-        uint32_t a[4];
-        if (d < 4 * kV64) {
-          const int b = d / 4, i = d % 4, h = i % 2;
-          a[0] = pair(vr[0].b64[b][i / 2], vr[1].b64[b][i / 2], h), a[1] = pair(vr[0].b64[b][i / 2 + 2], vr[1].b64[b][i / 2 + 2], h);
-          a[2] = pair(vr[2].b64[b][i / 2], vr[3].b64[b][i / 2], h), a[3] = pair(vr[2].b64[b][i / 2 + 2], vr[3].b64[b][i / 2 + 2], h);
-        } else if (d < 4 * kV64 + 2 * kV32) {
-          const int h = d % 2;
-          a[0] = pair(vr[0].b32[0][0], vr[1].b32[0][0], h), a[1] = pair(vr[0].b32[0][1], vr[1].b32[0][1], h);
-          a[2] = pair(vr[2].b32[0][0], vr[3].b32[0][0], h), a[3] = pair(vr[2].b32[0][1], vr[3].b32[0][1], h);
-        } else {
-          a[0] = pair(vr[0].b16[0][0], vr[1].b16[0][0], 0), a[1] = pair(vr[0].b16[0][0], vr[1].b16[0][0], 1);
-          a[2] = pair(vr[2].b16[0][0], vr[3].b16[0][0], 0), a[3] = pair(vr[2].b16[0][0], vr[3].b16[0][0], 1);
-        }
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          Half<T>::mma(o[x][d], a, hi[x][0], hi[x][1]);
-          Half<T>::mma(o[x][d], a, lo[x][0], lo[x][1]);
-        }
-      }
-      if (j + 1 < n) { load_values(vp); }
-    }
-
-    constexpr int kRow = D + 4, kPitch = 8 * NT * kRow;
-    any = __any_sync(~0u, any);
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float* to = sums + warp * kPitch + (x * 8 + t4 * 2 + c) * kRow;
-#pragma unroll
-        for (int d = 0; d < kTiles; ++d) {
-          // the coordinates of rows g8 and g8 + 8 of product d
-          int at, step;
-          if (d < 4 * kV64) {
-            at = d / 4 * 64 + g8 * 8 + d % 4, step = 4;
-          } else if (d < 4 * kV64 + 2 * kV32) {
-            at = kV64 * 64 + g8 * 4 + d % 2, step = 2;
-          } else {
-            at = kV64 * 64 + kV32 * 32 + g8 * 2, step = 1;
-          }
-          to[at]        = o[x][d][c];
-          to[at + step] = o[x][d][c + 2];
-        }
-        const float sum = sum_over_keys(l[x][c]);
-        if (g8 == 0) { to[D] = m[x][c], to[D + 1] = sum, to[D + 2] = any ? 1.f : 0.f; }
-      }
-    }
-    finish_segment<T, D>(p, g, sums, kPitch, Half<T>::kRaise);
-  });
-}
-
-// Wider heads do not fit the registers that way: their tiles are copied into a ring in shared memory that belongs to a warp.
-template <int D>  // the head dimension, padded to what the tiles are built for
-struct HalfTile {
-  static constexpr int kPitch = D * 2 + 16;  // bytes of a row in shared memory: eight rows start in eight different banks
-  static constexpr int kBytes = kKeys * kPitch;
-  static constexpr int kWarp  = kStages * 2 * kBytes;
-  static constexpr int kAll   = kWarps * kWarp;
-  static constexpr int kLanes = 32;           // lanes that copy a row
-};
-
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) attend_ring_kernel(const Params p)
-{
-  using Tile = HalfTile<D>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
-  unsigned char* ring = smem + warp * Tile::kWarp;
-  const uint32_t ring_at = smem_of(ring);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (p.dim < D) {
-    // the columns behind the last coordinate are multiplied by zeros of the queries: they must hold numbers
-    for (int i = lane * 16; i < Tile::kWarp; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
-    __syncwarp();
-  }
-
-  for_segments<T>(p, [&](const Segment& g) {
-    // the queries, as the 8-column side of the first product
-    uint32_t qf[NT][D / 16][2];
-    {
-      const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int i  = n * 8 + g8;
-        const T* row = q + i * p.q_head;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c = k * 16 + h * 8 + t4 * 2;
-            uint32_t v  = 0;
-            if (i < g.n_heads && c < p.dim) {
-              const auto a = *reinterpret_cast<const uint16_t*>(row + c), b = *reinterpret_cast<const uint16_t*>(row + c + 1);
-              v            = a | (uint32_t(b) << 16);
-            }
-            qf[n][k][h] = v;
-          }
-        }
-      }
-    }
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) { o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f; }
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
-    }
-
-    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(T);
-    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(T);
-    // tiles of this warp: warp, warp + kWarps, ...
-    const int tiles = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
-    const int n     = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-    // the place of key lane % 16 of the next tile to be copied
-    Place at{kNowhere, kNowhere};
-    auto look_up = [&](int j) {
-      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
-      at              = j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
-    };
-    uint32_t masks = 0;  // of the tiles in the ring: which keys are real, newest lowest
-    uint32_t older = 0;
-    auto copy = [&](int stage) {
-      constexpr int kRows = 32 / Tile::kLanes;  // rows that the warp copies at once
-      const int chunk = lane % Tile::kLanes, sub = lane / Tile::kLanes;
-      const uint32_t to = ring_at + stage * 2 * Tile::kBytes + chunk * 16;
-      const bool inside = chunk * 8 < p.dim;
-#pragma unroll
-      for (int r = 0; r < kKeys; r += kRows) {
-        const int row     = r + sub;
-        const uint32_t ka = __shfl_sync(~0u, at.k, row), va = __shfl_sync(~0u, at.v, row);
-        const bool ok     = ka != kNowhere;
-        if (inside) {
-          copy16(to + row * Tile::kPitch, keys + (ok ? static_cast<uint64_t>(ka) << p.unit_shift : 0) + chunk * 16, ok);
-          copy16(to + Tile::kBytes + row * Tile::kPitch, values + (ok ? static_cast<uint64_t>(va) << p.unit_shift : 0) + chunk * 16, ok);
-        }
-      }
-      older = masks >> 16;
-      masks = (masks << 16) | (__ballot_sync(~0u, at.k != kNowhere) & 0xffffu);
-    };
-    bool any = false;
-    look_up(0);
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      copy(s);
-      copy_commit();
-      look_up(s + 1);
-    }
-    int stage = 0;
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      copy_wait<kStages - 2>();
-      __syncwarp();
-      copy(stage == 0 ? kStages - 1 : stage - 1);
-      copy_commit();
-      look_up(j + kStages);
-      const uint32_t mask = older & 0xffffu;  // kStages - 1 = 2 tiles were copied behind this one
-      any                 = any || mask != 0;
-      const uint32_t k_tile = ring_at + stage * 2 * Tile::kBytes, v_tile = k_tile + Tile::kBytes;
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-
-      float s[NT][4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) { s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f; }
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        uint32_t a[4];
-        load_matrix(a, k_tile + (lane % 16) * Tile::kPitch + (k * 2 + lane / 16) * 16);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) { Half<T>::mma(s[i], a, qf[i][k][0], qf[i][k][1]); }
-      }
-      const bool see0 = mask >> g8 & 1, see1 = mask >> (g8 + 8) & 1;
-      uint32_t hi[NT][2], lo[NT][2];
-      bool grew = false;
-      float alpha[NT][2];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) { grew |= soften<T>(s[i], p.scale, see0, see1, m[i], l[i], alpha[i], hi[i], lo[i]); }
-      if (__any_sync(~0u, grew)) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            o[i][d][0] *= alpha[i][0], o[i][d][1] *= alpha[i][1];
-            o[i][d][2] *= alpha[i][0], o[i][d][3] *= alpha[i][1];
-          }
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        uint32_t a[4];
-        load_matrix_t(a, v_tile + (lane % 8 + (lane / 16) * 8) * Tile::kPitch + (d * 2 + lane / 8 % 2) * 16);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          Half<T>::mma(o[i][d], a, hi[i][0], hi[i][1]);
-          Half<T>::mma(o[i][d], a, lo[i][0], lo[i][1]);
-        }
-      }
-    }
-    copy_wait<0>();
-    __syncwarp();
-
-    // the warps' results meet in shared memory, each in its own ring
-    constexpr int kRow = D + 4;
-    auto* sums         = reinterpret_cast<float*>(ring);  // [8 NT][kRow]: output, m, l, any
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float* to = sums + (i * 8 + t4 * 2 + c) * kRow;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          to[d * 16 + g8]     = o[i][d][c];
-          to[d * 16 + g8 + 8] = o[i][d][c + 2];
-        }
-        const float sum = sum_over_keys(l[i][c]);
-        if (g8 == 0) { to[D] = m[i][c], to[D + 1] = sum, to[D + 2] = any ? 1.f : 0.f; }
-      }
-    }
-    finish_segment<T, D>(p, g, reinterpret_cast<const float*>(smem), Tile::kWarp / 4, Half<T>::kRaise);
-    if (p.dim < D) {
-      for (int i = lane * 16; i < Tile::kWarp; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
-      __syncwarp();
-    }
-  });
-}
-
-// ------------------------------------------------------------------------------------------------ float32
-// No tensor core keeps float32's products, so this is fused multiply-adds, two at a time (fma.f32x2). Keys lie in registers like
-// above, four lanes per key with 16 bytes in a row each; the queries come from shared memory, one read for both keys of a lane.
-// The four lanes' parts of a score are added while the queries are dealt out to them. For the second product a lane owns four
-// coordinates of every value, and the weights come from shared memory. 830 instructions per tile of 16 KB (8 queries, d = 128).
-__device__ __forceinline__ void fma2(float2& d, float2 a, float2 b)
-{
-  auto& x = reinterpret_cast<unsigned long long&>(d);
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(x) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-}
-
-template <int D, int Q>
-struct FloatTile {
-  static constexpr int kPer    = D <= 128 ? 2 : 1;      // keys of a lane
-  static constexpr int kKeys   = 8 * kPer;              // of a tile
-  static constexpr int kChunks = D / 16;                // 16-byte parts of a key that a lane holds
-  static constexpr int kRows   = D <= 64 ? 2 : 1;       // values that the warp reads at once
-  static constexpr int kWide   = D <= 128 ? 1 : D / 128;  // 16-byte parts of a value that a lane holds
-  static constexpr int kOwn    = Q >= 4 ? Q / 4 : 1;    // queries whose softmax a lane does
-  static constexpr int kWeights = 2 * Q * kKeys + (Q < 4 ? 4 : Q);  // floats of a warp: weights, twice each for fma2, and factors
-  static constexpr int kSums   = Q * (D + 4);           // of a warp: what it found
-  static constexpr int kBytes  = 4 * (Q * D + kWarps * (kWeights + kSums));
-};
-
-/// D: the head dimension, padded; Q: queries of a unit, padded to 1, 4 or 8.
-template <int D, int Q>
-__global__ void __launch_bounds__(kThreads, 2) attend_float_kernel(const Params p)
-{
-  using Tile = FloatTile<D, Q>;
-  constexpr int kPer = Tile::kPer, kKeys = Tile::kKeys, kChunks = Tile::kChunks, kRows = Tile::kRows, kWide = Tile::kWide, kOwn = Tile::kOwn;
-  extern __shared__ __align__(16) float shared[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
-  float* q_s     = shared;                                            // [Q][D]
-  float* weights = q_s + Q * D + warp * Tile::kWeights;               // [Q][keys][2]
-  float* factors = weights + 2 * Q * kKeys;                           // [Q]
-  float* sums    = q_s + Q * D + kWarps * Tile::kWeights;             // [warps][Q][D + 4]
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  for_segments<float>(p, [&](const Segment& g) {
-    const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(float) + t4 * 16;
-    const int column   = D <= 64 ? lane % 16 * 4 : lane * 4;  // the lane's first coordinate of a value
-    const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(float) + column * 4;
-    const int tiles    = static_cast<int>((g.i1 - g.i0 + kKeys - 1) / kKeys);
-    const int n        = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-    auto look_up       = [&](int j) {
-      const int64_t i = g.i0 + int64_t(warp + j * kWarps) * kKeys + lane % kKeys;
-      return j < n && i < g.i1 ? place_of(p, g, i) : Place{kNowhere, kNowhere};
-    };
-    Place now = look_up(0), next = look_up(1);
-    const float* q = static_cast<const float*>(p.q) + g.row * p.q_row + g.head * p.q_head;
-    for (int i = threadIdx.x; i < Q * D; i += kThreads) {
-      const int x = i / D, c = i % D;
-      q_s[i] = x < g.n_heads && c < p.dim ? q[x * p.q_head + c] : 0.f;
-    }
-    __syncthreads();
-
-    float4 kr[kPer][kChunks], vr[kKeys / kRows][kWide];
-#pragma unroll
-    for (int x = 0; x < kPer; ++x) {
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) { kr[x][c] = float4{0.f, 0.f, 0.f, 0.f}; }
-    }
-#pragma unroll
-    for (int x = 0; x < kKeys / kRows; ++x) {
-#pragma unroll
-      for (int c = 0; c < kWide; ++c) { vr[x][c] = float4{0.f, 0.f, 0.f, 0.f}; }
-    }
-    auto at_of     = [&](uint32_t place) { return static_cast<uint64_t>(place == kNowhere ? 0 : place) << p.unit_shift; };
-    auto load_keys = [&](const Place& at) {
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) {
-        const char* from = keys + at_of(__shfl_sync(~0u, at.k, g8 + 8 * x));
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          if (c * 16 + t4 * 4 < p.dim) { read_once<4>(reinterpret_cast<uint32_t(&)[4]>(kr[x][c]), from + c * 64); }
-        }
-      }
-    };
-    auto load_values = [&](const Place& at) {
-#pragma unroll
-      for (int x = 0; x < kKeys / kRows; ++x) {
-        const char* from = values + at_of(__shfl_sync(~0u, at.v, x * kRows + (kRows == 2 ? lane / 16 : 0)));
-#pragma unroll
-        for (int c = 0; c < kWide; ++c) {
-          if (column + c * 128 < p.dim) { read_once<4>(reinterpret_cast<uint32_t(&)[4]>(vr[x][c]), from + c * 512); }
-        }
-      }
-    };
-
-    float2 o[Q][kWide][2];
-    float m[kOwn], l[kOwn];
-#pragma unroll
-    for (int i = 0; i < Q; ++i) {
-#pragma unroll
-      for (int c = 0; c < kWide; ++c) { o[i][c][0] = o[i][c][1] = float2{0.f, 0.f}; }
-    }
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) { m[i] = -INFINITY, l[i] = 0.f; }
-    bool any = false;
-    if (n > 0) {
-      load_keys(now);
-      load_values(now);
-    }
-    uint32_t seen = __ballot_sync(~0u, now.k != kNowhere);  // bit i: key i of the tile
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      float s[Q][kPer];
-      {
-        float2 sum[Q][kPer];
-#pragma unroll
-        for (int i = 0; i < Q; ++i) {
-#pragma unroll
-          for (int x = 0; x < kPer; ++x) { sum[i][x] = float2{0.f, 0.f}; }
-        }
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-          for (int i = 0; i < Q; ++i) {
-            const float4 w = *reinterpret_cast<const float4*>(q_s + i * D + c * 16 + t4 * 4);
-#pragma unroll
-            for (int x = 0; x < kPer; ++x) {
-              fma2(sum[i][x], float2{w.x, w.y}, float2{kr[x][c].x, kr[x][c].y});
-              fma2(sum[i][x], float2{w.z, w.w}, float2{kr[x][c].z, kr[x][c].w});
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < Q; ++i) {
-#pragma unroll
-          for (int x = 0; x < kPer; ++x) { s[i][x] = sum[i][x].x + sum[i][x].y; }
-        }
-      }
-      const uint32_t mask = seen;
-      any                 = any || (mask & ((1u << kKeys) - 1)) != 0;
-      if (j + 1 < n) { load_keys(next); }
-      seen = __ballot_sync(~0u, next.k != kNowhere);
-      now  = next;
-      next = look_up(j + 2);
-
-      // the four lanes of a key add their parts; with four queries or more each ends with its own queries
-      if constexpr (Q >= 4) {
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-#pragma unroll
-          for (int i = 0; i < Q / 2; ++i) {
-            const float mine = t4 & 2 ? s[i + Q / 2][x] : s[i][x], other = t4 & 2 ? s[i][x] : s[i + Q / 2][x];
-            s[i][x] = mine + __shfl_xor_sync(~0u, other, 2);
-          }
-#pragma unroll
-          for (int i = 0; i < Q / 4; ++i) {
-            const float mine = t4 & 1 ? s[i + Q / 4][x] : s[i][x], other = t4 & 1 ? s[i][x] : s[i + Q / 4][x];
-            s[i][x] = mine + __shfl_xor_sync(~0u, other, 1);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          s[0][x] += __shfl_xor_sync(~0u, s[0][x], 2);
-          s[0][x] += __shfl_xor_sync(~0u, s[0][x], 1);
-        }
-      }
-      const int own = Q >= 4 ? t4 * kOwn : 0;  // the lane's first query
-      bool grew     = false;
-      float alpha[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          s[i][x] = mask >> (g8 + 8 * x) & 1 ? s[i][x] * p.scale : -INFINITY;
-          top     = fmaxf(top, s[i][x]);
-        }
-        top              = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-        top              = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-        top              = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-        top              = fmaxf(top, m[i]);
-        const float base = top == -INFINITY ? 0.f : top;
-        alpha[i]         = exp2_fast(m[i] - base);
-        grew             = grew || top > m[i];
-        m[i]             = top;
-        l[i] *= alpha[i];
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          const float w = exp2_fast(s[i][x] - base);
-          l[i] += w;
-          if (Q >= 4 || t4 == 0) { *reinterpret_cast<float2*>(weights + 2 * ((own + i) * kKeys + g8 + 8 * x)) = float2{w, w}; }
-        }
-      }
-      if (__any_sync(~0u, grew)) {
-        if (g8 == 0) {
-#pragma unroll
-          for (int i = 0; i < kOwn; ++i) { factors[own + i] = alpha[i]; }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < Q; ++i) {
-          const float f = factors[i];
-#pragma unroll
-          for (int c = 0; c < kWide; ++c) {
-            o[i][c][0].x *= f, o[i][c][0].y *= f;
-            o[i][c][1].x *= f, o[i][c][1].y *= f;
-          }
-        }
-      }
-      __syncwarp();
-      if ((mask & ((1u << kKeys) - 1)) != (1u << kKeys) - 1) {
-#pragma unroll
-        for (int x = 0; x < kKeys / kRows; ++x) {
-          if (!(mask >> (x * kRows + (kRows == 2 ? lane / 16 : 0)) & 1)) {
-#pragma unroll
-            for (int c = 0; c < kWide; ++c) { vr[x][c] = float4{0.f, 0.f, 0.f, 0.f}; }
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < Q; ++i) {
-#pragma unroll
-        for (int x = 0; x < kKeys / kRows; x += 2) {
-          // the weights of two values of the lane
-          float2 w[2];
-          if constexpr (kRows == 1) {
-            const float4 both = *reinterpret_cast<const float4*>(weights + 2 * (i * kKeys + x));
-            w[0] = float2{both.x, both.y}, w[1] = float2{both.z, both.w};
-          } else {
-            w[0] = *reinterpret_cast<const float2*>(weights + 2 * (i * kKeys + x * 2 + lane / 16));
-            w[1] = *reinterpret_cast<const float2*>(weights + 2 * (i * kKeys + x * 2 + 2 + lane / 16));
-          }
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-#pragma unroll
-            for (int c = 0; c < kWide; ++c) {
-              fma2(o[i][c][0], w[y], float2{vr[x + y][c].x, vr[x + y][c].y});
-              fma2(o[i][c][1], w[y], float2{vr[x + y][c].z, vr[x + y][c].w});
-            }
-          }
-        }
-      }
-      __syncwarp();
-      if (j + 1 < n) { load_values(now); }
-    }
-
-    float* mine = sums + warp * Tile::kSums;
-#pragma unroll
-    for (int i = 0; i < Q; ++i) {
-#pragma unroll
-      for (int c = 0; c < kWide; ++c) {
-        float4 v{o[i][c][0].x, o[i][c][0].y, o[i][c][1].x, o[i][c][1].y};
-        if constexpr (kRows == 2) {
-          v.x += __shfl_xor_sync(~0u, v.x, 16), v.y += __shfl_xor_sync(~0u, v.y, 16);
-          v.z += __shfl_xor_sync(~0u, v.z, 16), v.w += __shfl_xor_sync(~0u, v.w, 16);
-        }
-        if (column + c * 128 < D) { *reinterpret_cast<float4*>(mine + i * (D + 4) + column + c * 128) = v; }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      const float sum = sum_over_keys(l[i]);
-      if (g8 == 0 && (Q >= 4 || t4 == 0)) {
-        float* to = mine + ((Q >= 4 ? t4 * kOwn : 0) + i) * (D + 4) + D;
-        to[0] = m[i], to[1] = sum, to[2] = any ? 1.f : 0.f;
-      }
-    }
-    finish_segment<float, D>(p, g, sums, Tile::kSums, 0.f);
-  });
-}
-
-// ------------------------------------------------------------------------------------------------ joining the shares
-// Block (x, i, z): joins the partial results of the unit that worker x left unfinished, or of unit x, for query i and coordinates
-// 4 * join_lanes * z on. They lie in the second slot of the worker w that began the unit and in the first slots of those behind it. A chain of three reads (mark, sums, outputs) is all its time,
-// so every thread reads at once what it needs: one share's sums, then four coordinates of every eighth share.
-constexpr int kJoinThreads = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p)
-{
-  extern __shared__ float weight[];  // [workers]
-  __shared__ float red[3][kJoinThreads / 32];
-  __shared__ float4 outs[kJoinThreads];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int i = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int n = static_cast<int>(p.marks[2 * blockIdx.x + 1]);
-  if (n == 0) { return; }
-  const int64_t mark = p.marks[2 * blockIdx.x];
-  const int64_t id   = p.by_unit ? blockIdx.x : mark;
-  const int w        = static_cast<int>(p.by_unit ? mark : blockIdx.x);
-  const int64_t row = id / p.units;
-  const Segment g   = segment_of(p, row, Span{0, 0, 0}, static_cast<int>(id - row * p.units));
-  if (i >= g.n_heads) { return; }
-  auto part = [&](int x) { return p.parts + (x == 0 ? 2 * int64_t(w) + 1 : 2 * int64_t(w + x)) * p.part_floats; };
-  // the largest m of all, then the weights, the sum and whether anything was seen
-  float top = -INFINITY;
-  for (int x = threadIdx.x; x < n; x += kJoinThreads) {
-    weight[x] = part(x)[4 * i];
-    top       = fmaxf(top, weight[x]);
-  }
-  for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, o)); }
-  if (lane == 0) { red[0][warp] = top; }
-  __syncthreads();
-  for (float r : red[0]) { top = fmaxf(top, r); }
-  float sum = 0.f, seen = 0.f;
-  for (int x = threadIdx.x; x < n; x += kJoinThreads) {
-    const float* from = part(x) + 4 * i;
-    weight[x]         = top == -INFINITY ? 1.f : exp2_fast(weight[x] - top);
-    sum += weight[x] * from[1];
-    seen += from[2];
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(~0u, sum, o);
-    seen += __shfl_xor_sync(~0u, seen, o);
-  }
-  if (lane == 0) { red[1][warp] = sum, red[2][warp] = seen; }
-  __syncthreads();
-  sum = seen = 0.f;
-  for (int x = 0; x < kJoinThreads / 32; ++x) { sum += red[1][x], seen += red[2][x]; }
-  const int lanes = p.join_lanes, groups = kJoinThreads / lanes, from_c = blockIdx.z * lanes * 4;
-  const int c = from_c + threadIdx.x % lanes * 4, first = threadIdx.x / lanes;
-  float4 v{0.f, 0.f, 0.f, 0.f};
-  if (c < p.dim) {
-#pragma unroll 8
-    for (int x = first; x < n; x += groups) {
-      const float4 o = *reinterpret_cast<const float4*>(part(x) + 4 * p.per_unit + i * p.dim + c);
-      const float f  = weight[x];
-      v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
-    }
-  }
-  outs[threadIdx.x] = v;
-  __syncthreads();
-  for (int x = threadIdx.x; x < min(lanes * 4, p.dim - from_c); x += kJoinThreads) {
-    float r = 0.f;
-    for (int y = 0; y < groups; ++y) { r += reinterpret_cast<const float*>(outs + y * lanes)[x]; }
-    (static_cast<T*>(p.out) + row * p.o_row + (g.head + i) * p.o_head)[from_c + x] = Type<T>::down(seen > 0.f ? r / sum : 0.f);
-  }
-  if (p.lse && threadIdx.x == 0 && blockIdx.z == 0) { p.lse[row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
-}
-
-// ------------------------------------------------------------------------------------------------ launch
-/// Units whose rows see at most so many tokens, as far as the host can tell, get a block each.
-constexpr int64_t kDirectTokens = 512;
+/// Shares at most: what the joining kernel's threads read the sums of.
+constexpr int64_t kMostShares = kJoinSums * kJoinThreads;
+/// Tokens that a block of a cluster goes through at most, as far as the host can tell from the width of the table. Without a split
+/// there is one launch and no second pass over partial results, but a block's time is that of the longest row.
+constexpr int64_t kClusterTokens = 192;
 
 struct Plan {
   int32_t per_unit, subs, units;
-  int direct;
-  int64_t blocks;
-  int part_floats, by_unit;
+  int cluster;
+  int64_t blocks, shares;
+  int part_floats, by_unit, abreast;
   size_t bytes;
 };
 
@@ -1288,13 +34,20 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   n.units          = static_cast<int32_t>(a.cache.n_kv_heads) * n.subs;
   int64_t most     = a.n_lists > 0 ? a.k : a.table.pages_per_sequence * a.cache.page_size;
   if (a.n_lists == 0 && a.window > 0) { most = std::min(most, a.window); }
-  const int64_t units = a.n_rows * n.units;
-  n.direct            = most <= kDirectTokens;
-  const int resident  = sm_count * (half ? (dim > 128 ? 1 : n.per_unit <= 8 ? 3 : 2) : 2);
-  n.blocks            = n.direct ? units : std::min<int64_t>(resident, units * ((most + kStep - 1) / kStep + kLead));
-  n.part_floats       = n.per_unit * (dim + 4);
-  n.bytes             = n.direct ? 0 : static_cast<size_t>(n.blocks) * 2 * (8 + sizeof(float) * n.part_floats);
-  n.by_unit           = units <= n.blocks;
+  const int64_t units = a.n_rows * n.units, steps = (most + kStep - 1) / kStep;
+  const int64_t warps    = int64_t(sm_count) * (half ? (dim > 128 ? 4 : n.per_unit <= 8 ? 12 : 8) : 8);  // resident ones
+  // as many blocks of four warps per unit as fill the GPU, with 64 tokens each at least
+  n.cluster = 1;
+  while (n.cluster < 8 && units * n.cluster * 8 <= warps && n.cluster * 64 < most) { n.cluster *= 2; }
+  if (most > kClusterTokens * n.cluster) { n.cluster = 0; }
+  const int64_t resident = warps / (half ? 2 : 1);
+  // units side by side, where that leaves few blocks without work; lists of positions have no common tokens
+  n.abreast = a.n_lists == 0 && n.units <= resident && resident % n.units * 16 <= resident ? n.units : 1;
+  n.shares  = std::min({resident / n.abreast, kMostShares, units / n.abreast * (steps + kLead)});
+  n.blocks  = n.cluster ? units * n.cluster : n.shares * n.abreast;
+  n.part_floats = n.per_unit * (dim + 4);
+  n.bytes       = n.cluster ? 0 : static_cast<size_t>(n.blocks) * 2 * (sizeof(float) * n.part_floats + sizeof(int64_t));
+  n.by_unit     = units <= n.blocks;
   return n;
 }
 
@@ -1306,83 +59,6 @@ int unit_shift(const certexB200PagedCache_t& c)
   uint64_t all   = 0;
   for (int i = 0; i < 2; ++i) { all |= static_cast<uint64_t>(c.key_strides[i] * size) | static_cast<uint64_t>(c.value_strides[i] * size); }
   return all == 0 ? 4 : __builtin_ctzll(all);
-}
-
-template <typename Kernel>
-void launch(Kernel kernel, int smem, const Params& p, int64_t blocks, cudaStream_t s)
-{
-  if (smem > 40 * 1024) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
-  kernel<<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(p);
-}
-
-template <typename T, int D, bool PAD>
-void launch_direct(const Params& p, int64_t blocks, cudaStream_t s)
-{
-  constexpr int kSums = kWarps * 8 * (D + 4) * 4;
-  if (p.per_unit <= 8) {
-    launch(attend_direct_kernel<T, D, 1, PAD>, kSums, p, blocks, s);
-  } else {
-    launch(attend_direct_kernel<T, D, 2, PAD>, 2 * kSums, p, blocks, s);
-  }
-}
-
-template <typename T, int D>
-void launch_ring(const Params& p, int64_t blocks, cudaStream_t s)
-{
-  if (p.per_unit <= 8) {
-    launch(attend_ring_kernel<T, D, 1>, HalfTile<D>::kAll, p, blocks, s);
-  } else {
-    launch(attend_ring_kernel<T, D, 2>, HalfTile<D>::kAll, p, blocks, s);
-  }
-}
-
-template <typename T>
-void launch_half(const Params& p, int64_t blocks, cudaStream_t s)
-{
-  switch (p.dim) {
-    case 64: return launch_direct<T, 64, false>(p, blocks, s);
-    case 80: return launch_direct<T, 80, false>(p, blocks, s);
-    case 96: return launch_direct<T, 96, false>(p, blocks, s);
-    case 128: return launch_direct<T, 128, false>(p, blocks, s);
-  }
-  if (p.dim < 64) {
-    launch_direct<T, 64, true>(p, blocks, s);
-  } else if (p.dim < 128) {
-    launch_direct<T, 128, true>(p, blocks, s);
-  } else if (p.dim <= 192) {
-    launch_ring<T, 192>(p, blocks, s);
-  } else {
-    launch_ring<T, 256>(p, blocks, s);
-  }
-}
-
-template <int D>
-void launch_float(const Params& p, int64_t blocks, cudaStream_t s)
-{
-  if (p.per_unit == 1) {
-    launch(attend_float_kernel<D, 1>, FloatTile<D, 1>::kBytes, p, blocks, s);
-  } else if (p.per_unit <= 4) {
-    launch(attend_float_kernel<D, 4>, FloatTile<D, 4>::kBytes, p, blocks, s);
-  } else {
-    launch(attend_float_kernel<D, 8>, FloatTile<D, 8>::kBytes, p, blocks, s);
-  }
-}
-
-template <typename T>
-void launch_join(const Params& p, cudaStream_t s)
-{
-  cudaLaunchConfig_t c{};
-  const auto joined  = static_cast<unsigned>(p.by_unit ? p.n_rows * p.units : p.workers);
-  c.gridDim          = dim3(joined, static_cast<unsigned>(p.per_unit), static_cast<unsigned>((p.dim + p.join_lanes * 4 - 1) / (p.join_lanes * 4)));
-  c.blockDim         = dim3(kJoinThreads);
-  c.dynamicSmemBytes = sizeof(float) * static_cast<size_t>(p.workers);
-  c.stream           = s;
-  cudaLaunchAttribute early{};
-  early.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs                                          = &early;
-  c.numAttrs                                       = 1;
-  cudaLaunchKernelEx(&c, join_kernel<T>, p);
 }
 
 }  // namespace
@@ -1404,7 +80,7 @@ size_t paged_attend_workspace(const AttendArgs& a, int sm_count) { return plan_o
 void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
 {
   const Plan n = plan_of(a, sm_count);
-  Params p{};
+  AttendParams p{};
   p.keys            = a.cache.keys;
   p.values          = a.cache.values;
   p.unit_shift      = unit_shift(a.cache);
@@ -1448,31 +124,22 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.per_unit        = n.per_unit;
   p.units           = n.units;
   p.scale           = a.scale * kLog2e;
-  p.direct          = n.direct;
-  p.workers         = static_cast<int32_t>(n.blocks);
+  p.cluster         = n.cluster;
+  p.shares          = static_cast<int32_t>(n.shares);
+  p.abreast         = n.cluster ? 1 : n.abreast;
+  p.in_line         = n.units / n.abreast;
   p.by_unit         = n.by_unit;
-  // few units have many shares each: more blocks for each of them
-  p.join_lanes      = a.n_rows * n.units * n.per_unit <= sm_count ? 8 : p.dim <= 128 ? 32 : 64;
+  p.joints          = n.by_unit ? a.n_rows * n.units : n.shares * n.abreast;
+  const int64_t all = p.joints * n.per_unit;  // queries to be joined
+  p.join_lanes      = all > 4 * sm_count ? 0 : all <= sm_count ? 8 : p.dim <= 128 ? 32 : 64;
   p.part_floats     = n.part_floats;
   p.parts           = static_cast<float*>(a.workspace);
-  p.marks           = n.direct ? nullptr : reinterpret_cast<int64_t*>(p.parts + 2 * n.blocks * n.part_floats);
-  if (a.cache.dtype == kPagedF32) {
-    if (p.dim <= 64) {
-      launch_float<64>(p, n.blocks, s);
-    } else if (p.dim <= 96) {
-      launch_float<96>(p, n.blocks, s);
-    } else if (p.dim <= 128) {
-      launch_float<128>(p, n.blocks, s);
-    } else {
-      launch_float<256>(p, n.blocks, s);
-    }
-    if (!n.direct) { launch_join<float>(p, s); }
-  } else if (a.cache.dtype == kPagedF16) {
-    launch_half<__half>(p, n.blocks, s);
-    if (!n.direct) { launch_join<__half>(p, s); }
-  } else {
-    launch_half<__nv_bfloat16>(p, n.blocks, s);
-    if (!n.direct) { launch_join<__nv_bfloat16>(p, s); }
+  const bool one    = a.n_lists > 0 || a.n_rows == 1;
+  p.marks           = n.cluster || one ? nullptr : reinterpret_cast<int64_t*>(p.parts + 2 * n.blocks * n.part_floats);
+  switch (a.cache.dtype) {
+    case kPagedF32: return launch_attend_f32(p, n.blocks, s);
+    case kPagedF16: return launch_attend_f16(p, n.blocks, s);
+    default: return launch_attend_bf16(p, n.blocks, s);
   }
 }
 
