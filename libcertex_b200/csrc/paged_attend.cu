@@ -13,8 +13,13 @@ constexpr int64_t kMostShares = kJoinSums * kJoinThreads;
 /// there is one launch and no second pass over partial results, but a block's time is that of the longest row.
 constexpr int64_t kClusterTokens = 192;
 
+/// Shares of a unit, on average, from which blocks have four warps. Below that smaller blocks wait less for one another: 128 rows of
+/// 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), float32 keys of 16 rows 192 us with four and 175 with
+/// one. Above, there are too many results to join: one row and KV head of 131 072 keys took 30 us with two warps and 24 with four.
+constexpr int64_t kManyShares = 64;
+
 struct Plan {
-  int32_t per_unit, subs, units;
+  int32_t per_unit, subs, units, warps;
   int cluster;
   int64_t blocks, shares;
   int part_floats, by_unit, abreast;
@@ -40,7 +45,9 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   n.cluster = 1;
   while (n.cluster < 8 && units * n.cluster * 8 <= warps && n.cluster * 64 < most) { n.cluster *= 2; }
   if (most > kClusterTokens * n.cluster) { n.cluster = 0; }
-  const int64_t resident = warps / (half ? 2 : 1);
+  const int few          = half ? 2 : 1;  // warps of a small block
+  n.warps                = n.cluster || warps / few > kManyShares * units ? 4 : few;
+  const int64_t resident = warps / n.warps;
   // units side by side, where that leaves few blocks without work; lists of positions have no common tokens
   n.abreast = a.n_lists == 0 && n.units <= resident && resident % n.units * 16 <= resident ? n.units : 1;
   n.shares  = std::min({resident / n.abreast, kMostShares, units / n.abreast * (steps + kLead)});
@@ -125,6 +132,7 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.units           = n.units;
   p.scale           = a.scale * kLog2e;
   p.cluster         = n.cluster;
+  p.warps           = n.warps;
   p.shares          = static_cast<int32_t>(n.shares);
   p.abreast         = n.cluster ? 1 : n.abreast;
   p.in_line         = n.units / n.abreast;

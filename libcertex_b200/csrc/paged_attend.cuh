@@ -68,7 +68,8 @@ struct AttendParams {
   int32_t units;                           // of a row
   float scale;                             // in units of log2 e
   // the split
-  int32_t cluster;     // blocks of a unit, in a cluster; 0: the work is split evenly over `workers` blocks
+  int32_t warps;       // of a block
+  int32_t cluster;     // blocks of a unit, in a cluster; 0: the work is split evenly
   int32_t shares;      // that the work is split into at most
   int32_t abreast;     // blocks of a share: 1, or the units of a row
   int32_t in_line;     // units of a row that lie behind one another among the steps: units / abreast
@@ -1584,9 +1585,6 @@ void launch(Kernel kernel, int warps, int smem, const AttendParams& p, int64_t b
   cudaLaunchKernelEx(&c, kernel, p);
 }
 
-// Blocks of clusters have four warps, so that a short unit is spread over as many as there are. Where the work is split, smaller
-// blocks wait less for one another: 128 rows of 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), float32
-// keys of 16 rows 192 us with four and 175 with one.
 template <typename T, int D, bool PAD, int W>
 void launch_direct(const AttendParams& p, int64_t blocks, cudaStream_t s)
 {
@@ -1600,7 +1598,7 @@ void launch_direct(const AttendParams& p, int64_t blocks, cudaStream_t s)
 template <typename T, int D, bool PAD>
 void launch_direct(const AttendParams& p, int64_t blocks, cudaStream_t s)
 {
-  p.cluster ? launch_direct<T, D, PAD, 4>(p, blocks, s) : launch_direct<T, D, PAD, 2>(p, blocks, s);
+  p.warps == 4 ? launch_direct<T, D, PAD, 4>(p, blocks, s) : launch_direct<T, D, PAD, 2>(p, blocks, s);
 }
 
 template <typename T, int D, int W>
@@ -1615,7 +1613,7 @@ void launch_ring(const AttendParams& p, int64_t blocks, cudaStream_t s)
 template <typename T, int D>
 void launch_ring(const AttendParams& p, int64_t blocks, cudaStream_t s)
 {
-  p.cluster ? launch_ring<T, D, 4>(p, blocks, s) : launch_ring<T, D, 2>(p, blocks, s);
+  p.warps == 4 ? launch_ring<T, D, 4>(p, blocks, s) : launch_ring<T, D, 2>(p, blocks, s);
 }
 
 template <typename T>
@@ -1652,7 +1650,7 @@ void launch_float(const AttendParams& p, int64_t blocks, cudaStream_t s)
 template <int D>
 void launch_float(const AttendParams& p, int64_t blocks, cudaStream_t s)
 {
-  p.cluster ? launch_float<D, 4>(p, blocks, s) : launch_float<D, 1>(p, blocks, s);
+  p.warps == 4 ? launch_float<D, 4>(p, blocks, s) : launch_float<D, 1>(p, blocks, s);
 }
 
 template <typename T>

@@ -83,6 +83,12 @@ struct TurnArgs {
   int32_t* fault;
 };
 
+/// a / b for a >= 0, in 32 bits where they will do.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b)
+{
+  return (a | b) >> 31 ? a / b : int64_t(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+
 /// The sine and cosine of `turn` (in units of 2^-64 of a turn).
 template <bool EXACT>
 __device__ __forceinline__ void turn_sincos(uint64_t turn, float& s, float& c)
@@ -150,19 +156,6 @@ __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
   const Section<T> sec = which == 0 ? a.sec[0] : which == 1 ? a.sec[1] : a.sec[2];
 
   const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[row] : static_cast<const int32_t*>(a.positions)[row];
-  int64_t to        = row * sec.dst_row;
-  if (sec.paged) {
-    if (pos < 0) { return; }  // a row that holds no token
-    const int64_t b = a.table.row_to_sequence ? a.table.row_to_sequence[row] : row;
-    const int64_t p = pos / a.page_size;
-    int64_t page    = -1;
-    if (b >= 0 && b < a.table.n_sequences && p < a.table.pages_per_sequence) { page = a.table.pages[b * a.table.row_stride + p]; }
-    if (page < 0 || page >= a.n_pages) {
-      if (a.fault) { *a.fault = 1; }
-      return;
-    }
-    to = page * sec.dst_row + (pos - p * a.page_size) * sec.dst_token;
-  }
 
   // where the unit's two vectors lie, and its first pair
   const int turned = a.rotary_dim / (2 * V);  // units that are turned
@@ -172,6 +165,38 @@ __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
     lo = unit * V;
     hi = lo + a.rotary_dim / 2;
   }
+  using P           = Pack<T, V>;
+  const int first   = chunk * HEADS;
+  const T* from     = sec.src + row * sec.src_row + int64_t(first) * sec.src_head;
+  const int n       = min(HEADS, sec.heads - first);
+  constexpr int kAt = HEADS < 2 ? HEADS : 2;  // heads whose loads are in flight together
+  P x[kAt], y[kAt];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      if (h + j < n) {
+        x[j] = *reinterpret_cast<const P*>(from + j * sec.src_head + lo);
+        y[j] = *reinterpret_cast<const P*>(from + j * sec.src_head + hi);
+      }
+    }
+    from += kAt * sec.src_head;
+  };
+  load(0);  // on their way while the page is looked up
+
+  int64_t to = row * sec.dst_row;
+  if (sec.paged) {
+    if (pos < 0) { return; }  // a row that holds no token
+    const int64_t b = a.table.row_to_sequence ? a.table.row_to_sequence[row] : row;
+    const int64_t p = divide(pos, a.page_size);
+    int64_t page    = -1;
+    if (b >= 0 && b < a.table.n_sequences && p < a.table.pages_per_sequence) { page = a.table.pages[b * a.table.row_stride + p]; }
+    if (page < 0 || page >= a.n_pages) {
+      if (a.fault) { *a.fault = 1; }
+      return;
+    }
+    to = page * sec.dst_row + (pos - p * a.page_size) * sec.dst_token;
+  }
+  T* dst = sec.dst + to + int64_t(first) * sec.dst_head;
   float c[V], s[V];
   if (turn) {
 #pragma unroll
@@ -181,23 +206,9 @@ __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
       s[i] *= a.inverse ? -a.magnitude : a.magnitude;
     }
   }
-
-  using P           = Pack<T, V>;
-  const int first   = chunk * HEADS;
-  const T* from     = sec.src + row * sec.src_row + int64_t(first) * sec.src_head;
-  T* dst            = sec.dst + to + int64_t(first) * sec.dst_head;
-  const int n       = min(HEADS, sec.heads - first);
-  constexpr int kAt = HEADS < 2 ? HEADS : 2;  // heads whose loads are in flight together
 #pragma unroll 1
   for (int h = 0; h < n; h += kAt) {
-    P x[kAt], y[kAt];
-#pragma unroll
-    for (int j = 0; j < kAt; ++j) {
-      if (h + j < n) {
-        x[j] = *reinterpret_cast<const P*>(from + j * sec.src_head + lo);
-        y[j] = *reinterpret_cast<const P*>(from + j * sec.src_head + hi);
-      }
-    }
+    if (h > 0) { load(h); }
 #pragma unroll
     for (int j = 0; j < kAt; ++j) {
       if (h + j < n) {
@@ -206,7 +217,6 @@ __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
         *reinterpret_cast<P*>(dst + j * sec.dst_head + hi) = y[j];
       }
     }
-    from += kAt * sec.src_head;
     dst += kAt * sec.dst_head;
   }
 }
