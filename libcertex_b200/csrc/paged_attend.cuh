@@ -628,38 +628,46 @@ __device__ __forceinline__ void finish_segment(const AttendParams& p, const Segm
   cluster.sync();  // the others may still read this block's memory
 }
 
-/// The softmax of a tile's scores s (16 keys x 8 queries, as the first product leaves them), one group of eight queries:
+/// The softmax of a tile's scores s (R times 16 keys x 8 queries, as the first product leaves them), one group of eight queries:
 /// scores become weights as the second product's operand, m and l go on. Returns whether m grew (in this thread's queries).
-template <typename T>
-__device__ __forceinline__ bool soften(float (&s)[4], float scale, bool see0, bool see1, float (&m)[2], float (&l)[2], float (&alpha)[2],
-                                       uint32_t (&hi)[2], uint32_t (&lo)[2])
+template <typename T, int R>
+__device__ __forceinline__ bool soften(float (&s)[R][4], float scale, const bool (&see)[R][2], float (&m)[2], float (&l)[2], float (&alpha)[2],
+                                       uint32_t (&hi)[R][2], uint32_t (&lo)[R][2])
 {
   float base[2];
   bool grew = false;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    s[c]      = see0 ? s[c] * scale : -INFINITY;
-    s[c + 2]  = see1 ? s[c + 2] * scale : -INFINITY;
-    float top = fmaxf(s[c], s[c + 2]);
-    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-    top       = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-    top       = fmaxf(top, m[c]);
-    base[c]   = top == -INFINITY ? 0.f : top;
-    alpha[c]  = exp2_fast(m[c] - base[c]);
-    grew      = grew || top > m[c];
-    m[c]      = top;
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r][c]     = see[r][0] ? s[r][c] * scale : -INFINITY;
+      s[r][c + 2] = see[r][1] ? s[r][c + 2] * scale : -INFINITY;
+      top         = fmaxf(top, fmaxf(s[r][c], s[r][c + 2]));
+    }
+    top      = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+    top      = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+    top      = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+    top      = fmaxf(top, m[c]);
+    base[c]  = top == -INFINITY ? 0.f : top;
+    alpha[c] = exp2_fast(m[c] - base[c]);
+    grew     = grew || top > m[c];
+    m[c]     = top;
     base[c] -= Half<T>::kRaise;
+    l[c] *= alpha[c];
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c) { s[c] = exp2_fast(s[c] - base[c & 1]); }
-  l[0] = l[0] * alpha[0] + (s[0] + s[2]);
-  l[1] = l[1] * alpha[1] + (s[1] + s[3]);
-  Half<T>::split(s[0], s[1], hi[0], lo[0]);
-  Half<T>::split(s[2], s[3], hi[1], lo[1]);
-  // from keys by lanes to queries by lanes
-  hi[0] = transpose8x8(hi[0]), hi[1] = transpose8x8(hi[1]);
-  lo[0] = transpose8x8(lo[0]), lo[1] = transpose8x8(lo[1]);
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) { s[r][c] = exp2_fast(s[r][c] - base[c & 1]); }
+    l[0] += s[r][0] + s[r][2];
+    l[1] += s[r][1] + s[r][3];
+    Half<T>::split(s[r][0], s[r][1], hi[r][0], lo[r][0]);
+    Half<T>::split(s[r][2], s[r][3], hi[r][1], lo[r][1]);
+    // from keys by lanes to queries by lanes
+    hi[r][0] = transpose8x8(hi[r][0]), hi[r][1] = transpose8x8(hi[r][1]);
+    lo[r][0] = transpose8x8(lo[r][0]), lo[r][1] = transpose8x8(lo[r][1]);
+  }
   return grew;
 }
 
@@ -692,6 +700,10 @@ __device__ __forceinline__ void read_once(uint32_t (&r)[N], const char* at)
   }
 }
 
+/// Narrow heads take 32 keys at a time: as many bytes in flight, and half the steps of the softmax. 16 rows of 16 384 keys of 8 heads
+/// of 64: 116 us with 16 keys, 98 with 32; heads of 80: 131 and 128.
+constexpr int kDoubleDim = 80;
+
 /// A lane's share of a row's coordinates in blocks: 8 * E coordinates where every lane of eight (or 4 * E, of four) takes E.
 template <int N64, int N32, int N16>
 struct RowPart {
@@ -704,6 +716,7 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
   constexpr int kK32 = D / 32, kK16 = D % 32 / 16;                  // keys: blocks of 32 and 16 coordinates
   constexpr int kV64 = D / 64, kV32 = D % 64 / 32, kV16 = D % 32 / 16;  // values: of 64, 32 and 16
   constexpr int kSteps = 2 * kK32 + kK16, kTiles = 4 * kV64 + 2 * kV32 + kV16;
+  constexpr int R = D <= kDoubleDim ? 2 : 1, kKeys = 16 * R;  // keys of a tile
   extern __shared__ __align__(16) float sums[];  // [warps][8 NT][D + 4]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -713,11 +726,11 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
     const char* values = static_cast<const char*>(p.values) + g.kv * p.v_head * sizeof(T) + g8 * 16;
     const int i0 = g.i0, i1 = g.i1, begin = g.begin;
     const void* index  = g.index;
-    const int tiles    = (i1 - i0 + 15) / 16;
+    const int tiles    = (i1 - i0 + kKeys - 1) / kKeys;
     const int n        = tiles > warp ? (tiles - warp + W - 1) / W : 0;
 
-    // token lane % 16 of tile j, its entry and its place
-    auto token_of = [&](int j) { return i0 + (warp + j * W) * 16 + lane % 16; };
+    // token lane % kKeys of tile j, its entry and its place
+    auto token_of = [&](int j) { return i0 + (warp + j * W) * kKeys + lane % kKeys; };
     auto ask      = [&](int j) { return j < n && token_of(j) < i1 ? entry_of(p, begin, index, token_of(j)) : 0; };
     auto find     = [&](int j, int64_t entry) {
       return j < n && token_of(j) < i1 ? place_of(p, begin, token_of(j), entry) : Place{kNowhere, kNowhere};
@@ -756,12 +769,13 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
       l[x][0] = l[x][1] = 0.f;
     }
 
-    uint32_t kr[2][kK32 + kK16][4];  // keys g8 and g8 + 8
-    RowPart<kV64, kV32, kV16> vr[4];  // values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+    // of every sixteen keys: keys g8 and g8 + 8, values of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
+    uint32_t kr[2 * R][kK32 + kK16][4];
+    RowPart<kV64, kV32, kV16> vr[4 * R];
     auto at_of = [&](uint32_t place) { return static_cast<uint64_t>(place == kNowhere ? 0 : place) << p.unit_shift; };
-    auto load_keys = [&](const uint32_t (&place)[2]) {
+    auto load_keys = [&](const uint32_t (&place)[2 * R]) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < 2 * R; ++r) {
         const char* at = keys + at_of(place[r]);
 #pragma unroll
         for (int b = 0; b < kK32; ++b) {
@@ -774,9 +788,9 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
         }
       }
     };
-    auto load_values = [&](const uint32_t (&place)[4]) {
+    auto load_values = [&](const uint32_t (&place)[4 * R]) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < 4 * R; ++r) {
         const char* at = values + at_of(place[r]);
 #pragma unroll
         for (int b = 0; b < kV64; ++b) {
@@ -786,13 +800,13 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
         if constexpr (kV16 > 0) { read_once<1>(vr[r].b16[0], at + kV64 * 128 + kV32 * 64 - g8 * 12); }
       }
     };
-    auto keys_of = [&](const Place& x, uint32_t (&place)[2]) {
-      place[0] = __shfl_sync(~0u, x.k, g8);
-      place[1] = __shfl_sync(~0u, x.k, g8 + 8);
-    };
-    auto values_of = [&](const Place& x, uint32_t (&place)[4]) {
+    auto keys_of = [&](const Place& x, uint32_t (&place)[2 * R]) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) { place[r] = __shfl_sync(~0u, x.v, t4 * 2 + (r & 1) + (r & 2) * 4); }
+      for (int r = 0; r < 2 * R; ++r) { place[r] = __shfl_sync(~0u, x.k, g8 + 8 * r); }
+    };
+    auto values_of = [&](const Place& x, uint32_t (&place)[4 * R]) {
+#pragma unroll
+      for (int r = 0; r < 4 * R; ++r) { place[r] = __shfl_sync(~0u, x.v, r / 4 * 16 + t4 * 2 + (r & 1) + (r & 2) * 4); }
     };
     // a register of two neighbouring keys' values at one coordinate
     auto pair = [](uint32_t a, uint32_t b, int odd) { return __byte_perm(a, b, odd ? 0x7632 : 0x5410); };
@@ -800,17 +814,17 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
     if (PAD) {
       // what lies behind the last coordinate is never loaded, and must be a number
 #pragma unroll
-      for (int b = 0; b < kK32; ++b) {
+      for (int r = 0; r < 2 * R; ++r) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) { kr[0][b][x] = kr[1][b][x] = 0; }
+        for (int b = 0; b < kK32; ++b) { kr[r][b][0] = kr[r][b][1] = kr[r][b][2] = kr[r][b][3] = 0; }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < 4 * R; ++r) {
 #pragma unroll
         for (int b = 0; b < kV64; ++b) { vr[r].b64[b][0] = vr[r].b64[b][1] = vr[r].b64[b][2] = vr[r].b64[b][3] = 0; }
       }
     }
-    uint32_t kp[2], vp[4];
+    uint32_t kp[2 * R], vp[4 * R];
     bool any = false;
     if (n > 0) {
       const Place at = find(0, entry0);
@@ -822,28 +836,39 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       // where the next tile lies is worked out while this one's keys are on their way
-      const bool see0 = kp[0] != kNowhere, see1 = kp[1] != kNowhere;
-      const Place at  = find(j + 1, entry);
-      entry           = ask(j + 2);
-      keys_of(at, kp);
-      float s[NT][4];
+      bool see[R][2], all = true;
 #pragma unroll
-      for (int x = 0; x < NT; ++x) { s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f; }
+      for (int r = 0; r < R; ++r) {
+        see[r][0] = kp[2 * r] != kNowhere, see[r][1] = kp[2 * r + 1] != kNowhere;
+        any       = any || see[r][0] || see[r][1];
+        all       = all && see[r][0] && see[r][1];
+      }
+      const Place at = find(j + 1, entry);
+      entry          = ask(j + 2);
+      keys_of(at, kp);
+      float s[NT][R][4];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) { s[x][r][0] = s[x][r][1] = s[x][r][2] = s[x][r][3] = 0.f; }
+      }
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         const int b = k / 2, h = k % 2 * 2;
-        const uint32_t a[4] = {kr[0][b][h], kr[1][b][h], kr[0][b][h + 1], kr[1][b][h + 1]};
 #pragma unroll
-        for (int x = 0; x < NT; ++x) { Half<T>::mma(s[x], a, qf[x][k][0], qf[x][k][1]); }
+        for (int r = 0; r < R; ++r) {
+          const uint32_t a[4] = {kr[2 * r][b][h], kr[2 * r + 1][b][h], kr[2 * r][b][h + 1], kr[2 * r + 1][b][h + 1]};
+#pragma unroll
+          for (int x = 0; x < NT; ++x) { Half<T>::mma(s[x][r], a, qf[x][k][0], qf[x][k][1]); }
+        }
       }
-      any = any || see0 || see1;
       if (j + 1 < n) { load_keys(kp); }
 
-      uint32_t hi[NT][2], lo[NT][2];
+      uint32_t hi[NT][R][2], lo[NT][R][2];
       float alpha[NT][2];
       bool grew = false;
 #pragma unroll
-      for (int x = 0; x < NT; ++x) { grew |= soften<T>(s[x], p.scale, see0, see1, m[x], l[x], alpha[x], hi[x], lo[x]); }
+      for (int x = 0; x < NT; ++x) { grew |= soften<T, R>(s[x], p.scale, see, m[x], l[x], alpha[x], hi[x], lo[x]); }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -855,10 +880,9 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
         }
       }
       // every key of the tile is seen, or the values of those that are not become zeros
-      const bool full = __all_sync(~0u, see0 && see1);
-      if (!full) {
+      if (!__all_sync(~0u, all)) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 4 * R; ++r) {
           if (vp[r] == kNowhere) {
 #pragma unroll
             for (int b = 0; b < kV64; ++b) { vr[r].b64[b][0] = vr[r].b64[b][1] = vr[r].b64[b][2] = vr[r].b64[b][3] = 0; }
@@ -867,24 +891,28 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
         }
       }
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) {
-        uint32_t a[4];
-        if (d < 4 * kV64) {
-          const int b = d / 4, i = d % 4, h = i % 2;
-          a[0] = pair(vr[0].b64[b][i / 2], vr[1].b64[b][i / 2], h), a[1] = pair(vr[0].b64[b][i / 2 + 2], vr[1].b64[b][i / 2 + 2], h);
-          a[2] = pair(vr[2].b64[b][i / 2], vr[3].b64[b][i / 2], h), a[3] = pair(vr[2].b64[b][i / 2 + 2], vr[3].b64[b][i / 2 + 2], h);
-        } else if (d < 4 * kV64 + 2 * kV32) {
-          const int h = d % 2;
-          a[0] = pair(vr[0].b32[0][0], vr[1].b32[0][0], h), a[1] = pair(vr[0].b32[0][1], vr[1].b32[0][1], h);
-          a[2] = pair(vr[2].b32[0][0], vr[3].b32[0][0], h), a[3] = pair(vr[2].b32[0][1], vr[3].b32[0][1], h);
-        } else {
-          a[0] = pair(vr[0].b16[0][0], vr[1].b16[0][0], 0), a[1] = pair(vr[0].b16[0][0], vr[1].b16[0][0], 1);
-          a[2] = pair(vr[2].b16[0][0], vr[3].b16[0][0], 0), a[3] = pair(vr[2].b16[0][0], vr[3].b16[0][0], 1);
-        }
+      for (int r = 0; r < R; ++r) {
+        const auto* v = vr + 4 * r;
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          Half<T>::mma(o[x][d], a, hi[x][0], hi[x][1]);
-          Half<T>::mma(o[x][d], a, lo[x][0], lo[x][1]);
+        for (int d = 0; d < kTiles; ++d) {
+          uint32_t a[4];
+          if (d < 4 * kV64) {
+            const int b = d / 4, i = d % 4, h = i % 2;
+            a[0] = pair(v[0].b64[b][i / 2], v[1].b64[b][i / 2], h), a[1] = pair(v[0].b64[b][i / 2 + 2], v[1].b64[b][i / 2 + 2], h);
+            a[2] = pair(v[2].b64[b][i / 2], v[3].b64[b][i / 2], h), a[3] = pair(v[2].b64[b][i / 2 + 2], v[3].b64[b][i / 2 + 2], h);
+          } else if (d < 4 * kV64 + 2 * kV32) {
+            const int h = d % 2;
+            a[0] = pair(v[0].b32[0][0], v[1].b32[0][0], h), a[1] = pair(v[0].b32[0][1], v[1].b32[0][1], h);
+            a[2] = pair(v[2].b32[0][0], v[3].b32[0][0], h), a[3] = pair(v[2].b32[0][1], v[3].b32[0][1], h);
+          } else {
+            a[0] = pair(v[0].b16[0][0], v[1].b16[0][0], 0), a[1] = pair(v[0].b16[0][0], v[1].b16[0][0], 1);
+            a[2] = pair(v[2].b16[0][0], v[3].b16[0][0], 0), a[3] = pair(v[2].b16[0][0], v[3].b16[0][0], 1);
+          }
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            Half<T>::mma(o[x][d], a, hi[x][r][0], hi[x][r][1]);
+            Half<T>::mma(o[x][d], a, lo[x][r][0], lo[x][r][1]);
+          }
         }
       }
       values_of(at, vp);
@@ -1033,22 +1061,22 @@ __global__ void __launch_bounds__(W * 32, 4 / W) attend_ring_kernel(const Attend
       const uint32_t k_tile = ring_at + stage * 2 * Tile::kBytes, v_tile = k_tile + Tile::kBytes;
       stage = stage + 1 == kStages ? 0 : stage + 1;
 
-      float s[NT][4];
+      float s[NT][1][4];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) { s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f; }
+      for (int i = 0; i < NT; ++i) { s[i][0][0] = s[i][0][1] = s[i][0][2] = s[i][0][3] = 0.f; }
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         uint32_t a[4];
         load_matrix(a, k_tile + (lane % 16) * Tile::kPitch + (k * 2 + lane / 16) * 16);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) { Half<T>::mma(s[i], a, qf[i][k][0], qf[i][k][1]); }
+        for (int i = 0; i < NT; ++i) { Half<T>::mma(s[i][0], a, qf[i][k][0], qf[i][k][1]); }
       }
-      const bool see0 = mask >> g8 & 1, see1 = mask >> (g8 + 8) & 1;
-      uint32_t hi[NT][2], lo[NT][2];
+      const bool see[1][2] = {{(mask >> g8 & 1) != 0, (mask >> (g8 + 8) & 1) != 0}};
+      uint32_t hi[NT][1][2], lo[NT][1][2];
       bool grew = false;
       float alpha[NT][2];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) { grew |= soften<T>(s[i], p.scale, see0, see1, m[i], l[i], alpha[i], hi[i], lo[i]); }
+      for (int i = 0; i < NT; ++i) { grew |= soften<T, 1>(s[i], p.scale, see, m[i], l[i], alpha[i], hi[i], lo[i]); }
       if (__any_sync(~0u, grew)) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -1065,8 +1093,8 @@ __global__ void __launch_bounds__(W * 32, 4 / W) attend_ring_kernel(const Attend
         load_matrix_t(a, v_tile + (lane % 8 + (lane / 16) * 8) * Tile::kPitch + (d * 2 + lane / 8 % 2) * 16);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          Half<T>::mma(o[i][d], a, hi[i][0], hi[i][1]);
-          Half<T>::mma(o[i][d], a, lo[i][0], lo[i][1]);
+          Half<T>::mma(o[i][d], a, hi[i][0][0], hi[i][0][1]);
+          Half<T>::mma(o[i][d], a, lo[i][0][0], lo[i][0][1]);
         }
       }
     }
