@@ -10,8 +10,9 @@ namespace {
 /// Shares at most: what the joining kernel's threads read the sums of.
 constexpr int64_t kMostShares = kJoinSums * kJoinThreads;
 /// Tokens that a block of a cluster goes through at most, as far as the host can tell from the width of the table. Without a split
-/// there is one launch and no second pass over partial results, but a block's time is that of the longest row.
-constexpr int64_t kClusterTokens = 192;
+/// there is one launch and no second pass over partial results, but a block's time is that of the longest row. Rows of 8 KV heads: 1 of
+/// 1000 keys 8.8 us in clusters and 10.1 split, 4 of 2000 14.4 and 19.5; with 512 tokens a block 1 of 4000 16.2 and 12.7.
+constexpr int64_t kClusterTokens = 256;
 
 /// Shares of a unit, on average, from which blocks have four warps. Below that smaller blocks wait less for one another: 128 rows of
 /// 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), float32 keys of 16 rows 192 us with four and 175 with

@@ -171,7 +171,7 @@ __device__ __forceinline__ Segment segment_of(const AttendParams& p, int64_t row
 {
   Segment g;
   g.row     = row;
-  g.kv      = unit / p.subs;
+  g.kv      = p.subs == 1 ? unit : unit / p.subs;
   const int sub = unit - g.kv * p.subs;
   g.head    = g.kv * p.group + sub * p.per_unit;
   g.n_heads = min(p.per_unit, p.group - sub * p.per_unit);
@@ -245,6 +245,7 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b)
 
 struct Split {
   int64_t total, shares, each, more;  // the first `more` shares have a step more than `each`
+  Split() = default;
   __device__ Split(int64_t steps, int64_t most) : total(steps), shares(min(most, steps)), each(0), more(0)
   {
     if (shares > 0) {
@@ -267,72 +268,89 @@ struct Unit {
   Span span;
 };
 
-/// Steps of all rows together; a block of THREADS threads calls it as a whole.
-template <int THREADS>
-__device__ __forceinline__ int64_t all_steps(const AttendParams& p)
-{
-  __shared__ int64_t sums[THREADS / 32];
-  if (!p.lengths) { return p.n_rows * steps_for(static_cast<int32_t>(p.k)) * p.in_line; }
-  if (p.n_rows == 1) { return steps_for(span_of(p, 0).count) * p.in_line; }
-  int64_t mine = 0;
-  for (int64_t row = threadIdx.x; row < p.n_rows; row += THREADS) { mine += steps_for(span_of(p, row).count); }
-  for (int o = 16; o > 0; o >>= 1) { mine += __shfl_xor_sync(~0u, mine, o); }
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) { sums[threadIdx.x / 32] = mine; }
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < THREADS / 32; ++w) { total += sums[w]; }
-  return total * p.in_line;
-}
+/// The split and where a block's share of it begins; a block of W warps calls it as a whole.
+struct Start {
+  Split split;
+  int64_t at;  // the share's first step
+  Unit unit;   // whose steps that is among; undefined when the split has not so many shares
+};
 
-/// The row that `step` is among the steps of, and the first step of that row.
-template <int THREADS>
-__device__ __forceinline__ Unit row_of_step(const AttendParams& p, int64_t step)
+template <int W>
+__device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
 {
-  __shared__ int64_t sums[THREADS / 32];
+  constexpr int kThreads = W * 32;
+  __shared__ int64_t sums[W];
   __shared__ int64_t found[2];
-  Unit u{0, 0, 0, 0, {0, 0, 0}};
-  if (!p.lengths || p.n_rows == 1) {
-    const int64_t each = steps_for(span_of(p, 0).count) * p.in_line;
-    u.row              = divide(step, each);
-    u.begin            = u.row * each;
-    return u;
+  __shared__ Span spans;
+  const bool alike = !p.lengths || p.n_rows == 1;  // every unit has the same steps
+  if (alike) {
+    const Span span     = span_of(p, 0);
+    const int64_t steps = steps_for(span.count), each = steps * p.in_line;
+    Start x{Split(p.n_rows * each, p.shares), 0, {0, 0, steps, 0, span}};
+    if (share >= x.split.shares) { return x; }
+    x.at         = x.split.first_step(share);
+    x.unit.row   = p.n_rows == 1 ? 0 : divide(x.at, each);
+    const auto u = divide(x.at - x.unit.row * each, steps);
+    x.unit.unit  = static_cast<int>(u);
+    x.unit.begin = x.unit.row * each + u * steps;
+    return x;
   }
+  // an inclusive sum over the block for kThreads rows at a time; the total first, where they are more
+  int64_t total = 0;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const bool once = p.n_rows <= kThreads;
+  if (!once) {
+    int64_t mine = 0;
+    for (int64_t row = threadIdx.x; row < p.n_rows; row += kThreads) { mine += steps_for(span_of(p, row).count); }
+    for (int o = 16; o > 0; o >>= 1) { mine += __shfl_xor_sync(~0u, mine, o); }
+    if (lane == 0) { sums[warp] = mine; }
+    __syncthreads();
+    for (int w = 0; w < W; ++w) { total += sums[w]; }
+    __syncthreads();
+  }
+  Start x{Split(total * p.in_line, p.shares), 0, {}};
+  if (!once) { x.at = x.split.first_step(share); }
   int64_t before = 0;
-  for (int64_t r0 = 0; r0 < p.n_rows && before <= step; r0 += THREADS) {
+  for (int64_t r0 = 0; r0 < p.n_rows; r0 += kThreads) {
     const int64_t r = r0 + threadIdx.x;
-    const int64_t n = r < p.n_rows ? steps_for(span_of(p, r).count) * p.in_line : 0;
-    int64_t upto    = n;  // inclusive sum over the warp
+    const Span span = r < p.n_rows ? span_of(p, r) : Span{0, 0, 0};
+    const int64_t n = steps_for(span.count) * p.in_line;
+    int64_t upto    = n;
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, upto, o);
-      if (threadIdx.x % 32 >= o) { upto += x; }
+      const int64_t y = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) { upto += y; }
     }
-    __syncthreads();
-    if (threadIdx.x % 32 == 31) { sums[threadIdx.x / 32] = upto; }
-    __syncthreads();
-    int64_t first = before;
-    for (int i = 0; i < THREADS / 32; ++i) {
-      if (i < threadIdx.x / 32) { first += sums[i]; }
-      before += sums[i];
+    if (W > 1) {
+      if (lane == 31) { sums[warp] = upto; }
+      __syncthreads();
     }
-    first += upto - n;
-    if (first <= step && step < first + n) { found[0] = r, found[1] = first; }
+    int64_t first = before + upto - n;
+    if (W > 1) {
+      for (int i = 0; i < W; ++i) {
+        if (i < warp) { first += sums[i]; }
+        before += sums[i];
+      }
+    } else {
+      before += __shfl_sync(~0u, upto, 31);
+    }
+    if (once) {
+      x.split = Split(before, p.shares);
+      x.at    = x.split.first_step(share);
+    }
+    if (first <= x.at && x.at < first + n) { found[0] = r, found[1] = first, spans = span; }
+    if (x.at < before) { break; }
+    if (W > 1) { __syncthreads(); }
   }
   __syncthreads();
-  u.row = found[0], u.begin = found[1];
-  return u;
-}
-
-/// The unit whose steps `step` is among.
-template <int THREADS>
-__device__ __forceinline__ Unit unit_of_step(const AttendParams& p, int64_t step)
-{
-  Unit u  = row_of_step<THREADS>(p, step);
-  u.span  = span_of(p, u.row);
-  u.steps = steps_for(u.span.count);
-  u.unit  = static_cast<int>(divide(step - u.begin, u.steps));
-  u.begin += u.unit * u.steps;
-  return u;
+  if (share < x.split.shares) {
+    x.unit.row   = found[0];
+    x.unit.span  = spans;
+    x.unit.steps = steps_for(spans.count);
+    const auto u = divide(x.at - found[1], x.unit.steps);
+    x.unit.unit  = static_cast<int>(u);
+    x.unit.begin = found[1] + u * x.unit.steps;
+  }
+  return x;
 }
 
 /// Calls body(segment) for this block's share of the work. A block of W warps calls it as a whole.
@@ -350,7 +368,8 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
   // What a block works on lies in shared memory: the registers are needed for the work. The first thread of the last warp, which
   // has the fewest tiles, works out the next segment while the others begin with one.
   struct State {
-    int64_t at, end, total;
+    int64_t at, end;
+    Split split;
     Unit u;
   };
   __shared__ Segment segments[2];
@@ -375,7 +394,7 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
           const int64_t id = u.row * p.units + unit;
           int64_t* mark    = p.marks + 2 * (p.by_unit ? id : blockIdx.x);
           mark[0]          = p.by_unit ? share : id;
-          mark[1]          = ends ? 0 : Split(state.total, p.shares).share_of(u.begin + u.steps - 1) - share + 1;
+          mark[1]          = ends ? 0 : state.split.share_of(u.begin + u.steps - 1) - share + 1;
         }
       }
       if (to < end) {
@@ -421,13 +440,11 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
         }
       }
     }
-    const Split split(all_steps<kThreads>(p), p.shares);
+    const Start x = start_of<W>(p, share);
     if (p.marks && !p.by_unit && threadIdx.x == kScribe) { p.marks[2 * int64_t(blockIdx.x) + 1] = 0; }
-    if (share >= split.shares) { return; }
-    const int64_t at = split.first_step(share);
-    const Unit u     = unit_of_step<kThreads>(p, at);
+    if (share >= x.split.shares) { return; }
     if (threadIdx.x == kScribe) {
-      state = {at, split.first_step(share + 1), split.total, u};
+      state.at = x.at, state.end = x.split.first_step(share + 1), state.split = x.split, state.u = x.unit;
       next(segments[0]);
     }
   }
