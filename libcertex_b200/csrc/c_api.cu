@@ -757,7 +757,7 @@ cuvsError_t certexB200PagedAttendSelected(cuvsResources_t res, const certexB200P
   return translate([=] {
     CERTEX_EXPECTS(cache != nullptr && (n_lists == 1 || n_lists == n_heads || n_lists == cache->n_kv_heads),
                    "certex: one list of positions per query head, per KV head or for all heads");
-    CERTEX_EXPECTS(k >= 0 && k < (int64_t(1) << 31) && (selected != nullptr || k == 0 || n_rows == 0), "certex: null positions");
+    CERTEX_EXPECTS(k >= 0 && k <= kMostTokens && (selected != nullptr || k == 0 || n_rows == 0), "certex: null positions, or too many of them");
     AttendArgs a{};
     a.selected    = selected;
     a.selected_64 = selected_64 != 0;

@@ -16,6 +16,7 @@ enum PagedType : int { kPagedF32 = 0, kPagedF16 = 1, kPagedBF16 = 2 };
 inline int paged_type_size(int t) { return t == kPagedF32 ? 4 : 2; }
 
 constexpr int kPagedMaxDim = 256;
+constexpr int64_t kMostTokens = (int64_t(1) << 31) - 64;  // that a row may see: tokens are counted in 32 bits
 
 /// y = x turned by `positions` (or back, `inverse`): rows x heads x dim, the first rotary_dim coordinates.
 void launch_rotate(const certexB200Rotary_t& plan, const certexB200Rows_t& x, const certexB200Rows_t& y, int64_t n_rows,

@@ -110,7 +110,7 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.pages           = a.table.pages;
   p.page_row        = a.table.row_stride;
   p.n_sequences     = a.table.n_sequences;
-  p.most            = a.table.pages_per_sequence * a.cache.page_size;
+  p.most            = std::min(a.table.pages_per_sequence * a.cache.page_size, kMostTokens);
   p.row_to_sequence = a.table.row_to_sequence;
   p.lengths         = a.lengths;
   p.window          = a.window;

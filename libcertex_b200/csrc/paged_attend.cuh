@@ -1432,40 +1432,46 @@ struct Joint {
   int n;               // its shares; 0: there is nothing to join
 };
 
+/// Every thread of a joining kernel calls this: when it returns, the first kernel has ended and its results are there. (A kernel
+/// that is launched ahead of another's end must not end before it.)
 __device__ __forceinline__ Joint joint_of(const AttendParams& p, int64_t x)
 {
   Joint j{0, 0, 0, 0, 0};
-  int64_t id;
+  int64_t id = 0;
   if (p.marks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    j.n = static_cast<int>(p.marks[2 * x + 1]);
-    if (j.n == 0) { return j; }
+    if (x >= p.joints) { return j; }
+    j.n                = static_cast<int>(p.marks[2 * x + 1]);
     const int64_t mark = p.marks[2 * x];
-    id      = p.by_unit ? x : mark;
-    j.first = p.by_unit ? mark : divide(x, p.abreast);
+    id                 = p.by_unit ? x : mark;
+    j.first            = p.by_unit ? mark : divide(x, p.abreast);
   } else {
     // one length, so every unit has the same steps
-    const int64_t steps = steps_for(span_of(p, 0).count);
-    if (steps == 0) { return j; }
-    const Split split(steps * p.n_rows * p.in_line, p.shares);
-    int64_t at;  // the unit's number among those that lie behind one another
-    if (p.by_unit) {
-      id = x;
-      at = p.abreast == 1 ? id : divide(id, p.units);
-    } else {
+    const int64_t steps = x < p.joints ? steps_for(span_of(p, 0).count) : 0;
+    if (steps > 0) {
+      const Split split(steps * p.n_rows * p.in_line, p.shares);
       const int64_t share = divide(x, p.abreast);
-      if (share >= split.shares) { return j; }
-      at = divide(split.first_step(share + 1) - 1, steps);
-      id = p.abreast == 1 ? at : at * p.units + (x - share * p.abreast);
+      int64_t at          = -1;  // the unit's number among those that lie behind one another
+      if (p.by_unit) {
+        id = x;
+        at = p.abreast == 1 ? id : divide(id, p.units);
+      } else if (share < split.shares) {
+        at = divide(split.first_step(share + 1) - 1, steps);
+        id = p.abreast == 1 ? at : at * p.units + (x - share * p.abreast);
+      }
+      if (at >= 0) {
+        j.first         = split.share_of(at * steps + kLead);
+        const int64_t n = split.share_of((at + 1) * steps - 1) - j.first + 1;
+        if (n > 1 && (p.by_unit || j.first == share)) { j.n = static_cast<int>(n); }
+      }
     }
-    j.first         = split.share_of(at * steps + kLead);
-    const int64_t n = split.share_of((at + 1) * steps - 1) - j.first + 1;
-    if (n == 1 || (!p.by_unit && j.first != divide(x, p.abreast))) { return j; }
-    j.n = static_cast<int>(n);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
   }
-  j.row    = divide(id, p.units);
-  j.unit   = static_cast<int>(id - j.row * p.units);
-  j.beside = p.abreast == 1 ? 0 : j.unit;
+  if (j.n > 0) {
+    j.row    = divide(id, p.units);
+    j.unit   = static_cast<int>(id - j.row * p.units);
+    j.beside = p.abreast == 1 ? 0 : j.unit;
+  }
   return j;
 }
 
@@ -1474,7 +1480,7 @@ __device__ __forceinline__ const float* part_of(const AttendParams& p, const Joi
   return p.parts + (2 * ((j.first + x) * p.abreast + j.beside) + (x == 0 ? 1 : 0)) * p.part_floats;
 }
 
-/// Many units with few shares each: a warp joins one query of one of them.
+/// Many units with few shares each: a warp joins one query of one of them, four shares at a time with a running maximum.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_many_kernel(const AttendParams p)
 {
@@ -1482,31 +1488,44 @@ __global__ void __launch_bounds__(kJoinThreads) join_many_kernel(const AttendPar
   const int lane     = threadIdx.x % 32;
   const int64_t x    = divide(item, p.per_unit);
   const int i        = static_cast<int>(item - x * p.per_unit);
-  Joint j{0, 0, 0, 0, 0};
-  if (x < p.joints) { j = joint_of(p, x); }
+  const Joint j      = joint_of(p, x);
   if (j.n == 0) { return; }
   const Segment g = segment_of(p, j.row, Span{0, 0, 0}, j.unit);
   if (i >= g.n_heads) { return; }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  float top = -INFINITY;
-  for (int y = lane; y < j.n; y += 32) { top = fmaxf(top, part_of(p, j, y)[4 * i]); }
-  for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(~0u, top, o)); }
-  float sum = 0.f, seen = 0.f;
+  constexpr int kAhead = 4;
+  float top = -INFINITY, sum = 0.f, seen = 0.f;
   float4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll 4
-  for (int y = 0; y < j.n; ++y) {
-    const float* from = part_of(p, j, y);
-    const float4 s    = *reinterpret_cast<const float4*>(from + 4 * i);
-    const float f     = top == -INFINITY ? 1.f : exp2_fast(s.x - top);
-    sum += f * s.y;
-    seen += s.z;
+  for (int y0 = 0; y0 < j.n; y0 += kAhead) {
+    float4 s[kAhead], o[kAhead][2];
+    float next = top;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = lane * 4 + h * 128;
-      if (c < p.dim) {
-        const float4 o = *reinterpret_cast<const float4*>(from + 4 * p.per_unit + i * p.dim + c);
-        v[h].x += f * o.x, v[h].y += f * o.y, v[h].z += f * o.z, v[h].w += f * o.w;
+    for (int y = 0; y < kAhead; ++y) {
+      s[y] = float4{-INFINITY, 0.f, 0.f, 0.f};
+      o[y][0] = o[y][1] = float4{0.f, 0.f, 0.f, 0.f};
+      if (y0 + y < j.n) {
+        const float* from = part_of(p, j, y0 + y);
+        s[y]              = *reinterpret_cast<const float4*>(from + 4 * i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = lane * 4 + h * 128;
+          if (c < p.dim) { o[y][h] = *reinterpret_cast<const float4*>(from + 4 * p.per_unit + i * p.dim + c); }
+        }
       }
+    }
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) { next = fmaxf(next, s[y].x); }
+    const float base = next == -INFINITY ? 0.f : next, alpha = exp2_fast(top - base);
+    top              = next;
+    sum *= alpha;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) { v[h].x *= alpha, v[h].y *= alpha, v[h].z *= alpha, v[h].w *= alpha; }
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      const float f = exp2_fast(s[y].x - base);
+      sum += f * s[y].y;
+      seen += s[y].z;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) { v[h].x += f * o[y][h].x, v[h].y += f * o[y][h].y, v[h].z += f * o[y][h].z, v[h].w += f * o[y][h].w; }
     }
   }
   T* out = static_cast<T*>(p.out) + j.row * p.o_row + (g.head + i) * p.o_head;
@@ -1541,7 +1560,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendParams p
   auto part   = [&](int x) { return part_of(p, j, x); };
   const int lanes = p.join_lanes, groups = kJoinThreads / lanes, from_c = blockIdx.z * lanes * 4;
   const int c = from_c + threadIdx.x % lanes * 4, mine = threadIdx.x / lanes;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // this thread's first outputs set out before the sums are known
   constexpr int kAhead = 8;
