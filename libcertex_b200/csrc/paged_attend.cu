@@ -47,7 +47,8 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   while (n.cluster < 8 && units * n.cluster * 8 <= warps && n.cluster * 64 < most) { n.cluster *= 2; }
   if (most > kClusterTokens * n.cluster) { n.cluster = 0; }
   const int few          = half ? 2 : 1;  // warps of a small block
-  n.warps                = n.cluster || warps / few > kManyShares * units ? 4 : few;
+  const bool small       = n.cluster ? units * n.cluster * 4 > warps : warps / few <= kManyShares * units;
+  n.warps                = small ? few : 4;
   const int64_t resident = warps / n.warps;
   // units side by side, where that leaves few blocks without work; lists of positions have no common tokens
   n.abreast = a.n_lists == 0 && n.units <= resident && resident % n.units * 16 <= resident ? n.units : 1;
