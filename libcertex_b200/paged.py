@@ -19,7 +19,6 @@ and `PagedCache.faulted` tells.
 
 import math
 import struct
-from fractions import Fraction
 
 import torch
 
@@ -32,8 +31,8 @@ _TABLE = struct.Struct("5q")
 _ROTARY = struct.Struct("3qd")
 _CACHE = struct.Struct("14q")
 _MOST_DIM = 256
-# 2 pi to 40 digits: a frequency's share of a turn is rounded once, to 2**-64
-_TURN = Fraction("6.283185307179586476925286766559005768394")
+# 2 pi in units of 10**-39: a frequency's share of a turn is rounded once, to 2**-64
+_TURN = 6283185307179586476925286766559005768394
 
 
 def _fail(message):
@@ -168,7 +167,7 @@ class Rotary:
             magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" and factor > 1 else 1.0
         self.frequencies, self.magnitude = w, float(magnitude)
         # what one position adds to an angle, as a fraction of a turn in units of 2**-64
-        turns = [round(Fraction(f) / _TURN * 2**64) % 2**64 for f in w]
+        turns = [_turns(f) for f in w]
         self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device=device)
         self.device = self._turns.device
         self._index = self._turns.get_device()
@@ -196,6 +195,12 @@ class Rotary:
             L.check(L.lib().certexB200Rotate(L.resources(self._index), self._plan, _packed(x), _packed(y), n, heads, dim, _KIND[x.dtype],
                                              positions.data_ptr(), positions.dtype is torch.int64, bool(inverse)))
         return y
+
+
+def _turns(w):
+    """w radians as a fraction of a turn in units of 2**-64, whole turns left out."""
+    n, d = w.as_integer_ratio()
+    return ((n * 10**39 << 65) // (d * _TURN) + 1) // 2 % 2**64
 
 
 def _frequencies(r, base, scaling, factor, length, low, high):
