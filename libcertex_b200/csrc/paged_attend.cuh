@@ -11,15 +11,22 @@
 //
 //  * One pass. Scores, the running maximum m, the running sum l and the output stay in registers in float32;
 //    when m grows, l and the output are multiplied by exp2(m_old - m_new). Scores are kept in units of log2 e, so that a
-//    weight is one multiply-add and one exp2.
+//    weight is one subtraction and one exp2.
 //  * The stream is split evenly. The tokens that all rows of the call see, in steps of kStep, are one sequence of work that
-//    is cut into equal shares, a share per resident block ("worker"), wherever the cuts fall: 1 row of 131 072 keys and 64
-//    rows of 1 to 8192 keys load the GPU alike, and lengths are read on the device only. A row and KV head ("unit") that
+//    is cut into equal shares, a share per resident block, wherever the cuts fall: 1 row of 131 072 keys and 64 rows of 1 to
+//    8192 keys load the GPU alike, and lengths are read on the device only. A row and KV head ("unit") that
 //    a cut divides leaves a partial result (m, l, output) per share, which a second, small kernel joins in the order of the
 //    shares: results do not depend on timing. It is launched while the first still runs and waits for it.
 //    Calls whose units are known to be short take a block, or a cluster of blocks, per unit and one launch.
-//  * A warp works by itself on tiles of 16 keys, by turns with the W warps of its block: no barrier until a unit ends, and the
-//    loads of the next tile are in flight while one is computed. The table's entries for a tile are fetched one tile before its loads.
+//  * A warp works by itself on tiles of 16 or 32 keys, by turns with the W warps of its block: no barrier until a unit ends, and
+//    the loads of the next tile are in flight while one is computed. The table's entries for a tile are asked for a tile before
+//    its loads, and where it lies is worked out while the tile before it arrives: done between two tiles' products instead, a call
+//    over 131 072 keys took 105 us instead of 94, and float32 keys 240 instead of 192.
+//
+// 131 072 bfloat16 keys of 8 heads of 128: 92 us, 5.8 TB/s, of which about 11 us are the launches, the first tile's chain of
+// reads (length, page, row) and the joining; the rest runs at 6.4 TB/s, the rate of a copy. Rows of 256 bytes in a random order (selected
+// positions) come at 4.9 TB/s. Asking L2 for rows two tiles ahead made everything slower (a prefetch per row 108 and 160 us for
+// these two, one per line 98 and 208): the reads in flight are enough, and DRAM has its own order to keep.
 //
 // Rows that are not to be seen have scores of -infinity and values of zero, so nothing that lies there (NaN, infinity,
 // another sequence's tokens) has an effect.
@@ -296,6 +303,8 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
     return x;
   }
   // an inclusive sum over the block for kThreads rows at a time; the total first, where they are more
+  if (threadIdx.x == 0) { found[0] = -1; }
+  __syncthreads();
   int64_t total = 0;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const bool once = p.n_rows <= kThreads;
@@ -342,6 +351,7 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
     if (W > 1) { __syncthreads(); }
   }
   __syncthreads();
+  if (found[0] < 0) { x.split = Split(0, 0); }  // no share, or lengths that somebody changes meanwhile
   if (share < x.split.shares) {
     x.unit.row   = found[0];
     x.unit.span  = spans;
@@ -401,14 +411,14 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
         u.begin += u.steps;
         if (++u.unit == p.in_line) {
           u.unit = 0;
-          do {
-            u.span = span_of(p, ++u.row);
-          } while (u.span.count == 0);  // (there are steps left: a row behind has some)
+          do {  // (there are steps left: a row behind has some, unless somebody changes the lengths meanwhile)
+            u.span = ++u.row < p.n_rows ? span_of(p, u.row) : Span{0, 0, 0};
+          } while (u.span.count == 0 && u.row < p.n_rows);
           u.steps = steps_for(u.span.count);
         }
         state.u = u;
       }
-      state.at = to;
+      state.at = u.steps > 0 ? to : end;
       if (i0 < i1) { break; }
     }
   };
@@ -701,7 +711,7 @@ __device__ __forceinline__ float sum_over_keys(float v)
 // key's four lanes takes 16 bytes in a row for two steps of the product; and the second product's rows, the
 // coordinates of the result, may be any eight coordinates, so lane g of a value's eight lanes takes 16 bytes in a row for
 // four products. What is left is to pair the values of neighbouring keys, one byte permutation per register.
-// Against copies into shared memory and ldmatrix this takes 250 instructions per tile instead of 470.
+// Against copies into shared memory and ldmatrix this takes 380 instructions per tile of 8 KB instead of 470.
 
 /// N * 4 bytes that are read once.
 template <int N>

@@ -84,12 +84,21 @@ def _check_out(out, x, in_place):
     _need(isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype == x.dtype and out.device == x.device,
           f"out must be a {x.dtype} tensor of shape {tuple(x.shape)} on {x.device}")
     _need(not out.is_neg() and not (torch.is_grad_enabled() and out.requires_grad), "out must be a plain tensor without a gradient")
-    _need(out.numel() == 0 or (out.stride(2) == 1 and all(s >= x.shape[2] or n == 1 for n, s in zip(out.shape[:2], out.stride()))),
-          "out must have rows of its own for every head, with a dense last axis")
-    if out.numel() and not (in_place and out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
-        (a, b), (c, d) = _span(out), _span(x)
-        _need(b <= c or d <= a, "out must not share memory with the rows" + (" unless it is them" if in_place else ""))
+    if out.numel():
+        (n, heads, dim), (row, head, one) = out.shape, out.stride()
+        _need(one == 1 and (row >= (heads - 1) * head + dim or n == 1 or head >= (n - 1) * row + dim) and (head >= dim or heads == 1)
+              and (row >= dim or n == 1), "out must have memory of its own for every head, with a dense last axis")
+        if not (in_place and out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+            (a, b), (c, d) = _span(out), _span(x)
+            _need(b <= c or d <= a, "out must not share memory with the rows" + (" unless it is them" if in_place else ""))
     return out
+
+
+def _written(*tensors):
+    """Tells autograd that the library wrote into tensors of the caller's: a graph that saved one of them before finds out."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def _no_gradient(*tensors):
@@ -176,7 +185,9 @@ class Rotary:
     @_on_device
     def __call__(self, x, positions, inverse=False, out=None):
         """x (n, heads, head_dim) float32, float16 or bfloat16, its rows turned by positions (n,) int32 or int64, which may be
-        negative; inverse=True turns back. Differentiable in x. out: where to write, x itself allowed; without a gradient."""
+        negative; inverse=True turns back. Differentiable in x (as for every function of torch, a backward pass that is captured
+        in a CUDA graph wants leaves of which no eager graph is alive). out: where to write, x itself allowed; without a
+        gradient."""
         x = _check_rows(x, "x", dim=self.head_dim)
         if x.dtype not in _KIND:
             _fail(f"rows are float32, float16 or bfloat16, not {x.dtype}")
@@ -194,6 +205,8 @@ class Rotary:
         if n and heads:
             L.check(L.lib().certexB200Rotate(L.resources(self._index), self._plan, _packed(x), _packed(y), n, heads, dim, _KIND[x.dtype],
                                              positions.data_ptr(), positions.dtype is torch.int64, bool(inverse)))
+        if out is not None:
+            _written(y)
         return y
 
 
@@ -244,8 +257,8 @@ class PagedCache:
                 _need(v is not None and v >= 1, f"{what} must be positive")
             inner = (page_size, n_kv_heads) if layout == "NHD" else (n_kv_heads, page_size)
             keys, values = (torch.zeros((n_pages, *inner, head_dim), dtype=dtype, device=device) for _ in range(2))
-        _need(all(isinstance(t, torch.Tensor) and t.is_cuda and t.ndim == 4 and not t.is_neg() for t in (keys, values)),
-              "keys and values must be CUDA tensors of four axes")
+        _need(all(isinstance(t, torch.Tensor) and t.is_cuda and t.ndim == 4 and not t.is_neg() and not t.requires_grad
+                  for t in (keys, values)), "keys and values must be CUDA tensors of four axes, without a gradient")
         _need(keys.shape == values.shape and keys.dtype == values.dtype and keys.device == values.device,
               "keys and values must have the same shape, type and device")
         _need(keys.dtype in _KIND, f"a paged cache holds float32, float16 or bfloat16, not {keys.dtype}")
@@ -328,6 +341,7 @@ class PagedCache:
             L.check(L.lib().certexB200PagedAppend(L.resources(self._index), self._args, self.rotary._plan if self.rotary else None, table,
                                                   _packed(k), _packed(v), q_in, q_to, n, heads, positions.data_ptr(),
                                                   positions.dtype is torch.int64))
+            _written(self.keys, self.values)
         return turned
 
     def _prepared(self, q, scale, return_lse, out):
@@ -343,6 +357,12 @@ class PagedCache:
         if not math.isfinite(scale):
             _fail("the scale must be finite")
         return q, out, lse, scale
+
+    @staticmethod
+    def _answer(out, lse, given):
+        if given is not None:
+            _written(out)
+        return out if lse is None else (out, lse)
 
     def _workspace(self, n, heads, lists, k, window):
         """(tensor or None, its address, its bytes): memory for the partial results of one call, of the stream's allocator, so
@@ -367,6 +387,7 @@ class PagedCache:
         h // (heads / n_kv_heads). scale defaults to head_dim ** -0.5. Returns (n, heads, head_dim), and with return_lse the
         float32 logarithm of the sum of exponentials (n, heads). A row that sees nothing gets zeros and -inf. Several rows of
         one sequence (drafted tokens) name it in row_to_batch and have their own lengths."""
+        given = out
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
         if window is None:
@@ -379,13 +400,14 @@ class PagedCache:
             w, at, size = self._workspace(n, heads, 0, page_table.shape[1] * self.page_size, window)
             L.check(L.lib().certexB200PagedAttend(L.resources(self._index), self._args, table, lengths.data_ptr(), window, _packed(q),
                                                   _packed(out), n, heads, scale, None if lse is None else lse.data_ptr(), at, size))
-        return (out, lse) if return_lse else out
+        return self._answer(out, lse, given)
 
     @_on_device
     def attend_selected(self, q, selected, scale=None, return_lse=False, out=None):
         """attend() over positions that were selected before: selected (n, heads, k), (n, n_kv_heads, k) or (n, 1, k), int32 or
         int64, are places of the cache, page * page_size + place, as `flashinfer.ExactTopK.page_table_transform` returns them;
         negative ones are left out, one that is named twice counts twice."""
+        given = out
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
         if (not isinstance(selected, torch.Tensor) or selected.ndim != 3 or selected.shape[0] != n
@@ -398,4 +420,4 @@ class PagedCache:
             L.check(L.lib().certexB200PagedAttendSelected(L.resources(self._index), self._args, selected.data_ptr(),
                                                           selected.dtype is torch.int64, lists, k, _packed(q), _packed(out), n,
                                                           heads, scale, None if lse is None else lse.data_ptr(), at, size))
-        return (out, lse) if return_lse else out
+        return self._answer(out, lse, given)

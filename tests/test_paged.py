@@ -476,3 +476,38 @@ def test_two_graphs_two_streams_and_eager_calls_at_once():
     lengths.copy_(torch.tensor([5, 20_000, 13, 1], dtype=torch.int32))  # a captured call sees the new lengths
     graphs[0].replay()
     assert torch.equal(outs[0][0], cache.attend(q[0], table, lengths))
+
+
+@gpu
+def test_what_the_library_overwrites_is_known_to_autograd():
+    """A tensor that a graph saved and a call overwrote makes the backward pass fail instead of using what lies there now."""
+    rotary = certex.Rotary(64)
+    cache = certex.PagedCache(4, 16, 1, 64, dtype=torch.float32)
+    p, table = torch.arange(5, device="cuda"), torch.arange(4, device="cuda", dtype=torch.int32)[None]
+    n, to = torch.full((5,), 5, device="cuda", dtype=torch.int32), torch.zeros(5, device="cuda", dtype=torch.int32)
+    x = torch.randn((5, 1, 64), device="cuda")
+    a = torch.ones((5, 1, 64), device="cuda", requires_grad=True)
+    overwrite = ((x, lambda: rotary(x, p, out=x)), (cache.keys, lambda: cache.append(x, x, table, p, row_to_batch=to)),
+                 (cache.values, lambda: cache.append(x, x, table, p, row_to_batch=to)), (x, lambda: cache.attend(x.clone(), table, n, row_to_batch=to, out=x)),
+                 (x, lambda: cache.attend_selected(x.clone(), p.int().view(5, 1, 1), out=x)))
+    for t, call in overwrite:
+        loss = (a * t.view(-1)[: a.numel()].view_as(a)).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        y = torch.randn((5, 1, 64), device="cuda")
+        rotary(y, p, out=y)
+        cache.append(y, y, table, p, row_to_batch=to)
+
+
+@gpu
+def test_outputs_whose_rows_overlap_are_refused():
+    rotary, p = certex.Rotary(8), torch.arange(4, device="cuda")
+    x, memory = torch.randn((4, 3, 8), device="cuda"), torch.zeros(400, device="cuda")
+    for strides in ((8, 8, 1), (16, 8, 1), (24, 4, 1), (0, 8, 1), (8, 16, 1), (24, 8, 2)):
+        with pytest.raises(ValueError, match="memory of its own"):
+            rotary(x, p, out=memory.as_strided((4, 3, 8), strides))
+    for strides in ((24, 8, 1), (30, 9, 1), (8, 32, 1), (9, 40, 1)):
+        out = memory.as_strided((4, 3, 8), strides)
+        assert torch.equal(rotary(x, p, out=out), rotary(x, p))

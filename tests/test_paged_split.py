@@ -109,6 +109,12 @@ def test_calls_of_all_kinds_in_a_row(dtype):
     for _ in range(3):
         for a, b in zip([call() for call in calls], alone):
             assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [call() for call in calls]
+    graph.replay()
+    for a, b in zip(captured, alone):
+        assert torch.equal(a, b)
 
 
 def test_the_tables_width_changes_nothing_that_is_seen():

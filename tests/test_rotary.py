@@ -182,3 +182,27 @@ def test_on_another_stream_and_in_a_graph():
     p.add_(100)
     graph.replay()
     assert torch.equal(y, plan(x, p)) and not torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_a_captured_training_step():
+    """Forward and gradient in one graph, replayed on other inputs."""
+    plan = certex.Rotary(32, interleaved=True)
+    x = torch.randn((50, 4, 32), device="cuda").requires_grad_()
+    dy, p = torch.randn((50, 4, 32), device="cuda"), torch.randint(0, 9999, (50,), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            torch.autograd.grad(plan(x, p), x, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = plan(x, p)
+        (dx,) = torch.autograd.grad(y, x, dy)
+    with torch.no_grad():
+        x.mul_(2)
+        p.add_(7)
+    graph.replay()
+    close(y.detach(), x, p, plan)
+    close(dx, dy, p, plan, inverse=True)
