@@ -122,6 +122,8 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.q               = a.q.data;
   p.q_row           = a.q.row_stride;
   p.q_head          = a.q.head_stride;
+  const int in_16   = 16 / paged_type_size(static_cast<int>(a.cache.dtype));
+  p.q_wide          = reinterpret_cast<uintptr_t>(a.q.data) % 16 == 0 && a.q.row_stride % in_16 == 0 && a.q.head_stride % in_16 == 0;
   p.out             = a.out.data;
   p.o_row           = a.out.row_stride;
   p.o_head          = a.out.head_stride;
@@ -141,7 +143,8 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.by_unit         = n.by_unit;
   p.joints          = n.by_unit ? a.n_rows * n.units : n.shares * n.abreast;
   const int64_t all = p.joints * n.per_unit;  // queries to be joined
-  p.join_lanes      = all > 4 * sm_count ? 0 : all <= sm_count ? 8 : p.dim <= 128 ? 32 : 64;
+  const bool few    = n.blocks <= 8 * a.n_rows * n.units;  // shares each, on average
+  p.join_lanes      = few || all > 4 * sm_count ? 0 : all <= sm_count ? 8 : p.dim <= 128 ? 32 : 64;
   p.part_floats     = n.part_floats;
   p.parts           = static_cast<float*>(a.workspace);
   const bool one    = a.n_lists > 0 || a.n_rows == 1;

@@ -67,6 +67,7 @@ struct AttendParams {
   // queries and answers
   const void* q;
   int64_t q_row, q_head;
+  int32_t q_wide;  // every query lies on 16 bytes
   void* out;
   int64_t o_row, o_head;
   float* lse;
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
     };
     int64_t entry0 = ask(0), entry = ask(1);
 
-    // the queries, as the 8-column side of the first product
+    // the queries, as the 8-column side of the first product; a lane takes the same coordinates of a query as of a key
     uint32_t qf[NT][kSteps][2];
     {
       const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
@@ -772,17 +773,30 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
       for (int x = 0; x < NT; ++x) {
         const int i  = x * 8 + g8;
         const T* row = q + i * p.q_head;
+        if (p.q_wide && i < g.n_heads) {
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
+          for (int k = 0; k < kK32; ++k) {
+            uint4 v{0, 0, 0, 0};
+            if (!PAD || k * 32 + t4 * 8 < p.dim) { v = *reinterpret_cast<const uint4*>(row + k * 32 + t4 * 8); }
+            qf[x][2 * k][0] = v.x, qf[x][2 * k][1] = v.y, qf[x][2 * k + 1][0] = v.z, qf[x][2 * k + 1][1] = v.w;
+          }
+          if constexpr (kK16 > 0) {
+            const uint2 v = *reinterpret_cast<const uint2*>(row + kK32 * 32 + t4 * 4);
+            qf[x][2 * kK32][0] = v.x, qf[x][2 * kK32][1] = v.y;
+          }
+        } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c = k < 2 * kK32 ? k / 2 * 32 + t4 * 8 + k % 2 * 4 + h * 2 : kK32 * 32 + t4 * 4 + h * 2;
-            uint32_t v  = 0;
-            if (i < g.n_heads && (!PAD || c < p.dim)) {
-              const auto a = *reinterpret_cast<const uint16_t*>(row + c), b = *reinterpret_cast<const uint16_t*>(row + c + 1);
-              v            = a | (uint32_t(b) << 16);
+          for (int k = 0; k < kSteps; ++k) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = k < 2 * kK32 ? k / 2 * 32 + t4 * 8 + k % 2 * 4 + h * 2 : kK32 * 32 + t4 * 4 + h * 2;
+              uint32_t v  = 0;
+              if (i < g.n_heads && (!PAD || c < p.dim)) {
+                const auto a = *reinterpret_cast<const uint16_t*>(row + c), b = *reinterpret_cast<const uint16_t*>(row + c + 1);
+                v            = a | (uint32_t(b) << 16);
+              }
+              qf[x][k][h] = v;
             }
-            qf[x][k][h] = v;
           }
         }
       }
