@@ -390,11 +390,16 @@ Resources::Resources()
   int major = 0;
   CERTEX_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
   CERTEX_EXPECTS(major == 10, "certex: this library is built for sm_100a (B200) only");
-  // keep freed scratch memory in the stream-ordered pool instead of returning it to the driver at every sync
+  // Keep freed scratch memory in the stream-ordered pool instead of returning it to the driver at every sync. A thread's first call
+  // may come while a stream is being captured, which forbids this kind of call unless the thread says that it concerns no stream.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  CERTEX_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
   cudaMemPool_t pool;
-  CERTEX_CUDA(cudaDeviceGetDefaultMemPool(&pool, device));
   uint64_t keep = UINT64_MAX;
-  CERTEX_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
+  cudaError_t e = cudaDeviceGetDefaultMemPool(&pool, device);
+  if (e == cudaSuccess) { e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep); }
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  CERTEX_CUDA(e);
 }
 
 Resources::~Resources()
