@@ -60,6 +60,8 @@ def _check_index(t, what, shape, device, wide=False):
         _fail(f"{what} must be {'int32 or int64' if wide else 'int32'}, not {t.dtype}")
     if t.shape != shape:
         _fail(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    if t.is_neg():
+        t = t.resolve_neg()
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -94,11 +96,8 @@ def _check_out(out, x, in_place):
     return out
 
 
-def _written(*tensors):
-    """Tells autograd that the library wrote into tensors of the caller's: a graph that saved one of them before finds out."""
-    for t in tensors:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+# Tells autograd that the library wrote into tensors of the caller's: a graph that saved one of them before finds out.
+_written = torch.autograd.graph.increment_version
 
 
 def _no_gradient(*tensors):
@@ -263,7 +262,7 @@ class PagedCache:
               "keys and values must have the same shape, type and device")
         _need(keys.dtype in _KIND, f"a paged cache holds float32, float16 or bfloat16, not {keys.dtype}")
         token, head = (1, 2) if layout == "NHD" else (2, 1)
-        self.keys, self.values, self.layout, self.rotary = keys, values, layout, rotary
+        self._keys, self._values, self._layout = keys, values, layout
         self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = (
             keys.shape[0], keys.shape[token], keys.shape[head], keys.shape[3])
         for given, have, what in ((n_pages, self.n_pages, "n_pages"), (page_size, self.page_size, "page_size"),
@@ -272,18 +271,33 @@ class PagedCache:
         self.dtype, self.device = keys.dtype, keys.device
         _need(self.head_dim % 8 == 0 and self.head_dim <= _MOST_DIM,
               f"head_dim must be a multiple of 8 and at most {_MOST_DIM}, not {self.head_dim}")
-        _need(rotary is None or (rotary.head_dim == self.head_dim and rotary._turns.device == self.device),
-              "the rotation must be for heads of this size, on this device")
+        self.rotary = rotary
         size = keys.element_size()
         for t in (keys, values):
             _need(t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s * size % 16 == 0 for s in t.stride()[:3]),
                   "keys and values need a dense last axis and strides of whole 16 bytes")
-        self._index = keys.get_device()
+        self._index, self._at = keys.get_device(), (keys.data_ptr(), values.data_ptr())
+        self._pages = (keys, values)
         self._needs = {}  # sizes of a call -> bytes of its workspace
         self._fault = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._args = _CACHE.pack(keys.data_ptr(), values.data_ptr(),
+        self._args = _CACHE.pack(*self._at,
                                  *(t.stride(i) for t in (keys, values) for i in (0, token, head)), self.n_pages,
                                  self.page_size, self.n_kv_heads, self.head_dim, _KIND[self.dtype], self._fault.data_ptr())
+
+    keys = property(lambda self: self._keys, doc="The pages of keys.")
+    values = property(lambda self: self._values, doc="The pages of values.")
+    layout = property(lambda self: self._layout, doc='"NHD" or "HND".')
+
+    @property
+    def rotary(self):
+        """What append() turns keys and queries with, or None."""
+        return self._rotary
+
+    @rotary.setter
+    def rotary(self, rotary):
+        _need(rotary is None or (rotary.head_dim == self.head_dim and rotary.device == self.device),
+              "the rotation must be for heads of this size, on this device")
+        self._rotary = rotary
 
     def faulted(self):
         """Whether an index of a call since the last time was out of range (and was left out). Waits for the device."""
@@ -297,6 +311,12 @@ class PagedCache:
         if x.dtype is not self.dtype or x.device != self.device:
             _fail(f"{what} must be {self.dtype} on {self.device} like the cache, not {x.dtype} on {x.device}")
         return x
+
+    def _unmoved(self):
+        """The cache as the library takes it, whose memory must still be where it was."""
+        if self._keys.data_ptr() != self._at[0] or self._values.data_ptr() != self._at[1]:
+            _fail("the pages were given other memory since this cache was made of them: make a new one")
+        return self._args
 
     def _table(self, page_table, row_to_batch, n):
         if (not isinstance(page_table, torch.Tensor) or page_table.device != self.device or page_table.dtype is not torch.int32
@@ -318,8 +338,9 @@ class PagedCache:
     def append(self, k, v, page_table, positions, row_to_batch=None, q=None):
         """Stores k, v (n, n_kv_heads, head_dim) at positions (n,) int32 or int64 of their sequences; a negative position is
         padding. With a rotation the keys are turned by their positions first, and q (n, heads, head_dim), if given, is
-        returned turned (rows of padding too, by the position as it stands). No two rows have the same place. The keys as
-        they are stored are what a selector wants: `rotary(k, positions)` gives them."""
+        returned turned (rows of padding too, by the position as it stands). No two rows have the same place, and k and v do not
+        lie in places that the call writes. The keys as they are stored are what a selector wants: `rotary(k, positions)` gives
+        them."""
         _no_gradient(k, v, q)
         k, v = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
         n = k.shape[0]
@@ -327,9 +348,9 @@ class PagedCache:
             _fail(f"{n} keys and {v.shape[0]} values")
         positions = _check_index(positions, "positions", (n,), self.device, wide=True)
         table, alive = self._table(page_table, row_to_batch, n)
-        heads, q_in, q_to, turned = 0, None, None, None
+        heads, q_in, q_to, turned, rotary = 0, None, None, None, self._rotary
         if q is not None:
-            _need(self.rotary is not None, "queries come along to be turned, but this cache has no rotation")
+            _need(rotary is not None, "queries come along to be turned, but this cache has no rotation")
             q = self._rows(q, "q")
             if q.shape[0] != n:
                 _fail(f"{n} keys and {q.shape[0]} queries")
@@ -338,10 +359,10 @@ class PagedCache:
             if heads:
                 q_in, q_to = _packed(q), _packed(turned)
         if n:
-            L.check(L.lib().certexB200PagedAppend(L.resources(self._index), self._args, self.rotary._plan if self.rotary else None, table,
+            L.check(L.lib().certexB200PagedAppend(L.resources(self._index), self._unmoved(), rotary._plan if rotary else None, table,
                                                   _packed(k), _packed(v), q_in, q_to, n, heads, positions.data_ptr(),
                                                   positions.dtype is torch.int64))
-            _written(self.keys, self.values)
+            _written(self._pages)
         return turned
 
     def _prepared(self, q, scale, return_lse, out):
@@ -398,26 +419,28 @@ class PagedCache:
         table, alive = self._table(page_table, row_to_batch, n)
         if n:
             w, at, size = self._workspace(n, heads, 0, page_table.shape[1] * self.page_size, window)
-            L.check(L.lib().certexB200PagedAttend(L.resources(self._index), self._args, table, lengths.data_ptr(), window, _packed(q),
+            L.check(L.lib().certexB200PagedAttend(L.resources(self._index), self._unmoved(), table, lengths.data_ptr(), window, _packed(q),
                                                   _packed(out), n, heads, scale, None if lse is None else lse.data_ptr(), at, size))
         return self._answer(out, lse, given)
 
     @_on_device
     def attend_selected(self, q, selected, scale=None, return_lse=False, out=None):
-        """attend() over positions that were selected before: selected (n, heads, k), (n, n_kv_heads, k) or (n, 1, k), int32 or
-        int64, are places of the cache, page * page_size + place, as `flashinfer.ExactTopK.page_table_transform` returns them;
+        """attend() over positions that were selected before: selected (n, heads, k), (n, n_kv_heads, k), (n, 1, k) or (n, k), int32
+        or int64, are places of the cache, page * page_size + place, as `flashinfer.ExactTopK.page_table_transform` returns them;
         negative ones are left out, one that is named twice counts twice."""
         given = out
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
+        if isinstance(selected, torch.Tensor) and selected.ndim == 2:
+            selected = selected[:, None]
         if (not isinstance(selected, torch.Tensor) or selected.ndim != 3 or selected.shape[0] != n
                 or selected.shape[1] not in (heads, self.n_kv_heads, 1)):
-            _fail(f"selected must have shape ({n}, {heads}, k), ({n}, {self.n_kv_heads}, k) or ({n}, 1, k)")
+            _fail(f"selected must have shape ({n}, {heads}, k), ({n}, {self.n_kv_heads}, k), ({n}, 1, k) or ({n}, k)")
         selected = _check_index(selected, "selected", selected.shape, self.device, wide=True)
         lists, k = selected.shape[1:]
         if n:
             w, at, size = self._workspace(n, heads, lists, k, 0)
-            L.check(L.lib().certexB200PagedAttendSelected(L.resources(self._index), self._args, selected.data_ptr(),
+            L.check(L.lib().certexB200PagedAttendSelected(L.resources(self._index), self._unmoved(), selected.data_ptr(),
                                                           selected.dtype is torch.int64, lists, k, _packed(q), _packed(out), n,
                                                           heads, scale, None if lse is None else lse.data_ptr(), at, size))
         return self._answer(out, lse, given)

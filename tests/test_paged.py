@@ -511,3 +511,52 @@ def test_outputs_whose_rows_overlap_are_refused():
     for strides in ((24, 8, 1), (30, 9, 1), (8, 32, 1), (9, 40, 1)):
         out = memory.as_strided((4, 3, 8), strides)
         assert torch.equal(rotary(x, p, out=out), rotary(x, p))
+
+
+@gpu
+def test_a_cache_stays_what_it_was_made_of():
+    cache = certex.PagedCache(4, 16, 1, 64, dtype=torch.float16)
+    for name, value in (("keys", cache.values), ("values", cache.keys), ("layout", "HND")):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, value)
+    for rotary in (certex.Rotary(32), certex.Rotary(64, device="cpu")):
+        with pytest.raises(ValueError, match="rotation"):
+            cache.rotary = rotary
+    cache.rotary = certex.Rotary(64)
+    k, p, t = torch.ones((1, 1, 64), device="cuda").half(), torch.zeros(1, device="cuda", dtype=torch.int32), torch.zeros((1, 1), device="cuda", dtype=torch.int32)
+    cache.append(k, k, t, p)
+    selected = p.view(1, 1)
+    assert torch.equal(cache.attend_selected(k, selected), cache.attend(k, t, p + 1))
+    keys = cache.keys
+    keys.data = torch.zeros_like(keys)
+    for call in (lambda: cache.append(k, k, t, p), lambda: cache.attend(k, t, p + 1), lambda: cache.attend_selected(k, selected)):
+        with pytest.raises(ValueError, match="other memory"):
+            call()
+
+
+@gpu
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Kernels that were never launched before, recorded in a graph."""
+    import subprocess
+    import sys
+
+    code = """
+import torch, libcertex_b200 as certex
+rotary = certex.Rotary(64)
+cache = certex.PagedCache(600, 16, 2, 64, dtype=torch.float16, rotary=rotary)
+k = torch.randn((1, 2, 64), device="cuda").half(); q = torch.randn((1, 8, 64), device="cuda").half()
+table = torch.arange(600, device="cuda", dtype=torch.int32)[None]
+p, n = torch.tensor([9000], device="cuda", dtype=torch.int32), torch.tensor([9001], device="cuda", dtype=torch.int32)
+cache.keys.normal_(); cache.values.normal_()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    r = cache.append(k, k, table, p, q=q)
+    a = cache.attend(r, table, n)
+    b = cache.attend(r, table[:, :5], torch.clamp(n, max=70))
+    c = cache.attend_selected(r, p.view(1, 1, 1))
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(a, cache.attend(r, table, n)) and torch.equal(c, k.repeat_interleave(4, 1)) and not cache.faulted()
+print("captured")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert "captured" in done.stdout, done.stderr[-2000:]
