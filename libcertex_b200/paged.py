@@ -112,19 +112,6 @@ except AttributeError:
     _current_device = torch.cuda.current_device
 
 
-def _on_device(method):
-    """Runs a call with the device of its first tensor current: kernels, streams and handles are the current device's."""
-
-    def call(self, x, *args, **kwargs):
-        if isinstance(x, torch.Tensor) and x.is_cuda and x.get_device() != _current_device():
-            with torch.cuda.device(x.device):
-                return method(self, x, *args, **kwargs)
-        return method(self, x, *args, **kwargs)
-
-    call.__doc__, call.__name__ = method.__doc__, method.__name__
-    return call
-
-
 # ------------------------------------------------------------------------------------------------------------ rotation
 class _Turn(torch.autograd.Function):
     """The rotation is linear and its transpose turns back, with the same magnitude."""
@@ -181,7 +168,6 @@ class Rotary:
         self._index = self._turns.get_device()
         self._plan = _ROTARY.pack(self._turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.magnitude)
 
-    @_on_device
     def __call__(self, x, positions, inverse=False, out=None):
         """x (n, heads, head_dim) float32, float16 or bfloat16, its rows turned by positions (n,) int32 or int64, which may be
         negative; inverse=True turns back. Differentiable in x (as for every function of torch, a backward pass that is captured
@@ -199,6 +185,9 @@ class Rotary:
         return self._turn(x, positions, inverse, out)
 
     def _turn(self, x, positions, inverse, out):
+        if _current_device() != self._index:  # kernels, streams and handles are the current device's
+            with torch.cuda.device(self._index):
+                return self._turn(x, positions, inverse, out)
         y = _new_like(x) if out is None else _check_out(out, x, True)
         n, heads, dim = x.shape
         if n and heads:
@@ -334,7 +323,6 @@ class PagedCache:
         args = _TABLE.pack(page_table.data_ptr(), page_table.stride(0), sequences, pages, rows)
         return args, (page_table, row_to_batch)  # what must live until the launch
 
-    @_on_device
     def append(self, k, v, page_table, positions, row_to_batch=None, q=None):
         """Stores k, v (n, n_kv_heads, head_dim) at positions (n,) int32 or int64 of their sequences; a negative position is
         padding. With a rotation the keys are turned by their positions first, and q (n, heads, head_dim), if given, is
@@ -342,6 +330,9 @@ class PagedCache:
         lie in places that the call writes. The keys as they are stored are what a selector wants: `rotary(k, positions)` gives
         them."""
         _no_gradient(k, v, q)
+        if _current_device() != self._index:  # kernels, streams and handles are the current device's
+            with torch.cuda.device(self._index):
+                return self.append(k, v, page_table, positions, row_to_batch, q)
         k, v = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
         n = k.shape[0]
         if v.shape[0] != n:
@@ -401,13 +392,15 @@ class PagedCache:
         w = torch.empty(need, dtype=torch.uint8, device=self.device)
         return w, w.data_ptr(), need
 
-    @_on_device
     def attend(self, q, page_table, lengths, row_to_batch=None, scale=None, window=None, return_lse=False, out=None):
         """Softmax attention of every row of q (n, heads, head_dim) over the first lengths[i] tokens of its sequence (n,)
         int32, or over the last `window` of those; heads is a multiple of n_kv_heads, query head h reads KV head
         h // (heads / n_kv_heads). scale defaults to head_dim ** -0.5. Returns (n, heads, head_dim), and with return_lse the
         float32 logarithm of the sum of exponentials (n, heads). A row that sees nothing gets zeros and -inf. Several rows of
         one sequence (drafted tokens) name it in row_to_batch and have their own lengths."""
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.attend(q, page_table, lengths, row_to_batch, scale, window, return_lse, out)
         given = out
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
@@ -423,11 +416,13 @@ class PagedCache:
                                                   _packed(out), n, heads, scale, None if lse is None else lse.data_ptr(), at, size))
         return self._answer(out, lse, given)
 
-    @_on_device
     def attend_selected(self, q, selected, scale=None, return_lse=False, out=None):
         """attend() over positions that were selected before: selected (n, heads, k), (n, n_kv_heads, k), (n, 1, k) or (n, k), int32
         or int64, are places of the cache, page * page_size + place, as `flashinfer.ExactTopK.page_table_transform` returns them;
         negative ones are left out, one that is named twice counts twice."""
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.attend_selected(q, selected, scale, return_lse, out)
         given = out
         q, out, lse, scale = self._prepared(q, scale, return_lse, out)
         n, heads, _ = q.shape
