@@ -352,7 +352,9 @@ typedef struct {
 } certexB200Rotary_t;
 
 /** key_strides / value_strides: from a page, a token of a page and a head to the next. keys, values and all strides are
- *  multiples of 16 bytes; head_dim is a multiple of 8 and at most 256. fault: one int32 of device memory. */
+ *  multiples of 16 bytes; head_dim is a multiple of 8 and at most 256; there are fewer than 2^31 - 1 places (n_pages *
+ *  page_size), no stride of pages or tokens is negative, and the last place lies within 2^32 of the largest power of two that divides these
+ *  strides. fault: one int32 of device memory. */
 typedef struct {
   void* keys;
   void* values;
@@ -399,7 +401,8 @@ CERTEX_B200_EXPORT cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, con
 
 /** out[i, h] = the values that row i sees, weighed by the softmax of scale * <q[i, h], key> over KV head h / (n_heads /
  *  n_kv_heads). Row i sees the first lengths[i] tokens of its sequence, of those the last `window` if window > 0; a row that
- *  sees none gets zeros. lse (may be NULL) [n_rows, n_heads]: the logarithm of the sum of exponentials (-inf for such a row). */
+ *  sees none gets zeros. lse (may be NULL) [n_rows, n_heads]: the logarithm of the sum of exponentials (-inf for such a row).
+ *  n_rows * n_heads is below 2^27; a row sees 2^31 - 64 tokens at most. */
 CERTEX_B200_EXPORT cuvsError_t certexB200PagedAttend(cuvsResources_t res, const certexB200PagedCache_t* cache,
                                                      const certexB200PageTable_t* table, const int32_t* lengths, int64_t window,
                                                      const certexB200Rows_t* q, const certexB200Rows_t* out, int64_t n_rows,

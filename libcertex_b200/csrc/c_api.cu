@@ -619,6 +619,7 @@ const certexB200PagedCache_t& checked_cache(const certexB200PagedCache_t* c)
   CERTEX_EXPECTS(c->n_pages >= 1 && c->page_size >= 1 && c->n_kv_heads >= 1 && c->n_pages < (int64_t(1) << 31) &&
                    c->page_size < (int64_t(1) << 31) && c->n_kv_heads <= 65535,
                  "certex: the cache needs pages, tokens in them and KV heads");
+  CERTEX_EXPECTS(c->n_pages * c->page_size < (int64_t(1) << 31) - 1, "certex: a cache has fewer than 2^31 - 1 places");
   CERTEX_EXPECTS(c->head_dim >= 8 && c->head_dim % 8 == 0 && c->head_dim <= kPagedMaxDim,
                  "certex: the head dimension of a paged cache is a multiple of 8 and at most " + std::to_string(kPagedMaxDim));
   const int64_t size = paged_type_size(static_cast<int>(c->dtype));
@@ -648,7 +649,7 @@ void attend_impl(cuvsResources_t res, AttendArgs a, const certexB200PagedCache_t
   a.cache = checked_cache(cache);
   CERTEX_EXPECTS(a.n_heads >= 1 && a.n_heads <= 65535 && a.n_heads % a.cache.n_kv_heads == 0,
                  "certex: the query heads must be a multiple of the KV heads");
-  CERTEX_EXPECTS(a.n_rows >= 0 && a.n_rows * a.n_heads < (int64_t(1) << 31), "certex: too many rows");
+  CERTEX_EXPECTS(a.n_rows >= 0 && a.n_rows * a.n_heads < (int64_t(1) << 27), "certex: too many rows");
   CERTEX_EXPECTS(std::isfinite(a.scale), "certex: the scale must be finite");
   if (a.n_rows == 0) { return; }
   check_rows(q, "queries");

@@ -44,6 +44,8 @@ struct AttendArgs {
   float* lse;              // [n_rows, n_heads] or null
   void* workspace;
 };
+/// n / d = (2 n * factor >> 32) >> shift for n < 2^31.
+void paged_divisor(uint32_t d, uint32_t& factor, int32_t& shift);
 /// Whether the kernels' 32-bit offsets, in units that the cache's strides are multiples of, reach all of the cache.
 bool paged_within_reach(const certexB200PagedCache_t& cache);
 size_t paged_attend_workspace(const AttendArgs& a, int sm_count);

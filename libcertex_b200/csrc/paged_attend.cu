@@ -23,7 +23,7 @@ struct Plan {
   int32_t per_unit, subs, units, warps;
   int cluster;
   int64_t blocks, shares;
-  int part_floats, by_unit, abreast;
+  int part_floats, by_unit, abreast, step_shift;
   size_t bytes;
 };
 
@@ -40,7 +40,7 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   n.units          = static_cast<int32_t>(a.cache.n_kv_heads) * n.subs;
   int64_t most     = a.n_lists > 0 ? a.k : a.table.pages_per_sequence * a.cache.page_size;
   if (a.n_lists == 0 && a.window > 0) { most = std::min(most, a.window); }
-  const int64_t units = a.n_rows * n.units, steps = (most + kStep - 1) / kStep;
+  const int64_t units = a.n_rows * n.units;
   const int64_t warps    = int64_t(sm_count) * (half ? (dim > 128 ? 4 : n.per_unit <= 8 ? 12 : 8) : 8);  // resident ones
   // as many blocks of four warps per unit as fill the GPU, with 64 tokens each at least
   n.cluster = 1;
@@ -52,10 +52,14 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   const int64_t resident = warps / n.warps;
   // units side by side, where that leaves few blocks without work; lists of positions have no common tokens
   n.abreast = a.n_lists == 0 && n.units <= resident && resident % n.units * 16 <= resident ? n.units : 1;
+  // steps are counted in 32 bits
+  n.step_shift = kStepShift;
+  while (units / n.abreast * ((most >> n.step_shift) + 1 + kLead) >= (int64_t(1) << 30)) { ++n.step_shift; }
+  const int64_t steps = (most + (int64_t(1) << n.step_shift) - 1) >> n.step_shift;
   n.shares  = std::min({resident / n.abreast, kMostShares, units / n.abreast * (steps + kLead)});
   n.blocks  = n.cluster ? units * n.cluster : n.shares * n.abreast;
   n.part_floats = n.per_unit * (dim + 4);
-  n.bytes       = n.cluster ? 0 : static_cast<size_t>(n.blocks) * 2 * (sizeof(float) * n.part_floats + sizeof(int64_t));
+  n.bytes       = n.cluster ? 0 : static_cast<size_t>(n.blocks) * 2 * (sizeof(float) * n.part_floats + sizeof(int32_t));
   n.by_unit     = units <= n.blocks;
   return n;
 }
@@ -71,6 +75,15 @@ int unit_shift(const certexB200PagedCache_t& c)
 }
 
 }  // namespace
+
+void paged_divisor(uint32_t d, uint32_t& factor, int32_t& shift)
+{
+  // with 2^(s-1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1, m d exceeds 2^(31 + s) by e <= d <= 2^s, and floor(n m / 2^(31 + s)) is
+  // n / d for all n < 2^31: the excess n e / (d 2^(31 + s)) stays below 1 / d
+  shift = 0;
+  while ((uint64_t(1) << shift) < d) { ++shift; }
+  factor = static_cast<uint32_t>((uint64_t(1) << (31 + shift)) / d + 1);
+}
 
 bool paged_within_reach(const certexB200PagedCache_t& c)
 {
@@ -102,23 +115,23 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.v_page          = units(a.cache.value_strides[0]);
   p.v_token         = units(a.cache.value_strides[1]);
   p.v_head          = a.cache.value_strides[2];
-  p.n_places        = a.cache.n_pages * a.cache.page_size;
+  p.n_places        = static_cast<int32_t>(a.cache.n_pages * a.cache.page_size);
   p.n_pages         = static_cast<int32_t>(a.cache.n_pages);
   p.page_size       = static_cast<uint32_t>(a.cache.page_size);
-  p.page_shift      = (a.cache.page_size & (a.cache.page_size - 1)) == 0 ? __builtin_ctzll(a.cache.page_size) : -1;
+  paged_divisor(p.page_size, p.page_factor, p.page_shift);
   p.dim             = static_cast<int32_t>(a.cache.head_dim);
   p.fault           = a.cache.fault;
   p.pages           = a.table.pages;
   p.page_row        = a.table.row_stride;
   p.n_sequences     = a.table.n_sequences;
-  p.most            = std::min(a.table.pages_per_sequence * a.cache.page_size, kMostTokens);
+  p.most            = static_cast<int32_t>(std::min(a.table.pages_per_sequence * a.cache.page_size, kMostTokens));
   p.row_to_sequence = a.table.row_to_sequence;
   p.lengths         = a.lengths;
-  p.window          = a.window;
+  p.window          = static_cast<int32_t>(std::min(a.window, kMostTokens));
   p.lists           = a.selected;
   p.lists_64        = a.selected_64;
   p.n_lists         = static_cast<int32_t>(a.n_lists);
-  p.k               = a.k;
+  p.k               = static_cast<int32_t>(a.k);
   p.q               = a.q.data;
   p.q_row           = a.q.row_stride;
   p.q_head          = a.q.head_stride;
@@ -128,7 +141,7 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.o_row           = a.out.row_stride;
   p.o_head          = a.out.head_stride;
   p.lse             = a.lse;
-  p.n_rows          = a.n_rows;
+  p.n_rows          = static_cast<int32_t>(a.n_rows);
   p.n_heads         = static_cast<int32_t>(a.n_heads);
   p.group           = static_cast<int32_t>(a.n_heads / a.cache.n_kv_heads);
   p.subs            = n.subs;
@@ -137,18 +150,19 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.scale           = a.scale * kLog2e;
   p.cluster         = n.cluster;
   p.warps           = n.warps;
+  p.step_shift      = n.step_shift;
   p.shares          = static_cast<int32_t>(n.shares);
   p.abreast         = n.cluster ? 1 : n.abreast;
   p.in_line         = n.units / n.abreast;
   p.by_unit         = n.by_unit;
-  p.joints          = n.by_unit ? a.n_rows * n.units : n.shares * n.abreast;
-  const int64_t all = p.joints * n.per_unit;  // queries to be joined
+  p.joints          = static_cast<int32_t>(n.by_unit ? a.n_rows * n.units : n.shares * n.abreast);
+  const int64_t all = int64_t(p.joints) * n.per_unit;  // queries to be joined
   const bool few    = n.blocks <= 8 * a.n_rows * n.units;  // shares each, on average
   p.join_lanes      = few || all > 4 * sm_count ? 0 : all <= sm_count ? 8 : p.dim <= 128 ? 32 : 64;
   p.part_floats     = n.part_floats;
   p.parts           = static_cast<float*>(a.workspace);
   const bool one    = a.n_lists > 0 || a.n_rows == 1;
-  p.marks           = n.cluster || one ? nullptr : reinterpret_cast<int64_t*>(p.parts + 2 * n.blocks * n.part_floats);
+  p.marks           = n.cluster || one ? nullptr : reinterpret_cast<int32_t*>(p.parts + 2 * n.blocks * n.part_floats);
   switch (a.cache.dtype) {
     case kPagedF32: return launch_attend_f32(p, n.blocks, s);
     case kPagedF16: return launch_attend_f16(p, n.blocks, s);

@@ -12,7 +12,7 @@
 //  * One pass. Scores, the running maximum m, the running sum l and the output stay in registers in float32;
 //    when m grows, l and the output are multiplied by exp2(m_old - m_new). Scores are kept in units of log2 e, so that a
 //    weight is one subtraction and one exp2.
-//  * The stream is split evenly. The tokens that all rows of the call see, in steps of kStep, are one sequence of work that
+//  * The stream is split evenly. The tokens that all rows of the call see, in steps of 32, are one sequence of work that
 //    is cut into equal shares, a share per resident block, wherever the cuts fall: 1 row of 131 072 keys and 64 rows of 1 to
 //    8192 keys load the GPU alike, and lengths are read on the device only. A row and KV head ("unit") that
 //    a cut divides leaves a partial result (m, l, output) per share, which a second, small kernel joins in the order of the
@@ -48,8 +48,9 @@ struct AttendParams {
   uint32_t k_page, k_token, v_page, v_token;
   int64_t k_head, v_head;
   int32_t unit_shift;
-  int32_t page_shift;  // log2 of page_size, -1: no power of two
-  int64_t n_places;    // n_pages * page_size
+  uint32_t page_factor;  // t / page_size = (2 t * page_factor >> 32) >> page_shift
+  int32_t page_shift;
+  int32_t n_places;      // n_pages * page_size
   int32_t n_pages;
   uint32_t page_size;
   int32_t dim;
@@ -57,13 +58,14 @@ struct AttendParams {
   // what a row sees
   const int32_t* pages;
   int64_t page_row;
-  int64_t n_sequences, most;  // most: tokens that the table can hold
+  int64_t n_sequences;
+  int32_t most;               // tokens that the table can hold
   const int32_t* row_to_sequence;
   const int32_t* lengths;     // null: lists
-  int64_t window;
+  int32_t window;
   const void* lists;
   int32_t lists_64, n_lists;
-  int64_t k;
+  int32_t k;
   // queries and answers
   const void* q;
   int64_t q_row, q_head;
@@ -71,13 +73,14 @@ struct AttendParams {
   void* out;
   int64_t o_row, o_head;
   float* lse;
-  int64_t n_rows;
+  int32_t n_rows;
   int32_t n_heads, group, subs, per_unit;  // query heads per KV head; units per KV head; query heads of a unit
   int32_t units;                           // of a row
   float scale;                             // in units of log2 e
   // the split
   int32_t warps;       // of a block
   int32_t cluster;     // blocks of a unit, in a cluster; 0: the work is split evenly
+  int32_t step_shift;  // log2 of the tokens of a step
   int32_t shares;      // that the work is split into at most
   int32_t abreast;     // blocks of a share: 1, or the units of a row
   int32_t in_line;     // units of a row that lie behind one another among the steps: units / abreast
@@ -85,8 +88,8 @@ struct AttendParams {
   // where that follows from one length it finds a unit's shares itself; otherwise (not null) the blocks leave it, [blocks][2]:
   // the unit that a block begins and leaves unfinished, and how many shares it has (0: there is none), or by unit, [units][2]:
   // the share that begins it, and how many it has (0: no more than that)
-  int64_t* marks;
-  int64_t joints;      // units or blocks that it looks at
+  int32_t* marks;
+  int32_t joints;      // units or blocks that it looks at
   int32_t join_lanes;  // 0: a warp for a joint's query; else its threads that share a partial result, with four coordinates each
   float* parts;        // [blocks][2] partial results of part_floats each
   int32_t part_floats;
@@ -99,8 +102,8 @@ void launch_attend_bf16(const AttendParams& p, int64_t blocks, cudaStream_t s);
 
 namespace {
 
-constexpr int kStep = 32;  // tokens of a step of the work split
-constexpr int kLead = 4;   // steps that a unit's beginning and end count for: fetching its first tiles, joining the warps
+constexpr int kStepShift = 5;  // the work is cut in steps of 32 tokens (more where 32 bits would not count them)
+constexpr int kLead      = 4;  // steps that a unit's beginning and end count for: fetching its first tiles, joining the warps
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2   = 0.6931471805599453f;
 
@@ -151,31 +154,30 @@ struct Span {
   int32_t sequence;
 };
 
-__device__ __forceinline__ Span span_of(const AttendParams& p, int64_t row)
+__device__ __forceinline__ Span span_of(const AttendParams& p, int32_t row)
 {
-  if (p.lengths == nullptr) { return {0, static_cast<int32_t>(p.k), 0}; }
-  int32_t end             = p.lengths[row];
-  const int64_t sequence = p.row_to_sequence ? p.row_to_sequence[row] : row;
+  if (p.lengths == nullptr) { return {0, p.k, 0}; }
+  int32_t end            = p.lengths[row];
+  const int32_t sequence = p.row_to_sequence ? p.row_to_sequence[row] : row;
   if (end <= 0) { return {0, 0, 0}; }
   const bool stranger = sequence < 0 || sequence >= p.n_sequences;
   if (stranger || end > p.most) { *p.fault = 1; }
   if (stranger) { return {0, 0, 0}; }
-  end                 = static_cast<int32_t>(min(int64_t(end), p.most));
-  const int32_t begin = p.window > 0 && end > p.window ? static_cast<int32_t>(end - p.window) : 0;
-  return {begin, end - begin, static_cast<int32_t>(sequence)};
+  end                 = min(end, p.most);
+  const int32_t begin = p.window > 0 && end > p.window ? end - p.window : 0;
+  return {begin, end - begin, sequence};
 }
 
 /// One unit's share: tokens [i0, i1) of what its row sees.
 struct Segment {
-  int64_t row;
-  int32_t kv, head, n_heads;  // KV head, first query head, query heads
+  int32_t row, kv, head, n_heads;  // KV head, first query head, query heads
   int32_t slot;               // of the partial result, -1: this is the whole unit
   int32_t i0, i1;
   int32_t begin;
   const void* index;          // the sequence's row of the table, or the list
 };
 
-__device__ __forceinline__ Segment segment_of(const AttendParams& p, int64_t row, const Span& s, int unit)
+__device__ __forceinline__ Segment segment_of(const AttendParams& p, int32_t row, const Span& s, int unit)
 {
   Segment g;
   g.row     = row;
@@ -187,7 +189,7 @@ __device__ __forceinline__ Segment segment_of(const AttendParams& p, int64_t row
   if (p.lengths) {
     g.index = p.pages + s.sequence * p.page_row;
   } else {
-    const int64_t list = p.n_lists == 1 ? row : p.n_lists == p.n_heads ? row * p.n_lists + g.head : row * p.n_lists + g.kv;
+    const int64_t list = int64_t(row) * p.n_lists + (p.n_lists == 1 ? 0 : p.n_lists == p.n_heads ? g.head : g.kv);
     g.index            = static_cast<const char*>(p.lists) + list * p.k * (p.lists_64 ? 8 : 4);
   }
   return g;
@@ -199,42 +201,27 @@ struct Place {
 };
 constexpr uint32_t kNowhere = ~0u;
 
+/// Whole pages in t < 2^31 tokens.
+__device__ __forceinline__ uint32_t pages_in(const AttendParams& p, uint32_t t) { return __umulhi(2 * t, p.page_factor) >> p.page_shift; }
+
 /// Entry of the table, or of the list, that token i of what a row sees goes by (with the segment's begin and index). Nothing here
 /// depends on what is read: the kernels ask for it a tile before they need it.
 __device__ __forceinline__ int64_t entry_of(const AttendParams& p, int32_t begin, const void* index, int32_t i)
 {
-  if (p.lengths) {
-    const auto t = static_cast<uint32_t>(begin + i);
-    return static_cast<const int32_t*>(index)[p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size];
-  }
+  if (p.lengths) { return static_cast<const int32_t*>(index)[pages_in(p, begin + i)]; }
   return p.lists_64 ? static_cast<const int64_t*>(index)[i] : static_cast<const int32_t*>(index)[i];
 }
 
 /// The place of token i from its entry.
 __device__ __forceinline__ Place place_of(const AttendParams& p, int32_t begin, int32_t i, int64_t entry)
 {
-  uint32_t page, place;
-  if (p.lengths) {
-    const auto t     = static_cast<uint32_t>(begin + i);
-    place            = p.page_shift >= 0 ? t & (p.page_size - 1) : t % p.page_size;
-    page             = static_cast<uint32_t>(entry);
-    if (page >= static_cast<uint32_t>(p.n_pages)) {  // negative entries too
-      *p.fault = 1;
-      return {kNowhere, kNowhere};
-    }
-  } else {
-    if (entry < 0) { return {kNowhere, kNowhere}; }
-    if (entry >= p.n_places) {
-      *p.fault = 1;
-      return {kNowhere, kNowhere};
-    }
-    if (p.page_shift >= 0) {
-      page = static_cast<uint32_t>(entry >> p.page_shift);
-    } else {
-      page = entry >> 32 ? static_cast<uint32_t>(entry / p.page_size) : static_cast<uint32_t>(entry) / p.page_size;
-    }
-    place = static_cast<uint32_t>(entry) - page * p.page_size;
-  }
+  // its number among the tokens of its sequence, or of the cache
+  const uint32_t t = p.lengths ? static_cast<uint32_t>(begin + i) : static_cast<uint32_t>(entry);
+  const uint32_t n = pages_in(p, t), place = t - n * p.page_size;
+  const uint32_t page = p.lengths ? static_cast<uint32_t>(entry) : n;
+  const bool wrong    = p.lengths ? page >= static_cast<uint32_t>(p.n_pages) : entry >= p.n_places;  // (pages: negative ones too)
+  if (wrong) { *p.fault = 1; }
+  if (wrong || (!p.lengths && entry < 0)) { return {kNowhere, kNowhere}; }
   return {page * p.k_page + place * p.k_token, page * p.v_page + place * p.v_token};
 }
 
@@ -243,57 +230,57 @@ __device__ __forceinline__ Place place_of(const AttendParams& p, int32_t begin, 
 // Sequences are split with their units side by side instead (`abreast`): a row counts once, and every share belongs to as many
 // neighbouring blocks as a row has units, one each. They go through the same tokens at the same time, whose heads lie next to
 // one another in memory where the heads are the inner axis.
-__device__ __forceinline__ int64_t steps_for(int32_t count) { return count > 0 ? (static_cast<uint32_t>(count) + kStep - 1) / kStep + kLead : 0; }
-
-/// a / b, in 32 bits where they will do (64-bit divisions are long chains of instructions).
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b)
+__device__ __forceinline__ int32_t steps_for(const AttendParams& p, int32_t count)
 {
-  return (a | b) >> 31 ? a / b : int64_t(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+  return count > 0 ? static_cast<int32_t>((static_cast<uint32_t>(count) + (1u << p.step_shift) - 1) >> p.step_shift) + kLead : 0;
 }
 
+/// a / b of what is not negative (signed division is a longer chain of instructions).
+__device__ __forceinline__ int32_t divide(int32_t a, int32_t b) { return static_cast<uint32_t>(a) / static_cast<uint32_t>(b); }
+
 struct Split {
-  int64_t total, shares, each, more;  // the first `more` shares have a step more than `each`
+  int32_t total, shares, each, more;  // the first `more` shares have a step more than `each`
   Split() = default;
-  __device__ Split(int64_t steps, int64_t most) : total(steps), shares(min(most, steps)), each(0), more(0)
+  __device__ Split(int32_t steps, int32_t most) : total(steps), shares(min(most, steps)), each(0), more(0)
   {
     if (shares > 0) {
       each = divide(total, shares);
       more = total - each * shares;
     }
   }
-  __device__ int64_t first_step(int64_t w) const { return w * each + min(w, more); }
-  __device__ int64_t share_of(int64_t step) const
+  __device__ int32_t first_step(int32_t w) const { return w * each + min(w, more); }
+  __device__ int32_t share_of(int32_t step) const
   {
-    const int64_t x = more * (each + 1);
+    const int32_t x = more * (each + 1);
     return step < x ? divide(step, each + 1) : more + divide(step - x, each);
   }
 };
 
 /// A unit's place among the steps.
 struct Unit {
-  int64_t row, begin, steps;  // begin: its first step
-  int unit;
+  int32_t row, begin, steps;  // begin: its first step
+  int32_t unit;
   Span span;
 };
 
 /// The split and where a block's share of it begins; a block of W warps calls it as a whole.
 struct Start {
   Split split;
-  int64_t at;  // the share's first step
+  int32_t at;  // the share's first step
   Unit unit;   // whose steps that is among; undefined when the split has not so many shares
 };
 
 template <int W>
-__device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
+__device__ __forceinline__ Start start_of(const AttendParams& p, int32_t share)
 {
   constexpr int kThreads = W * 32;
-  __shared__ int64_t sums[W];
-  __shared__ int64_t found[2];
+  __shared__ int32_t sums[W];
+  __shared__ int32_t found[2];
   __shared__ Span spans;
   const bool alike = !p.lengths || p.n_rows == 1;  // every unit has the same steps
   if (alike) {
     const Span span     = span_of(p, 0);
-    const int64_t steps = steps_for(span.count), each = steps * p.in_line;
+    const int32_t steps = steps_for(p, span.count), each = steps * p.in_line;
     Start x{Split(p.n_rows * each, p.shares), 0, {0, 0, steps, 0, span}};
     if (share >= x.split.shares) { return x; }
     x.at         = x.split.first_step(share);
@@ -306,12 +293,12 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
   // an inclusive sum over the block for kThreads rows at a time; the total first, where they are more
   if (threadIdx.x == 0) { found[0] = -1; }
   __syncthreads();
-  int64_t total = 0;
+  int32_t total = 0;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const bool once = p.n_rows <= kThreads;
   if (!once) {
-    int64_t mine = 0;
-    for (int64_t row = threadIdx.x; row < p.n_rows; row += kThreads) { mine += steps_for(span_of(p, row).count); }
+    int32_t mine = 0;
+    for (int32_t row = threadIdx.x; row < p.n_rows; row += kThreads) { mine += steps_for(p, span_of(p, row).count); }
     for (int o = 16; o > 0; o >>= 1) { mine += __shfl_xor_sync(~0u, mine, o); }
     if (lane == 0) { sums[warp] = mine; }
     __syncthreads();
@@ -320,21 +307,21 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
   }
   Start x{Split(total * p.in_line, p.shares), 0, {}};
   if (!once) { x.at = x.split.first_step(share); }
-  int64_t before = 0;
-  for (int64_t r0 = 0; r0 < p.n_rows; r0 += kThreads) {
-    const int64_t r = r0 + threadIdx.x;
+  int32_t before = 0;
+  for (int32_t r0 = 0; r0 < p.n_rows; r0 += kThreads) {
+    const int32_t r = r0 + threadIdx.x;
     const Span span = r < p.n_rows ? span_of(p, r) : Span{0, 0, 0};
-    const int64_t n = steps_for(span.count) * p.in_line;
-    int64_t upto    = n;
+    const int32_t n = steps_for(p, span.count) * p.in_line;
+    int32_t upto    = n;
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(~0u, upto, o);
+      const int32_t y = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) { upto += y; }
     }
     if (W > 1) {
       if (lane == 31) { sums[warp] = upto; }
       __syncthreads();
     }
-    int64_t first = before + upto - n;
+    int32_t first = before + upto - n;
     if (W > 1) {
       for (int i = 0; i < W; ++i) {
         if (i < warp) { first += sums[i]; }
@@ -356,7 +343,7 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int64_t share)
   if (share < x.split.shares) {
     x.unit.row   = found[0];
     x.unit.span  = spans;
-    x.unit.steps = steps_for(spans.count);
+    x.unit.steps = steps_for(p, spans.count);
     const auto u = divide(x.at - found[1], x.unit.steps);
     x.unit.unit  = static_cast<int>(u);
     x.unit.begin = found[1] + u * x.unit.steps;
@@ -369,41 +356,40 @@ template <typename T, int W, typename F>
 __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
 {
   constexpr int kThreads = W * 32;
-  auto nothing_seen = [&](int64_t row, int head, int n_heads) {
+  auto nothing_seen = [&](int32_t row, int head, int n_heads) {
     for (int h = head; h < head + n_heads; ++h) {
-      T* o = static_cast<T*>(p.out) + row * p.o_row + h * p.o_head;
+      T* o = static_cast<T*>(p.out) + int64_t(row) * p.o_row + h * p.o_head;
       for (int c = threadIdx.x; c < p.dim; c += kThreads) { o[c] = Type<T>::down(0.f); }
-      if (p.lse && threadIdx.x == 0) { p.lse[row * p.n_heads + h] = -INFINITY; }
+      if (p.lse && threadIdx.x == 0) { p.lse[int64_t(row) * p.n_heads + h] = -INFINITY; }
     }
   };
   // What a block works on lies in shared memory: the registers are needed for the work. The first thread of the last warp, which
   // has the fewest tiles, works out the next segment while the others begin with one.
   struct State {
-    int64_t at, end;
+    int32_t at, end;
     Split split;
     Unit u;
   };
   __shared__ Segment segments[2];
   __shared__ State state;
-  const int64_t share = blockIdx.x / static_cast<uint32_t>(p.abreast);
-  const int beside    = static_cast<int>(blockIdx.x - share * p.abreast);
-  auto next           = [&](Segment& g) {
+  const int32_t block = blockIdx.x, share = divide(block, p.abreast), beside = block - share * p.abreast;
+  auto next = [&](Segment& g) {
     g.n_heads = 0;  // nothing left
     while (state.at < state.end) {
       Unit u           = state.u;
-      const int64_t at = state.at, end = state.end, to = min(end, u.begin + u.steps);
-      const auto i0 = static_cast<int32_t>(max(int64_t(0), at - u.begin - kLead) * kStep);
-      const auto i1 = static_cast<int32_t>(min(int64_t(u.span.count), max(int64_t(0), to - u.begin - kLead) * kStep));
+      const int32_t at = state.at, end = state.end, to = min(end, u.begin + u.steps);
+      const int32_t i0 = max(0, at - u.begin - kLead) << p.step_shift;
+      const auto i1    = static_cast<int32_t>(min(int64_t(u.span.count), int64_t(max(0, to - u.begin - kLead)) << p.step_shift));
       if (i0 < i1) {  // (a share may end within a unit's lead)
         const int unit    = u.unit + beside;
         g                 = segment_of(p, u.row, u.span, unit);
         const bool begins = i0 == 0, ends = i1 == u.span.count;
         g.i0 = i0, g.i1 = i1;
         // a partial result that begins a unit belongs to the block's second slot, one that goes on with it to the first
-        g.slot = begins && ends ? -1 : static_cast<int32_t>(2 * blockIdx.x + (begins ? 1 : 0));
+        g.slot = begins && ends ? -1 : 2 * block + (begins ? 1 : 0);
         if (p.marks && begins && (!ends || p.by_unit)) {
-          const int64_t id = u.row * p.units + unit;
-          int64_t* mark    = p.marks + 2 * (p.by_unit ? id : blockIdx.x);
+          const int32_t id = u.row * p.units + unit;
+          int32_t* mark    = p.marks + 2 * (p.by_unit ? id : block);
           mark[0]          = p.by_unit ? share : id;
           mark[1]          = ends ? 0 : state.split.share_of(u.begin + u.steps - 1) - share + 1;
         }
@@ -415,7 +401,7 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
           do {  // (there are steps left: a row behind has some, unless somebody changes the lengths meanwhile)
             u.span = ++u.row < p.n_rows ? span_of(p, u.row) : Span{0, 0, 0};
           } while (u.span.count == 0 && u.row < p.n_rows);
-          u.steps = steps_for(u.span.count);
+          u.steps = steps_for(p, u.span.count);
         }
         state.u = u;
       }
@@ -426,23 +412,22 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
   constexpr int kScribe = kThreads - 32;
   if (p.cluster) {
     // the blocks of a cluster share a unit's tokens, 16 by 16
-    const uint32_t unit = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
-    const int64_t row = unit / static_cast<uint32_t>(p.units);
-    const Span s      = span_of(p, row);
-    Segment g         = segment_of(p, row, s, static_cast<int>(unit - row * p.units));
+    const int32_t unit = divide(block, p.cluster), rank = block - unit * p.cluster, row = divide(unit, p.units);
+    const Span s = span_of(p, row);
+    Segment g    = segment_of(p, row, s, unit - row * p.units);
     if (s.count == 0) {
       if (rank == 0) { nothing_seen(row, g.head, g.n_heads); }
       return;
     }
-    const int64_t tiles = (int64_t(s.count) + 15) / 16;
-    g.i0   = static_cast<int32_t>(tiles * rank / p.cluster * 16);
-    g.i1   = static_cast<int32_t>(min(int64_t(s.count), tiles * (rank + 1) / p.cluster * 16));
+    const int32_t tiles = (s.count + 15) / 16;  // (a cluster's rows are short)
+    g.i0   = divide(tiles * rank, p.cluster) * 16;
+    g.i1   = min(s.count, divide(tiles * (rank + 1), p.cluster) * 16);
     g.slot = -1;
     if (threadIdx.x == kScribe) { segments[0] = g, state.at = state.end = 0; }
   } else {
     // rows that see nothing have no steps: the blocks share them out
     if (p.lengths) {
-      for (int64_t row = blockIdx.x; row < p.n_rows; row += gridDim.x) {
+      for (int32_t row = block; row < p.n_rows; row += gridDim.x) {
         if (span_of(p, row).count == 0) {
           nothing_seen(row, 0, p.n_heads);
           if (p.marks && p.by_unit) {
@@ -452,7 +437,7 @@ __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
       }
     }
     const Start x = start_of<W>(p, share);
-    if (p.marks && !p.by_unit && threadIdx.x == kScribe) { p.marks[2 * int64_t(blockIdx.x) + 1] = 0; }
+    if (p.marks && !p.by_unit && threadIdx.x == kScribe) { p.marks[2 * block + 1] = 0; }
     if (share >= x.split.shares) { return; }
     if (threadIdx.x == kScribe) {
       state.at = x.at, state.end = x.split.first_step(share + 1), state.split = x.split, state.u = x.unit;
@@ -474,7 +459,7 @@ __device__ __forceinline__ void put_out(const AttendParams& p, const Segment& g,
   if (g.slot >= 0) {
     p.parts[int64_t(g.slot) * p.part_floats + 4 * p.per_unit + i * p.dim + c] = v;
   } else {
-    (static_cast<T*>(p.out) + g.row * p.o_row + (g.head + i) * p.o_head)[c] = Type<T>::down(v);
+    (static_cast<T*>(p.out) + int64_t(g.row) * p.o_row + (g.head + i) * p.o_head)[c] = Type<T>::down(v);
   }
 }
 
@@ -485,7 +470,7 @@ __device__ __forceinline__ void put_sums(const AttendParams& p, const Segment& g
     float* to = p.parts + int64_t(g.slot) * p.part_floats + 4 * i;
     to[0] = m, to[1] = l, to[2] = any ? 1.f : 0.f;
   } else if (p.lse) {
-    p.lse[g.row * p.n_heads + g.head + i] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+    p.lse[int64_t(g.row) * p.n_heads + g.head + i] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
 }
 
@@ -768,7 +753,7 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
     // the queries, as the 8-column side of the first product; a lane takes the same coordinates of a query as of a key
     uint32_t qf[NT][kSteps][2];
     {
-      const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
+      const T* q = static_cast<const T*>(p.q) + int64_t(g.row) * p.q_row + g.head * p.q_head;
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
         const int i  = x * 8 + g8;
@@ -1017,7 +1002,7 @@ __global__ void __launch_bounds__(W * 32, 4 / W) attend_ring_kernel(const Attend
     // the queries, as the 8-column side of the first product
     uint32_t qf[NT][D / 16][2];
     {
-      const T* q = static_cast<const T*>(p.q) + g.row * p.q_row + g.head * p.q_head;
+      const T* q = static_cast<const T*>(p.q) + int64_t(g.row) * p.q_row + g.head * p.q_head;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int i  = n * 8 + g8;
@@ -1219,7 +1204,7 @@ __global__ void __launch_bounds__(W * 32, 8 / W) attend_float_kernel(const Atten
       return j < n && token_of(j) < i1 ? place_of(p, begin, token_of(j), entry) : Place{kNowhere, kNowhere};
     };
     int64_t entry0 = ask(0), entry = ask(1);
-    const float* q = static_cast<const float*>(p.q) + g.row * p.q_row + g.head * p.q_head;
+    const float* q = static_cast<const float*>(p.q) + int64_t(g.row) * p.q_row + g.head * p.q_head;
     for (int i = threadIdx.x; i < Q * D; i += W * 32) {
       const int x = i / D, c = i % D;
       q_s[i] = x < g.n_heads && c < p.dim ? q[x * p.q_head + c] : 0.f;
@@ -1451,31 +1436,31 @@ constexpr int kJoinThreads = 256;
 // What is joined is numbered by units, or by the blocks that may have begun one. Partial results lie in the second slot of the
 // block that began the unit and in the first slots of those of the shares behind it.
 struct Joint {
-  int64_t row, first;  // first: the share that begins the unit
-  int unit, beside;
-  int n;               // its shares; 0: there is nothing to join
+  int32_t row, first;  // first: the share that begins the unit
+  int32_t unit, beside;
+  int32_t n;           // its shares; 0: there is nothing to join
 };
 
 /// Every thread of a joining kernel calls this: when it returns, the first kernel has ended and its results are there. (A kernel
 /// that is launched ahead of another's end must not end before it.)
-__device__ __forceinline__ Joint joint_of(const AttendParams& p, int64_t x)
+__device__ __forceinline__ Joint joint_of(const AttendParams& p, int32_t x)
 {
   Joint j{0, 0, 0, 0, 0};
-  int64_t id = 0;
+  int32_t id = 0;
   if (p.marks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (x >= p.joints) { return j; }
-    j.n                = static_cast<int>(p.marks[2 * x + 1]);
-    const int64_t mark = p.marks[2 * x];
+    j.n                = p.marks[2 * x + 1];
+    const int32_t mark = p.marks[2 * x];
     id                 = p.by_unit ? x : mark;
     j.first            = p.by_unit ? mark : divide(x, p.abreast);
   } else {
     // one length, so every unit has the same steps
-    const int64_t steps = x < p.joints ? steps_for(span_of(p, 0).count) : 0;
+    const int32_t steps = x < p.joints ? steps_for(p, span_of(p, 0).count) : 0;
     if (steps > 0) {
       const Split split(steps * p.n_rows * p.in_line, p.shares);
-      const int64_t share = divide(x, p.abreast);
-      int64_t at          = -1;  // the unit's number among those that lie behind one another
+      const int32_t share = divide(x, p.abreast);
+      int32_t at          = -1;  // the unit's number among those that lie behind one another
       if (p.by_unit) {
         id = x;
         at = p.abreast == 1 ? id : divide(id, p.units);
@@ -1485,15 +1470,15 @@ __device__ __forceinline__ Joint joint_of(const AttendParams& p, int64_t x)
       }
       if (at >= 0) {
         j.first         = split.share_of(at * steps + kLead);
-        const int64_t n = split.share_of((at + 1) * steps - 1) - j.first + 1;
-        if (n > 1 && (p.by_unit || j.first == share)) { j.n = static_cast<int>(n); }
+        const int32_t n = split.share_of((at + 1) * steps - 1) - j.first + 1;
+        if (n > 1 && (p.by_unit || j.first == share)) { j.n = n; }
       }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
   }
   if (j.n > 0) {
     j.row    = divide(id, p.units);
-    j.unit   = static_cast<int>(id - j.row * p.units);
+    j.unit   = id - j.row * p.units;
     j.beside = p.abreast == 1 ? 0 : j.unit;
   }
   return j;
@@ -1501,18 +1486,16 @@ __device__ __forceinline__ Joint joint_of(const AttendParams& p, int64_t x)
 
 __device__ __forceinline__ const float* part_of(const AttendParams& p, const Joint& j, int x)
 {
-  return p.parts + (2 * ((j.first + x) * p.abreast + j.beside) + (x == 0 ? 1 : 0)) * p.part_floats;
+  return p.parts + int64_t(2 * ((j.first + x) * p.abreast + j.beside) + (x == 0 ? 1 : 0)) * p.part_floats;
 }
 
 /// Many units with few shares each: a warp joins one query of one of them, four shares at a time with a running maximum.
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_many_kernel(const AttendParams p)
 {
-  const int64_t item = (int64_t(blockIdx.x) * kJoinThreads + threadIdx.x) / 32;
-  const int lane     = threadIdx.x % 32;
-  const int64_t x    = divide(item, p.per_unit);
-  const int i        = static_cast<int>(item - x * p.per_unit);
-  const Joint j      = joint_of(p, x);
+  const int32_t item = blockIdx.x * (kJoinThreads / 32) + threadIdx.x / 32, x = divide(item, p.per_unit);
+  const int lane = threadIdx.x % 32, i = item - x * p.per_unit;
+  const Joint j  = joint_of(p, x);
   if (j.n == 0) { return; }
   const Segment g = segment_of(p, j.row, Span{0, 0, 0}, j.unit);
   if (i >= g.n_heads) { return; }
@@ -1552,7 +1535,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_many_kernel(const AttendPar
       for (int h = 0; h < 2; ++h) { v[h].x += f * o[y][h].x, v[h].y += f * o[y][h].y, v[h].z += f * o[y][h].z, v[h].w += f * o[y][h].w; }
     }
   }
-  T* out = static_cast<T*>(p.out) + j.row * p.o_row + (g.head + i) * p.o_head;
+  T* out = static_cast<T*>(p.out) + int64_t(j.row) * p.o_row + (g.head + i) * p.o_head;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int c = lane * 4 + h * 128;
@@ -1562,7 +1545,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_many_kernel(const AttendPar
       for (int y = 0; y < 4; ++y) { out[c + y] = Type<T>::down(seen > 0.f ? r[y] / sum : 0.f); }
     }
   }
-  if (p.lse && lane == 0) { p.lse[j.row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
+  if (p.lse && lane == 0) { p.lse[int64_t(j.row) * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY; }
 }
 
 /// Few units with many shares each: block (x, i, z) joins query i of joint x, coordinates 4 * join_lanes * z on. Sums and outputs are
@@ -1641,10 +1624,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendParams p
   for (int x = threadIdx.x; x < min(lanes * 4, p.dim - from_c); x += kJoinThreads) {
     float r = 0.f;
     for (int y = 0; y < groups; ++y) { r += reinterpret_cast<const float*>(outs + y * lanes)[x]; }
-    (static_cast<T*>(p.out) + g.row * p.o_row + (g.head + i) * p.o_head)[from_c + x] = Type<T>::down(seen > 0.f ? r / sum : 0.f);
+    (static_cast<T*>(p.out) + int64_t(g.row) * p.o_row + (g.head + i) * p.o_head)[from_c + x] = Type<T>::down(seen > 0.f ? r / sum : 0.f);
   }
   if (p.lse && threadIdx.x == 0 && blockIdx.z == 0) {
-    p.lse[g.row * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    p.lse[int64_t(g.row) * p.n_heads + g.head + i] = seen > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
   }
 }
 

@@ -125,7 +125,8 @@ def test_the_library_refuses_what_it_cannot_read(built_library):
         (lambda: attend(cache=_cache_args(keys=72)), b"16 bytes"), (lambda: attend(cache=_cache_args(v1=2)), b"16 bytes"),
         (lambda: attend(cache=_cache_args(fault=0)), b"null cache"), (lambda: attend(cache=_cache_args(page_size=0)), b"pages"),
         (lambda: attend(table=None), b"table"), (lambda: attend(lengths=None), b"lengths"), (lambda: attend(window=-1), b"window"),
-        (lambda: attend(cache=_cache_args(kv=2), heads=3), b"multiple"), (lambda: attend(n=-1), b"rows"), (lambda: attend(n=2**31), b"rows"),
+        (lambda: attend(cache=_cache_args(kv=2), heads=3), b"multiple"), (lambda: attend(n=-1), b"rows"), (lambda: attend(n=2**31), b"rows"), (lambda: attend(n=2**27), b"rows"),
+        (lambda: attend(cache=_cache_args(n_pages=2**16, page_size=2**15)), b"places"), (lambda: attend(cache=_cache_args(n_pages=2**20, page_size=16, k0=-64)), b"strides"),
         (lambda: attend(scale=math.inf), b"finite"), (lambda: attend(scale=math.nan), b"finite"), (lambda: attend(), b"null resources"),
         (lambda: selected(lists=2, heads=4), b"list"), (lambda: selected(at=None), b"positions"), (lambda: selected(k=-1), b"positions"),
         (lambda: selected(), b"null resources"), (lambda: append(k=None), b"null keys"), (lambda: append(heads=2, q=rows), b"rotation"),
