@@ -15,9 +15,10 @@ constexpr int64_t kMostShares = kJoinSums * kJoinThreads;
 constexpr int64_t kClusterTokens = 256;
 
 /// Shares of a unit, on average, from which blocks have four warps. Below that smaller blocks wait less for one another: 128 rows of
-/// 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), float32 keys of 16 rows 192 us with four and 175 with
-/// one. Above, there are too many results to join: one row and KV head of 131 072 keys took 30 us with two warps and 24 with four.
-constexpr int64_t kManyShares = 64;
+/// 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), one row of 131 072 keys of 8 heads 91.9 and 91.3, float32 keys of
+/// 16 rows 192 us with four and 175 with one. Above, there are too many results to join: one row and KV head of 131 072 keys took 30 us
+/// with two warps and 24 with four.
+constexpr int64_t kManyShares = 128;
 
 struct Plan {
   int32_t per_unit, subs, units, warps;

@@ -66,10 +66,11 @@ struct Section {
   bool turn, paged;
 };
 
+
 template <typename T>
 struct TurnArgs {
   Section<T> sec[3];
-  int32_t n_sec;
+  int32_t n_sec;  // sections that have threads of their own; the values after them, where a thread takes a key and its value
   const uint64_t* turns;
   int32_t rotary_dim, dim;
   float magnitude;
@@ -182,6 +183,13 @@ __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
     from += kAt * sec.src_head;
   };
   load(0);  // on their way while the page is looked up
+  const Section<T>& values = a.sec[HEADS == 1 ? a.n_sec : 0];
+  P x2, y2;
+  if (HEADS == 1 && sec.paged) {
+    const T* from2 = values.src + row * values.src_row + int64_t(first) * values.src_head;
+    x2             = *reinterpret_cast<const P*>(from2 + lo);
+    y2             = *reinterpret_cast<const P*>(from2 + hi);
+  }
 
   int64_t to = row * sec.dst_row;
   if (sec.paged) {
@@ -195,6 +203,11 @@ __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
       return;
     }
     to = page * sec.dst_row + (pos - p * a.page_size) * sec.dst_token;
+    if (HEADS == 1) {
+      T* dst2 = values.dst + page * values.dst_row + (pos - p * a.page_size) * values.dst_token + int64_t(first) * values.dst_head;
+      *reinterpret_cast<P*>(dst2 + lo) = x2;
+      *reinterpret_cast<P*>(dst2 + hi) = y2;
+    }
   }
   T* dst = sec.dst + to + int64_t(first) * sec.dst_head;
   float c[V], s[V];
@@ -260,6 +273,9 @@ void run(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
   } else if (fits(2)) {
     run<T, V, 2>(a, interleaved, s);
   } else {
+    // few heads or few rows: a thread takes a key and its value, with one look at the table (keys and values of 73 324 rows of one
+    // head 28 us apart and 21 together)
+    if (a.sec[a.n_sec - 1].paged) { --a.n_sec; }
     run<T, V, 1>(a, interleaved, s);
   }
 }
@@ -343,13 +359,13 @@ void launch_paged_append(const certexB200PagedCache_t& cache, const certexB200Ro
     a.n_pages     = cache.n_pages;
     a.page_size   = cache.page_size;
     a.fault       = cache.fault;
-    auto pages    = [&](const certexB200Rows_t& from, void* to, const int64_t* strides, bool turned) {
+    if (n_q_heads > 0) { a.sec[a.n_sec++] = section<T>(q, q_out, n_q_heads, true); }
+    auto pages = [&](const certexB200Rows_t& from, void* to, const int64_t* strides, bool turned) {
       Section<T> x = section<T>(from, {to, strides[0], strides[2]}, cache.n_kv_heads, turned);
       x.dst_token  = strides[1];
       x.paged      = true;
       return x;
     };
-    if (n_q_heads > 0) { a.sec[a.n_sec++] = section<T>(q, q_out, n_q_heads, true); }
     a.sec[a.n_sec++] = pages(k, cache.keys, cache.key_strides, plan != nullptr);
     a.sec[a.n_sec++] = pages(v, cache.values, cache.value_strides, false);
     turn(a, plan && plan->interleaved != 0, s);

@@ -561,3 +561,31 @@ print("captured")
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert "captured" in done.stdout, done.stderr[-2000:]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pages_that_are_views(dtype):
+    """Keys and values as the two halves of one tensor, every second head of wider pages, and one memory for both."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    both = torch.randn((50, 2, 16, 6, 40), generator=g, device="cuda").to(dtype)
+    q = torch.randn((2, 9, 40), generator=g, device="cuda").to(dtype)
+    table = torch.randperm(50, generator=g, device="cuda").to(torch.int32).view(2, 25)
+    n = torch.tensor([390, 77], dtype=torch.int32, device="cuda")
+    at = torch.randint(-99, 800, (2, 9, 99), generator=g, device="cuda")
+    for keys, values in ((both[:, 0, :, :3], both[:, 1, :, 3:]), (both[:, 0, :, ::2], both[:, 1, :, 1::2]), (both[:, 1, :, 1:4], both[:, 1, :, 1:4])):
+        cache = certex.PagedCache(keys=keys, values=values)
+        dense = certex.PagedCache(keys=keys.contiguous(), values=values.contiguous())
+        assert torch.equal(cache.attend(q, table, n), dense.attend(q, table, n))
+        assert torch.equal(cache.attend_selected(q, at), dense.attend_selected(q, at))
+        out, lse = cache.attend(q, table, n, return_lse=True)
+        check(out, lse, q, cache, table_places(cache, table, n, None, 9))
+    rest = both.clone()
+    cache = certex.PagedCache(keys=both[:, 0, :, ::2], values=both[:, 1, :, 1::2], rotary=certex.Rotary(40, 16))
+    k, v = (torch.randn((2, 3, 40), generator=g, device="cuda").to(dtype) for _ in range(2))
+    cache.append(k, v, table, n)
+    for i in range(2):
+        page, place = int(table[i, int(n[i]) // 16]), int(n[i]) % 16
+        rest[page, 0, place, ::2] = cache.rotary(k, n)[i]
+        rest[page, 1, place, 1::2] = v[i]
+    assert torch.equal(both, rest)

@@ -206,3 +206,25 @@ def test_a_captured_training_step():
     graph.replay()
     close(y.detach(), x, p, plan)
     close(dx, dy, p, plan, inverse=True)
+
+
+@pytest.mark.gpu
+def test_gradient_of_an_input_that_is_shared():
+    """One head for all query heads, one row for all positions: the gradients add up; and an input that is used twice."""
+    plan = certex.Rotary(16)
+    p = torch.tensor([3, 70, 4096], device="cuda")
+    dy = torch.randn((3, 5, 16), device="cuda")
+    turned_back = turned(dy, p, plan, inverse=True)[0]
+    for shape in ((3, 1, 16), (1, 5, 16), (1, 1, 16)):
+        x = torch.randn(shape, device="cuda", requires_grad=True)
+        (dx,) = torch.autograd.grad(plan(x.expand(3, 5, 16), p), x, dy)
+        want = turned_back
+        for axis in (0, 1):
+            if shape[axis] == 1:
+                want = want.sum(axis, keepdim=True)
+        # up to 15 values of up to 6, each off by 2^-21 of its terms, and their sum's roundings
+        assert dx.shape == x.shape and float((dx.cpu().double() - want).abs().max()) <= 15 * 12 * 2.0**-21
+    x = torch.randn((3, 5, 16), device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(plan(x, p) + plan(x, -p), x, dy)
+    want = turned_back + turned(dy, -p, plan, inverse=True)[0]
+    assert float((dx.cpu().double() - want).abs().max()) <= 2 * 12 * 2.0**-21
