@@ -39,27 +39,44 @@ def _fail(message):
     raise ValueError(message)
 
 
-# The checks below stand in front of kernels of a few microseconds: messages are made only when one fails.
-def _check_rows(x, what, heads=None, dim=None):
-    """A CUDA tensor (n, heads, dim) whose last axis is dense, as the kernels read it."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        _fail(f"{what} must be a CUDA tensor")
-    shape = x.shape
-    if len(shape) != 3 or (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
-        _fail(f"{what} must have shape (n, {heads or 'heads'}, {dim or 'head_dim'}), not {tuple(shape)}")
+# The checks below stand in front of kernels of a few microseconds: one expression decides, and messages are made when it fails.
+_I32, _I64 = torch.int32, torch.int64
+
+
+def _check_rows(x, what, index, dtype, heads, dim):
+    """A tensor (n, heads, dim) on CUDA device `index` whose last axis is dense, as the kernels read it; `heads` and `dtype` may be
+    None: any number, any of the types."""
+    try:
+        shape = x.shape
+        fine = (x.get_device() == index and (x.dtype is dtype or (dtype is None and x.dtype in _KIND)) and shape[2] == dim
+                and (heads is None or shape[1] == heads) and len(shape) == 3)
+    except (AttributeError, IndexError):
+        fine = False
+    if not fine:
+        _explain_rows(x, what, index, dtype, heads, dim)
     if x.is_neg():
         x = x.resolve_neg()
     return x if x.stride(2) == 1 else x.contiguous()
 
 
-def _check_index(t, what, shape, device, wide=False):
-    """An index tensor of this shape: int32 (or int64 if `wide`), dense."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        _fail(f"{what} must be a tensor on {device}")
-    if t.dtype is not torch.int32 and not (wide and t.dtype is torch.int64):
+def _explain_rows(x, what, index, dtype, heads, dim):
+    _need(isinstance(x, torch.Tensor) and x.is_cuda, f"{what} must be a CUDA tensor")
+    _need(x.get_device() == index, f"{what} must be on cuda:{index}, not {x.device}")
+    _need(x.ndim == 3 and x.shape[2] == dim and heads in (None, x.shape[1]),
+          f"{what} must have shape (n, {'heads' if heads is None else heads}, {dim}), not {tuple(x.shape)}")
+    _fail(f"{what} must be {dtype or 'float32, float16 or bfloat16'}, not {x.dtype}")
+
+
+def _check_index(t, what, shape, index, wide=False):
+    """An index tensor of this shape on CUDA device `index`: int32 (or int64 if `wide`), dense."""
+    try:
+        fine = t.get_device() == index and (t.dtype is _I32 or (wide and t.dtype is _I64)) and t.shape == shape
+    except AttributeError:
+        fine = False
+    if not fine:
+        _need(isinstance(t, torch.Tensor) and t.get_device() == index, f"{what} must be a tensor on cuda:{index}")
+        _need(t.shape == shape, f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
         _fail(f"{what} must be {'int32 or int64' if wide else 'int32'}, not {t.dtype}")
-    if t.shape != shape:
-        _fail(f"{what} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     if t.is_neg():
         t = t.resolve_neg()
     return t if t.is_contiguous() else t.contiguous()
@@ -67,7 +84,7 @@ def _check_index(t, what, shape, device, wide=False):
 
 def _new_like(x):
     """A dense tensor of x's shape."""
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _packed(x):
@@ -165,7 +182,7 @@ class Rotary:
         turns = [_turns(f) for f in w]
         self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device=device)
         self.device = self._turns.device
-        self._index = self._turns.get_device()
+        self._index = self._turns.get_device() if self._turns.is_cuda else -2  # (no row is there)
         self._plan = _ROTARY.pack(self._turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.magnitude)
 
     def __call__(self, x, positions, inverse=False, out=None):
@@ -173,12 +190,8 @@ class Rotary:
         negative; inverse=True turns back. Differentiable in x (as for every function of torch, a backward pass that is captured
         in a CUDA graph wants leaves of which no eager graph is alive). out: where to write, x itself allowed; without a
         gradient."""
-        x = _check_rows(x, "x", dim=self.head_dim)
-        if x.dtype not in _KIND:
-            _fail(f"rows are float32, float16 or bfloat16, not {x.dtype}")
-        if x.device != self.device:
-            _fail(f"this rotation lives on {self.device}, the rows on {x.device}")
-        positions = _check_index(positions, "positions", (x.shape[0],), x.device, wide=True)
+        x = _check_rows(x, "x", self._index, None, None, self.head_dim)
+        positions = _check_index(positions, "positions", x.shape[:1], self._index, True)
         if x.requires_grad and torch.is_grad_enabled():
             _need(out is None, "out takes no gradient: call without it, or under torch.no_grad()")
             return _Turn.apply(x, positions, self, bool(inverse))
@@ -295,12 +308,6 @@ class PagedCache:
             self._fault.zero_()
         return bad
 
-    def _rows(self, x, what, heads=None):
-        x = _check_rows(x, what, heads, self.head_dim)
-        if x.dtype is not self.dtype or x.device != self.device:
-            _fail(f"{what} must be {self.dtype} on {self.device} like the cache, not {x.dtype} on {x.device}")
-        return x
-
     def _unmoved(self):
         """The cache as the library takes it, whose memory must still be where it was."""
         if self._keys.data_ptr() != self._at[0] or self._values.data_ptr() != self._at[1]:
@@ -308,15 +315,18 @@ class PagedCache:
         return self._args
 
     def _table(self, page_table, row_to_batch, n):
-        if (not isinstance(page_table, torch.Tensor) or page_table.device != self.device or page_table.dtype is not torch.int32
-                or page_table.ndim != 2):
+        try:
+            sequences, pages = page_table.shape
+            fine = page_table.get_device() == self._index and page_table.dtype is _I32
+        except (AttributeError, ValueError):
+            fine = False
+        if not fine:
             _fail(f"the page table must be an int32 tensor (sequences, pages) on {self.device}")
         if page_table.stride(1) != 1:
             page_table = page_table.contiguous()
-        sequences, pages = page_table.shape
         rows = 0
         if row_to_batch is not None:
-            row_to_batch = _check_index(row_to_batch, "row_to_batch", (n,), self.device)
+            row_to_batch = _check_index(row_to_batch, "row_to_batch", (n,), self._index)
             rows = row_to_batch.data_ptr()
         elif sequences != n:
             _fail(f"{n} rows and a table of {sequences} sequences: give row_to_batch")
@@ -333,16 +343,17 @@ class PagedCache:
         if _current_device() != self._index:  # kernels, streams and handles are the current device's
             with torch.cuda.device(self._index):
                 return self.append(k, v, page_table, positions, row_to_batch, q)
-        k, v = self._rows(k, "k", self.n_kv_heads), self._rows(v, "v", self.n_kv_heads)
+        k = _check_rows(k, "k", self._index, self.dtype, self.n_kv_heads, self.head_dim)
+        v = _check_rows(v, "v", self._index, self.dtype, self.n_kv_heads, self.head_dim)
         n = k.shape[0]
         if v.shape[0] != n:
             _fail(f"{n} keys and {v.shape[0]} values")
-        positions = _check_index(positions, "positions", (n,), self.device, wide=True)
+        positions = _check_index(positions, "positions", (n,), self._index, True)
         table, alive = self._table(page_table, row_to_batch, n)
         heads, q_in, q_to, turned, rotary = 0, None, None, None, self._rotary
         if q is not None:
             _need(rotary is not None, "queries come along to be turned, but this cache has no rotation")
-            q = self._rows(q, "q")
+            q = _check_rows(q, "q", self._index, self.dtype, None, self.head_dim)
             if q.shape[0] != n:
                 _fail(f"{n} keys and {q.shape[0]} queries")
             turned = _new_like(q)
@@ -359,7 +370,7 @@ class PagedCache:
     def _prepared(self, q, scale, return_lse, out):
         """What both attentions do with their queries: checks, outputs."""
         _no_gradient(q)
-        q = self._rows(q, "q")
+        q = _check_rows(q, "q", self._index, self.dtype, None, self.head_dim)
         n, heads, dim = q.shape
         if heads < 1 or heads % self.n_kv_heads:
             _fail(f"{heads} query heads are no multiple of {self.n_kv_heads} KV heads")
@@ -408,7 +419,7 @@ class PagedCache:
             window = 0
         elif window < 1:
             _fail("window must be positive")
-        lengths = _check_index(lengths, "lengths", (n,), self.device)
+        lengths = _check_index(lengths, "lengths", (n,), self._index)
         table, alive = self._table(page_table, row_to_batch, n)
         if n:
             w, at, size = self._workspace(n, heads, 0, page_table.shape[1] * self.page_size, window)
@@ -431,7 +442,7 @@ class PagedCache:
         if (not isinstance(selected, torch.Tensor) or selected.ndim != 3 or selected.shape[0] != n
                 or selected.shape[1] not in (heads, self.n_kv_heads, 1)):
             _fail(f"selected must have shape ({n}, {heads}, k), ({n}, {self.n_kv_heads}, k), ({n}, 1, k) or ({n}, k)")
-        selected = _check_index(selected, "selected", selected.shape, self.device, wide=True)
+        selected = _check_index(selected, "selected", selected.shape, self._index, True)
         lists, k = selected.shape[1:]
         if n:
             w, at, size = self._workspace(n, heads, lists, k, 0)
