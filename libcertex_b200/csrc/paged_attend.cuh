@@ -351,6 +351,14 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int32_t share)
   return x;
 }
 
+/// The blocks are there before the kernel in front of them has ended (2 us less between calls in a stream) and wait for that; the
+/// joining kernel, if there is one, is let in the same way.
+__device__ __forceinline__ void begin(const AttendParams& p)
+{
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!p.cluster) { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+}
+
 /// Calls body(segment) for this block's share of the work. A block of W warps calls it as a whole.
 template <typename T, int W, typename F>
 __device__ __forceinline__ void for_segments(const AttendParams& p, F&& body)
@@ -732,7 +740,7 @@ __global__ void __launch_bounds__(W * 32, (NT == 1 ? 12 : 8) / W) attend_direct_
   constexpr int R = D <= kDoubleDim ? 2 : 1, kKeys = 16 * R;  // keys of a tile
   extern __shared__ __align__(16) float sums[];  // [warps][8 NT][D + 4]
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  begin(p);
 
   for_segments<T, W>(p, [&](const Segment& g) {
     const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(T) + t4 * 16;
@@ -991,7 +999,7 @@ __global__ void __launch_bounds__(W * 32, 4 / W) attend_ring_kernel(const Attend
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g8 = lane / 4, t4 = lane % 4;
   unsigned char* ring = smem + warp * Tile::kWarp;
   const uint32_t ring_at = smem_of(ring);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  begin(p);
   if (p.dim < D) {
     // the columns behind the last coordinate are multiplied by zeros of the queries: they must hold numbers
     for (int i = lane * 16; i < Tile::kWarp; i += 32 * 16) { *reinterpret_cast<uint4*>(ring + i) = uint4{0, 0, 0, 0}; }
@@ -1188,7 +1196,7 @@ __global__ void __launch_bounds__(W * 32, 8 / W) attend_float_kernel(const Atten
   float* weights = q_s + Q * D + warp * Tile::kWeights;               // [Q][keys][2]
   float* factors = weights + 2 * Q * kKeys;                           // [Q]
   float* sums    = q_s + Q * D + W * Tile::kWeights;             // [warps][Q][D + 4]
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  begin(p);
 
   for_segments<float, W>(p, [&](const Segment& g) {
     const char* keys   = static_cast<const char*>(p.keys) + g.kv * p.k_head * sizeof(float) + t4 * 16;
@@ -1637,21 +1645,19 @@ void launch(Kernel kernel, int warps, int smem, const AttendParams& p, int64_t b
 {
   // (40 KB: what needs no opt-in, with room for static shared memory)
   if (smem > 40 * 1024) { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
-  if (p.cluster <= 1) {
-    kernel<<<static_cast<unsigned>(blocks), warps * 32, smem, s>>>(p);
-    return;
-  }
   cudaLaunchConfig_t c{};
   c.gridDim          = dim3(static_cast<unsigned>(blocks));
   c.blockDim         = dim3(warps * 32);
   c.dynamicSmemBytes = smem;
   c.stream           = s;
-  cudaLaunchAttribute together{};
-  together.id               = cudaLaunchAttributeClusterDimension;
-  together.val.clusterDim.x = static_cast<unsigned>(p.cluster);
-  together.val.clusterDim.y = together.val.clusterDim.z = 1;
-  c.attrs    = &together;
-  c.numAttrs = 1;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id               = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  c.attrs    = at;
+  c.numAttrs = p.cluster <= 1 ? 1 : 2;
   cudaLaunchKernelEx(&c, kernel, p);
 }
 

@@ -142,6 +142,7 @@ template <typename T, int V, bool INTERLEAVED, int HEADS>
 __global__ void __launch_bounds__(256, 4) turn_rows_kernel(const TurnArgs<T> a)
 {
   constexpr bool kExact = sizeof(T) == 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the blocks are there before the kernel in front of them has ended
   const int units       = a.dim / (2 * V);  // of a head
   int chunks            = 0;
   for (int i = 0; i < a.n_sec; ++i) { chunks += a.sec[i].chunks; }
@@ -245,11 +246,16 @@ void run(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
   const int64_t items = a.n_rows * chunks * (a.dim / (2 * V));
   const int threads   = 256;
   const auto grid     = static_cast<unsigned>((items + threads - 1) / threads);
-  if (interleaved) {
-    turn_rows_kernel<T, V, true, HEADS><<<grid, threads, 0, s>>>(a);
-  } else {
-    turn_rows_kernel<T, V, false, HEADS><<<grid, threads, 0, s>>>(a);
-  }
+  cudaLaunchConfig_t c{};
+  c.gridDim  = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.stream   = s;
+  cudaLaunchAttribute early{};
+  early.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs                                          = &early;
+  c.numAttrs                                       = 1;
+  cudaLaunchKernelEx(&c, interleaved ? turn_rows_kernel<T, V, true, HEADS> : turn_rows_kernel<T, V, false, HEADS>, a);
 }
 
 template <typename T, int V>

@@ -127,3 +127,79 @@ def test_the_tables_width_changes_nothing_that_is_seen():
         out, lse = cache.attend(q, table[:, :width], lengths, return_lse=True)
         check(out, lse, q, keys, values, table_places(table, lengths, 16, 8))
     assert not cache.faulted()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_calls_see_what_was_enqueued_right_before_them(dtype):
+    """Kernels that are let in before the one in front has ended: fills, copies from and to the host, other streams' work and the library's
+    own kernels right before and behind them, eagerly and in a graph; whatever reads early would read the old."""
+    rotary = certex.Rotary(64)
+    pages = torch.zeros((700, 16, 4, 64), device="cuda").to(dtype)
+    cache = certex.PagedCache(keys=pages, values=torch.zeros_like(pages), rotary=rotary)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    table = torch.arange(700, device="cuda", dtype=torch.int32).view(2, 350)
+    source = [torch.randn((2, 4, 64), generator=g, device="cuda").to(dtype) for _ in range(4)]
+    big = torch.empty((1 << 26,), device="cuda")
+    k, q, lengths, p = (torch.zeros_like(source[0]), torch.zeros((2, 8, 64), device="cuda").to(dtype), torch.zeros(2, dtype=torch.int32, device="cuda"),
+                        torch.zeros(2, dtype=torch.int32, device="cuda"))
+    side = torch.cuda.Stream()
+
+    def step(i, n):
+        big.fill_(float(i))                       # a long kernel in front
+        k.copy_(source[i])
+        q.copy_(torch.cat([source[i], source[(i + 1) % 4]], 1))
+        p.fill_(n - 1)
+        r = cache.append(k, k, table, p, q=q)
+        k.zero_()
+        q.zero_()
+        lengths.fill_(n)
+        a, lse = cache.attend(r, table, lengths, return_lse=True)   # split: the table is wide
+        lengths.fill_(1)
+        b = cache.attend(r, table[:, :4], lengths)                   # a cluster
+        lengths.fill_(0)
+        at = (table[:, :1, None] * 16 + n - 1).expand(2, 8, 3)
+        at = torch.where(p[:, None, None] >= 0, table[:, (n - 1) // 16, None, None] * 16 + (n - 1) % 16, at)
+        c = cache.attend_selected(r, at.contiguous())
+        p.fill_(0)
+        t = rotary(r, p, inverse=True)
+        r.zero_()
+        return a, lse, b, c, t
+
+    def expected(i, n):
+        kk, qq = source[i], torch.cat([source[i], source[(i + 1) % 4]], 1)
+        pos = torch.full((2,), n - 1, dtype=torch.int32, device="cuda")
+        return rotary(qq, pos), kk.repeat_interleave(2, 1)
+
+    def verify(i, n, got):
+        turned, values = expected(i, n)
+        a, lse, b, c, t = got
+        assert torch.equal(t, turned)  # position 0 turns nothing
+        # one key, named three times, with equal weights: the sum of three values, 1 / 3 and their product are rounded, 3 * 2^-24, and the result
+        off = (c.double() - values.double()).abs() - values.double().abs() * (4 * 2.0**-24 + 1.01 * HALF_STEP[dtype])
+        assert float(off.max()) <= 0, float(off.max())
+        assert bool(torch.isfinite(a.float()).all()) and bool(torch.isfinite(lse).all())
+
+    for n in (1, 2, 17, 900):
+        for i in range(4):
+            got = step(i, n)
+            torch.cuda.synchronize()
+            verify(i, n, got)
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.current_stream())
+        got = step(1, 33)
+    side.synchronize()
+    verify(1, 33, got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(2, 40)
+    for _ in range(3):
+        for x in got:
+            x.fill_(9)
+        graph.replay()
+        torch.cuda.synchronize()
+        verify(2, 40, got)
+    # the whole attention over what the steps appended, against 64 bits
+    n = torch.tensor([900, 900], dtype=torch.int32, device="cuda")
+    x = torch.randn((2, 8, 64), generator=g, device="cuda").to(dtype)
+    out, lse = cache.attend(x, table, n, return_lse=True)
+    check(out, lse, x, cache.keys.view(-1, 4, 64), cache.values.view(-1, 4, 64), table_places(table, n, 16, 8))
