@@ -181,9 +181,17 @@ class Rotary:
         # what one position adds to an angle, as a fraction of a turn in units of 2**-64
         turns = [_turns(f) for f in w]
         self._turns = torch.tensor([t - 2**64 if t >= 2**63 else t for t in turns], dtype=torch.int64, device=device)
+        self._bind()
+
+    def _bind(self):
+        """What the library is told, with addresses in it."""
         self.device = self._turns.device
         self._index = self._turns.get_device() if self._turns.is_cuda else -2  # (no row is there)
         self._plan = _ROTARY.pack(self._turns.data_ptr(), self.rotary_dim, int(self.interleaved), self.magnitude)
+
+    def __setstate__(self, state):  # a copy, or another process: its tensors lie elsewhere
+        self.__dict__.update(state)
+        self._bind()
 
     def __call__(self, x, positions, inverse=False, out=None):
         """x (n, heads, head_dim) float32, float16 or bfloat16, its rows turned by positions (n,) int32 or int64, which may be
@@ -274,17 +282,28 @@ class PagedCache:
         _need(self.head_dim % 8 == 0 and self.head_dim <= _MOST_DIM,
               f"head_dim must be a multiple of 8 and at most {_MOST_DIM}, not {self.head_dim}")
         self.rotary = rotary
+        self._fault = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._bind()
+
+    def _bind(self):
+        """What the library is told, with addresses in it."""
+        keys, values = self._keys, self._values
+        token, head = (1, 2) if self._layout == "NHD" else (2, 1)
         size = keys.element_size()
         for t in (keys, values):
-            _need(t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s * size % 16 == 0 for s in t.stride()[:3]),
-                  "keys and values need a dense last axis and strides of whole 16 bytes")
+            _need(t.is_cuda and t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s * size % 16 == 0 for s in t.stride()[:3]),
+                  "keys and values need a dense last axis and strides of whole 16 bytes, on a CUDA device")
         self._index, self._at = keys.get_device(), (keys.data_ptr(), values.data_ptr())
         self._pages = (keys, values)
         self._needs = {}  # sizes of a call -> bytes of its workspace
-        self._fault = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._args = _CACHE.pack(*self._at,
                                  *(t.stride(i) for t in (keys, values) for i in (0, token, head)), self.n_pages,
                                  self.page_size, self.n_kv_heads, self.head_dim, _KIND[self.dtype], self._fault.data_ptr())
+
+    def __setstate__(self, state):  # a copy, or another process: its tensors lie elsewhere
+        self.__dict__.update(state)
+        self.device = self._keys.device
+        self._bind()
 
     keys = property(lambda self: self._keys, doc="The pages of keys.")
     values = property(lambda self: self._values, doc="The pages of values.")

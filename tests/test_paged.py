@@ -1,8 +1,11 @@
 """The paged cache: append against plain indexing, both attentions against the definition in 64 bits on the CPU, at the lengths,
 pages, heads, types and masks where they can go wrong; refusals; a decoding loop as it is used, with the exact selection."""
 
+import copy
 import ctypes
+import io
 import math
+import pickle
 import struct
 
 import pytest
@@ -589,3 +592,24 @@ def test_pages_that_are_views(dtype):
         rest[page, 0, place, ::2] = cache.rotary(k, n)[i]
         rest[page, 1, place, 1::2] = v[i]
     assert torch.equal(both, rest)
+
+
+@pytest.mark.gpu
+def test_copies_of_a_cache_have_their_own_memory():
+    cache, table, _ = make(torch.bfloat16, 2, 40, 8, 2, 16)
+    cache.rotary = certex.Rotary(16)
+    q = torch.randn((2, 4, 16), device="cuda").bfloat16()
+    lengths = torch.tensor([40, 3], device="cuda", dtype=torch.int32)
+    kv = torch.randn((2, 2, 2, 16), device="cuda").bfloat16()
+    want = cache.attend(q, table, lengths)
+    for twin in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert twin.keys.data_ptr() != cache.keys.data_ptr() and twin.rotary is not cache.rotary
+        assert torch.equal(twin.attend(q, table, lengths), want)
+        twin.append(kv[0], kv[1], table, torch.tensor([1, 99], device="cuda"))  # the second lies behind its table
+        assert twin.faulted() and not cache.faulted()
+        assert torch.equal(cache.attend(q, table, lengths), want) and not torch.equal(twin.attend(q, table, lengths), want)
+    stored = io.BytesIO()
+    torch.save(cache, stored)
+    stored.seek(0)
+    with pytest.raises(ValueError, match="CUDA"):
+        torch.load(stored, map_location="cpu", weights_only=False)

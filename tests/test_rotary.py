@@ -1,7 +1,10 @@
 """Rotation by position against the formula in 64 bits: types, both orders of pairs, part of a head, odd sizes and strides,
 far and negative positions, scaled frequencies, in place; its gradient against the formula's and against differences."""
 
+import copy
 import math
+import pickle
+import struct
 
 import pytest
 import torch
@@ -228,3 +231,12 @@ def test_gradient_of_an_input_that_is_shared():
     (dx,) = torch.autograd.grad(plan(x, p) + plan(x, -p), x, dy)
     want = turned_back + turned(dy, -p, plan, inverse=True)[0]
     assert float((dx.cpu().double() - want).abs().max()) <= 2 * 12 * 2.0**-21
+
+
+def test_copies_of_a_plan_have_their_own_memory():
+    plan = certex.Rotary(16, 8, interleaved=True, magnitude=0.5, device="cpu")
+    for twin in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan)), copy.copy(plan)):
+        at, r, interleaved, magnitude = struct.unpack("3qd", twin._plan)
+        assert at == twin._turns.data_ptr() and (r, interleaved, magnitude) == (8, 1, 0.5)
+        assert torch.equal(twin._turns, plan._turns) and twin.device == plan.device and twin._index == plan._index
+    assert copy.deepcopy(plan)._turns.data_ptr() != plan._turns.data_ptr()
