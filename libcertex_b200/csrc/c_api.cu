@@ -642,14 +642,19 @@ void check_table(const certexB200PageTable_t* t)
                  "certex: null page table");
 }
 
+void check_sizes(const certexB200PagedCache_t& c, int64_t n_rows, int64_t n_heads)
+{
+  CERTEX_EXPECTS(n_heads >= 1 && n_heads <= 65535 && n_heads % c.n_kv_heads == 0,
+                 "certex: the query heads must be a multiple of the KV heads");
+  CERTEX_EXPECTS(n_rows >= 0 && n_rows <= ((int64_t(1) << 27) - 1) / n_heads, "certex: too many rows");
+}
+
 /// What both attentions share: heads, outputs, the workspace.
 void attend_impl(cuvsResources_t res, AttendArgs a, const certexB200PagedCache_t* cache, const certexB200Rows_t* q,
                  const certexB200Rows_t* out, size_t workspace_bytes)
 {
   a.cache = checked_cache(cache);
-  CERTEX_EXPECTS(a.n_heads >= 1 && a.n_heads <= 65535 && a.n_heads % a.cache.n_kv_heads == 0,
-                 "certex: the query heads must be a multiple of the KV heads");
-  CERTEX_EXPECTS(a.n_rows >= 0 && a.n_rows * a.n_heads < (int64_t(1) << 27), "certex: too many rows");
+  check_sizes(a.cache, a.n_rows, a.n_heads);
   CERTEX_EXPECTS(std::isfinite(a.scale), "certex: the scale must be finite");
   if (a.n_rows == 0) { return; }
   check_rows(q, "queries");
@@ -714,11 +719,12 @@ cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCach
 cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedCache_t* cache, int64_t n_rows, int64_t n_heads,
                                      int64_t n_lists, int64_t k, int64_t window, size_t* bytes)
 {
-  return translate([=] {
+  return translate([=]() mutable {
     CERTEX_EXPECTS(bytes != nullptr && n_rows >= 0 && n_lists >= 0 && k >= 0 && window >= 0, "certex: null argument");
     AttendArgs a{};
     a.cache = checked_cache(cache);
-    CERTEX_EXPECTS(n_heads >= 1 && n_heads % a.cache.n_kv_heads == 0, "certex: the query heads must be a multiple of the KV heads");
+    check_sizes(a.cache, n_rows, n_heads);
+    k          = std::min(k, kMostTokens);
     a.n_rows                   = n_rows;
     a.n_heads                  = n_heads;
     a.n_lists                  = n_lists;

@@ -20,6 +20,12 @@ constexpr int64_t kClusterTokens = 256;
 /// with two warps and 24 with four.
 constexpr int64_t kManyShares = 128;
 
+/// Tokens that the table can hold of a sequence, as far as a row may see them.
+int64_t table_tokens(const AttendArgs& a)
+{
+  return std::min(std::min(a.table.pages_per_sequence, kMostTokens) * a.cache.page_size, kMostTokens);
+}
+
 struct Plan {
   int32_t per_unit, subs, units, warps;
   int cluster;
@@ -39,7 +45,7 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   n.per_unit       = alone ? 1 : std::min(group, half ? 16 : 8);
   n.subs           = (group + n.per_unit - 1) / n.per_unit;
   n.units          = static_cast<int32_t>(a.cache.n_kv_heads) * n.subs;
-  int64_t most     = a.n_lists > 0 ? a.k : a.table.pages_per_sequence * a.cache.page_size;
+  int64_t most     = a.n_lists > 0 ? a.k : table_tokens(a);
   if (a.n_lists == 0 && a.window > 0) { most = std::min(most, a.window); }
   const int64_t units = a.n_rows * n.units;
   const int64_t warps    = int64_t(sm_count) * (half ? (dim > 128 ? 4 : n.per_unit <= 8 ? 12 : 8) : 8);  // resident ones
@@ -125,7 +131,7 @@ void launch_paged_attend(const AttendArgs& a, int sm_count, cudaStream_t s)
   p.pages           = a.table.pages;
   p.page_row        = a.table.row_stride;
   p.n_sequences     = a.table.n_sequences;
-  p.most            = static_cast<int32_t>(std::min(a.table.pages_per_sequence * a.cache.page_size, kMostTokens));
+  p.most            = static_cast<int32_t>(table_tokens(a));
   p.row_to_sequence = a.table.row_to_sequence;
   p.lengths         = a.lengths;
   p.window          = static_cast<int32_t>(std::min(a.window, kMostTokens));

@@ -145,6 +145,24 @@ def test_the_library_refuses_what_it_cannot_read(built_library):
     assert L.certexB200PagedWorkspace(None, _cache_args(dim=9), 1, 1, 0, 1, 0, ctypes.byref(need)) == 0
 
 
+def test_sizes_beyond_all_bounds_are_refused(built_library):
+    """Products of sizes that would wrap, and those that the other calls refuse, are errors before the device is looked at."""
+    L, table, rows, need = built_library, paged._TABLE.pack(64, 1, 1, 1, 0), paged._ROWS.pack(64, 8, 8), ctypes.c_size_t()
+
+    def workspace(n=1, heads=1, lists=0, k=1):
+        return L.certexB200PagedWorkspace(None, _cache_args(), n, heads, lists, k, 0, ctypes.byref(need))
+
+    def attend(n, heads):
+        return L.certexB200PagedAttend(None, _cache_args(), table, 64, 0, rows, rows, n, heads, 1.0, None, None, 0)
+
+    for call, text in (
+        (lambda: workspace(n=2**27), b"too many rows"), (lambda: workspace(n=2**40), b"too many rows"), (lambda: workspace(n=2**62, heads=4), b"too many rows"),
+        (lambda: workspace(heads=65536), b"multiple"), (lambda: workspace(n=-1), b"null argument"), (lambda: attend(2**62, 4), b"too many rows"),
+        (lambda: attend(2**26, 2), b"too many rows"), (lambda: workspace(n=2**27 - 1, k=2**62), b"null resources"),
+    ):
+        assert call() == 0 and text in L.cuvsGetLastErrorText(), (text, L.cuvsGetLastErrorText())
+
+
 def test_packed_structures_have_the_headers_sizes(built_library, tmp_path):
     import os
     import shutil
