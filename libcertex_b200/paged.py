@@ -148,8 +148,8 @@ class _Turn(torch.autograd.Function):
 class Rotary:
     """Turns queries and keys by their positions: pair i of the first `rotary_dim` coordinates of a head (default: all) by
     the angle position * w_i, w_i = base ** (-2 i / rotary_dim). Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with
-    interleaved=True. Angles are exact to 2**-32 of a turn at every position up to 2**31, so no table of sines limits the
-    length.
+    interleaved=True. Angles are reduced to one turn exactly and off by at most 2**-26 of it at every position up to 2**31, so no
+    table of sines limits the length.
 
     scaling stretches the frequencies for sequences longer than the `original_length` a model was trained on, by `factor`:
       "linear"      w_i / factor
@@ -321,7 +321,8 @@ class PagedCache:
         self._rotary = rotary
 
     def faulted(self):
-        """Whether an index of a call since the last time was out of range (and was left out). Waits for the device."""
+        """Whether an index of a call since the last time was out of range (and was left out). Waits for the current stream, and
+        speaks for calls that were enqueued there, or that it waited for."""
         bad = bool(self._fault.item())
         if bad:
             self._fault.zero_()
@@ -379,6 +380,8 @@ class PagedCache:
             heads = q.shape[1]
             if heads:
                 q_in, q_to = _packed(q), _packed(turned)
+        if self._at[0] == self._at[1]:
+            _fail("the keys and values of this cache are the same memory, where both cannot be stored")
         if n:
             L.check(L.lib().certexB200PagedAppend(L.resources(self._index), self._unmoved(), rotary._plan if rotary else None, table,
                                                   _packed(k), _packed(v), q_in, q_to, n, heads, positions.data_ptr(),
@@ -427,7 +430,8 @@ class PagedCache:
         int32, or over the last `window` of those; heads is a multiple of n_kv_heads, query head h reads KV head
         h // (heads / n_kv_heads). scale defaults to head_dim ** -0.5. Returns (n, heads, head_dim), and with return_lse the
         float32 logarithm of the sum of exponentials (n, heads). A row that sees nothing gets zeros and -inf. Several rows of
-        one sequence (drafted tokens) name it in row_to_batch and have their own lengths."""
+        one sequence (drafted tokens) name it in row_to_batch and have their own lengths. out, if given, is written: memory that
+        no other argument and no page has."""
         if _current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.attend(q, page_table, lengths, row_to_batch, scale, window, return_lse, out)

@@ -612,7 +612,7 @@ def test_pages_that_are_views(dtype):
     assert torch.equal(both, rest)
 
 
-@pytest.mark.gpu
+@gpu
 def test_copies_of_a_cache_have_their_own_memory():
     cache, table, _ = make(torch.bfloat16, 2, 40, 8, 2, 16)
     cache.rotary = certex.Rotary(16)
@@ -631,3 +631,52 @@ def test_copies_of_a_cache_have_their_own_memory():
     stored.seek(0)
     with pytest.raises(ValueError, match="CUDA"):
         torch.load(stored, map_location="cpu", weights_only=False)
+
+
+@gpu
+def test_keys_and_values_of_one_memory_are_read_but_not_stored():
+    both = torch.randn((3, 4, 1, 8), device="cuda")
+    cache = certex.PagedCache(keys=both, values=both)
+    table, n = torch.tensor([[2, 0]], device="cuda", dtype=torch.int32), torch.tensor([1], device="cuda", dtype=torch.int32)
+    row = torch.ones((1, 1, 8), device="cuda")
+    assert torch.equal(cache.attend(row, table, n), both[2, :1])  # one key: its value, weight 1
+    with pytest.raises(ValueError, match="same memory"):
+        cache.append(row, row, table, n)
+
+
+@gpu
+def test_captured_calls_wait_for_all_that_is_in_front_of_them():
+    """A call whose place in a graph is behind a kernel of the library, a copy and another stream's work at once sees them all."""
+    cache, table, _ = make(torch.float32, 2, 2000, 16, 1, 8)
+    q, lengths, host = torch.randn((2, 1, 8), device="cuda"), torch.zeros(2, device="cuda", dtype=torch.int32), torch.zeros(2, dtype=torch.int32).pin_memory()
+    side, new = torch.cuda.Stream(), torch.zeros((2, 1, 8), device="cuda")
+    source = torch.zeros((2, 1, 8), device="cuda")
+    rotary = certex.Rotary(8)
+
+    def step():
+        now = torch.cuda.current_stream()
+        side.wait_stream(now)
+        lengths.copy_(host, non_blocking=True)
+        turned = rotary(q, lengths)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000)
+            new.copy_(source)
+        now.wait_stream(side)
+        cache.append(new, new, table, lengths - 1)
+        return turned, cache.attend(new, table, lengths)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turned, out = step()
+    for turn, n in enumerate((1, 2000, 3, 700, 1999)):
+        source.normal_()
+        host.fill_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = turned.clone(), out.clone()
+        want = rotary(q, torch.full((2,), n, device="cuda")), cache.attend(source, table, torch.full((2,), n, device="cuda", dtype=torch.int32))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), turn
+        for i in range(2):
+            place = table[i, (n - 1) // 16].item(), (n - 1) % 16
+            assert torch.equal(cache.values[place], source[i])
