@@ -21,6 +21,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib as L
 from .index import _need
@@ -113,13 +114,18 @@ def _check_out(out, x, in_place):
     return out
 
 
+def _has_tangent(x):
+    """Whether forward-mode differentiation goes through x (asked only inside of it)."""
+    return _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(x).tangent is not None
+
+
 # Tells autograd that the library wrote into tensors of the caller's: a graph that saved one of them before finds out.
 _written = torch.autograd.graph.increment_version
 
 
 def _no_gradient(*tensors):
     for t in tensors:
-        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+        if isinstance(t, torch.Tensor) and (t.requires_grad and torch.is_grad_enabled() or _has_tangent(t)):
             _fail("no gradient flows through a paged cache: call it under torch.no_grad()")
 
 
@@ -136,6 +142,7 @@ class _Turn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, rotary, inverse):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
         return rotary._turn(x, positions, inverse, None)
 
@@ -143,6 +150,11 @@ class _Turn(torch.autograd.Function):
     def backward(ctx, dy):
         (positions,) = ctx.saved_tensors
         return ctx.rotary(dy, positions, inverse=not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        (positions,) = ctx.saved_tensors
+        return ctx.rotary(dx, positions, inverse=ctx.inverse)
 
 
 class Rotary:
@@ -200,7 +212,7 @@ class Rotary:
         gradient."""
         x = _check_rows(x, "x", self._index, None, None, self.head_dim)
         positions = _check_index(positions, "positions", x.shape[:1], self._index, True)
-        if x.requires_grad and torch.is_grad_enabled():
+        if x.requires_grad and torch.is_grad_enabled() or _has_tangent(x):
             _need(out is None, "out takes no gradient: call without it, or under torch.no_grad()")
             return _Turn.apply(x, positions, self, bool(inverse))
         return self._turn(x, positions, inverse, out)

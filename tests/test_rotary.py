@@ -240,3 +240,21 @@ def test_copies_of_a_plan_have_their_own_memory():
         assert at == twin._turns.data_ptr() and (r, interleaved, magnitude) == (8, 1, 0.5)
         assert torch.equal(twin._turns, plan._turns) and twin.device == plan.device and twin._index == plan._index
     assert copy.deepcopy(plan)._turns.data_ptr() != plan._turns.data_ptr()
+
+
+@pytest.mark.gpu
+def test_forward_mode():
+    """The rotation is linear: its derivative along dx is the rotation of dx, by the same kernel."""
+    plan = certex.Rotary(16, 8)
+    x, dx = torch.randn((2, 5, 3, 16), device="cuda")
+    positions = torch.arange(5, device="cuda")
+    for inverse in (False, True):
+        with torch.autograd.forward_ad.dual_level():
+            y, dy = torch.autograd.forward_ad.unpack_dual(plan(torch.autograd.forward_ad.make_dual(x, dx), positions, inverse=inverse))
+            assert torch.equal(y, plan(x, positions, inverse=inverse)) and torch.equal(dy, plan(dx, positions, inverse=inverse))
+            cache = certex.PagedCache(1, 8, 3, 16, dtype=torch.float32)
+            table = torch.zeros((1, 1), device="cuda", dtype=torch.int32)
+            with pytest.raises(ValueError, match="gradient"):
+                cache.append(torch.autograd.forward_ad.make_dual(x, dx), x, table, positions, torch.zeros_like(positions, dtype=torch.int32))
+            with pytest.raises(ValueError, match="gradient"):
+                plan(torch.autograd.forward_ad.make_dual(x, dx), positions, out=torch.empty_like(x))
