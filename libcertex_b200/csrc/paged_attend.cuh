@@ -707,17 +707,17 @@ __device__ __forceinline__ float sum_over_keys(float v)
 // four products. What is left is to pair the values of neighbouring keys, one byte permutation per register.
 // Against copies into shared memory and ldmatrix this takes 380 instructions per tile of 8 KB instead of 470.
 
-/// N * 4 bytes that are read once.
+/// N * 4 bytes that are read once (not by .nc: a block is there while the kernel in front still writes them).
 template <int N>
 __device__ __forceinline__ void read_once(uint32_t (&r)[N], const char* at)
 {
   static_assert(N == 1 || N == 2 || N == 4, "");
   if constexpr (N == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(at));
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(at));
   } else if constexpr (N == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(at));
+    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(at));
   } else {
-    asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];" : "=r"(r[0]) : "l"(at));
+    asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(r[0]) : "l"(at));
   }
 }
 
