@@ -386,8 +386,8 @@ CERTEX_B200_EXPORT cuvsError_t certexB200Rotate(cuvsResources_t res, const certe
 
 /** Row i of k and v (n_kv_heads heads) goes to position positions[i] of its sequence; a negative position is a row without a
  *  token. With rotary (may be NULL) keys are turned by their positions on the way, and so are the n_q_heads heads of q, which
- *  go to q_out (q and q_out may be NULL, with n_q_heads = 0). Rows of one call have different places, and keys and values of the
- *  cache are not the same memory (which attention allows). */
+ *  go to q_out (q and q_out may be NULL, with n_q_heads = 0). Rows of one call have different places; where the
+ *  cache's keys and values are the same memory, k and v are equal and rotary is NULL. */
 CERTEX_B200_EXPORT cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCache_t* cache,
                                                      const certexB200Rotary_t* rotary, const certexB200PageTable_t* table,
                                                      const certexB200Rows_t* k, const certexB200Rows_t* v,

@@ -368,8 +368,8 @@ class PagedCache:
     def append(self, k, v, page_table, positions, row_to_batch=None, q=None):
         """Stores k, v (n, n_kv_heads, head_dim) at positions (n,) int32 or int64 of their sequences; a negative position is
         padding. With a rotation the keys are turned by their positions first, and q (n, heads, head_dim), if given, is
-        returned turned (rows of padding too, by the position as it stands). No two rows have the same place, and k and v do not
-        lie in places that the call writes. The keys as they are stored are what a selector wants: `rotary(k, positions)` gives
+        returned turned (rows of padding too, by the position as it stands). No two rows have the same place, k and v do not
+        lie in places that the call writes, and where the cache's keys and values are the same memory they are equal and unturned. The keys as they are stored are what a selector wants: `rotary(k, positions)` gives
         them."""
         _no_gradient(k, v, q)
         if _current_device() != self._index:  # kernels, streams and handles are the current device's
@@ -392,8 +392,6 @@ class PagedCache:
             heads = q.shape[1]
             if heads:
                 q_in, q_to = _packed(q), _packed(turned)
-        if self._at[0] == self._at[1]:
-            _fail("the keys and values of this cache are the same memory, where both cannot be stored")
         if n:
             L.check(L.lib().certexB200PagedAppend(L.resources(self._index), self._unmoved(), rotary._plan if rotary else None, table,
                                                   _packed(k), _packed(v), q_in, q_to, n, heads, positions.data_ptr(),

@@ -634,14 +634,14 @@ def test_copies_of_a_cache_have_their_own_memory():
 
 
 @gpu
-def test_keys_and_values_of_one_memory_are_read_but_not_stored():
+def test_keys_and_values_of_one_memory():
     both = torch.randn((3, 4, 1, 8), device="cuda")
     cache = certex.PagedCache(keys=both, values=both)
     table, n = torch.tensor([[2, 0]], device="cuda", dtype=torch.int32), torch.tensor([1], device="cuda", dtype=torch.int32)
     row = torch.ones((1, 1, 8), device="cuda")
     assert torch.equal(cache.attend(row, table, n), both[2, :1])  # one key: its value, weight 1
-    with pytest.raises(ValueError, match="same memory"):
-        cache.append(row, row, table, n)
+    cache.append(row, row, table, n)
+    assert torch.equal(both[2, 1], row[0]) and torch.equal(cache.attend(row, table, n), both[2, :1])
 
 
 @gpu
