@@ -369,8 +369,8 @@ class PagedCache:
         """Stores k, v (n, n_kv_heads, head_dim) at positions (n,) int32 or int64 of their sequences; a negative position is
         padding. With a rotation the keys are turned by their positions first, and q (n, heads, head_dim), if given, is
         returned turned (rows of padding too, by the position as it stands). No two rows have the same place, k and v do not
-        lie in places that the call writes, and where the cache's keys and values are the same memory they are equal and unturned. The keys as they are stored are what a selector wants: `rotary(k, positions)` gives
-        them."""
+        lie in places that the call writes, and where the cache's keys and values are the same memory k and v are equal and
+        unturned. The keys as they are stored are what a selector wants: `rotary(k, positions)` gives them."""
         _no_gradient(k, v, q)
         if _current_device() != self._index:  # kernels, streams and handles are the current device's
             with torch.cuda.device(self._index):
