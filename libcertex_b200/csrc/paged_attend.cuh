@@ -23,10 +23,10 @@
 //    its loads, and where it lies is worked out while the tile before it arrives: done between two tiles' products instead, a call
 //    over 131 072 keys took 105 us instead of 94, and float32 keys 240 instead of 192.
 //
-// 131 072 bfloat16 keys of 8 heads of 128: 92 us, 5.8 TB/s, of which about 11 us are the launches, the first tile's chain of
-// reads (length, page, row) and the joining; the rest runs at 6.4 TB/s, the rate of a copy. Rows of 256 bytes in a random order (selected
-// positions) come at 4.9 TB/s. Asking L2 for rows two tiles ahead made everything slower (a prefetch per row 108 and 160 us for
-// these two, one per line 98 and 208): the reads in flight are enough, and DRAM has its own order to keep.
+// 131 072 bfloat16 keys of 8 heads of 128: 91 us, 5.9 TB/s; 16 rows of 32 lists of 2048 positions 95 us, 5.1 TB/s. About 11 us of
+// either are the launches, the first tile's chain of reads (length, page, row), blocks that end unevenly and the joining; the rest runs
+// at 6 to 6.4 TB/s, near the rate of a copy. Asking L2 for rows two tiles ahead made everything slower (a prefetch per row 108 and 160 us
+// for these two, one per line 98 and 208): the reads in flight are enough, and DRAM has its own order to keep.
 //
 // Rows that are not to be seen have scores of -infinity and values of zero, so nothing that lies there (NaN, infinity,
 // another sequence's tokens) has an effect.

@@ -11,11 +11,12 @@
 // [-1/2, 1/2) turns. float32 outputs take sincospif of it; 16-bit outputs the hardware's sine and cosine, whose absolute
 // error of 2^-20.9 on [-pi, pi] lies far below half a step of their types (2^-12 relative and more).
 //
-// Both kernels move bytes: everything is read once and written once, and what bounds them is HBM (large calls) or the
-// launch (a decoding step). A thread owns one "unit" of a head: two vectors of 16 bytes that hold V whole pairs
+// One kernel for both. It moves bytes: everything is read once and written once, and what bounds it is HBM (32 768 rows of 32
+// bfloat16 heads of 128 in 84 us, 6.4 TB/s; 16 384 rows appended with 32 query heads and 8 KV heads in 66, 6.1 TB/s) or the launch
+// (a decoding step, 2 us). A thread owns one "unit" of a head: two vectors of 16 bytes that hold V whole pairs
 // (neighbouring vectors when interleaved, a vector of each half otherwise), so that a pair never crosses threads and the
 // call may be in place. It goes through up to eight heads with the same V sines and cosines: they depend on the row and the
-// pair alone.
+// pair alone; where that is one head, a thread takes a key and its value.
 #include "paged.cuh"
 
 #include <cuda_bf16.h>
