@@ -11,14 +11,17 @@ namespace {
 constexpr int64_t kMostShares = kJoinSums * kJoinThreads;
 /// Tokens that a block of a cluster goes through at most, as far as the host can tell from the width of the table. Without a split
 /// there is one launch and no second pass over partial results, but a block's time is that of the longest row. Rows of 8 KV heads: 1 of
-/// 1000 keys 8.8 us in clusters and 10.1 split, 4 of 2000 14.4 and 19.5; with 512 tokens a block 1 of 4000 16.2 and 12.7.
+/// 1000 keys 8.3 us in clusters and 9.0 split, 4 of 2000 13.7 and 17.9; with 512 tokens a block 1 of 4000 16.2 and 12.7. Half as many where
+/// the clusters leave three quarters of the GPU idle: 1 of 2000 10.9 and 9.4, float32 14.9 and 11.6.
 constexpr int64_t kClusterTokens = 256;
 
-/// Shares of a unit, on average, from which blocks have four warps. Below that smaller blocks wait less for one another: 128 rows of
-/// 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), one row of 131 072 keys of 8 heads 91.9 and 91.3, float32 keys of
-/// 16 rows 192 us with four and 175 with one. Above, there are too many results to join: one row and KV head of 131 072 keys took 30 us
-/// with two warps and 24 with four.
-constexpr int64_t kManyShares = 128;
+/// Shares of a unit, on average, from which blocks have four warps, for 16-bit types and float32. Below that smaller blocks wait less for
+/// one another: 128 rows of 100 to 1000 keys took 49 us with four warps and 45 with two (one: 46), one row of 131 072 keys of 8 heads 91.9
+/// and 91.3, float32 keys of 16 rows 192 us with four and 175 with one, of one row and 4 KV heads 100 and 90 (131 072) or 39 and 36
+/// (40 000). Above, there are too many results to join: one row and KV head of 131 072 keys took 30 us with two warps and 24 with four,
+/// two heads of 16 000 float32 keys 18 with one and 15 with four. The same goes for float32 keys with less than 32 tokens to a small
+/// block: one row of 2000 keys of 8 heads 12.2 with one and 11.5 with four.
+constexpr int64_t kManyShares = 128, kManySharesF32 = 320;
 
 /// Tokens that the table can hold of a sequence, as far as a row may see them.
 int64_t table_tokens(const AttendArgs& a)
@@ -52,9 +55,10 @@ Plan plan_of(const AttendArgs& a, int sm_count)
   // as many blocks of four warps per unit as fill the GPU, with 64 tokens each at least
   n.cluster = 1;
   while (n.cluster < 8 && units * n.cluster * 8 <= warps && n.cluster * 64 < most) { n.cluster *= 2; }
-  if (most > kClusterTokens * n.cluster) { n.cluster = 0; }
+  if (most > (units * n.cluster * 16 <= warps ? kClusterTokens / 2 : kClusterTokens) * n.cluster) { n.cluster = 0; }
   const int few          = half ? 2 : 1;  // warps of a small block
-  const bool small       = n.cluster ? units * n.cluster * 4 > warps : warps / few <= kManyShares * units;
+  const bool joinable    = half ? warps / few <= kManyShares * units : warps <= kManySharesF32 * units && units * most >= 32 * warps;
+  const bool small       = n.cluster ? units * n.cluster * 4 > warps : joinable;
   n.warps                = small ? few : 4;
   const int64_t resident = warps / n.warps;
   // units side by side, where that leaves few blocks without work; lists of positions have no common tokens
