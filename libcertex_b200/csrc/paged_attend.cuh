@@ -488,10 +488,11 @@ __device__ __forceinline__ void put_sums(const AttendParams& p, const Segment& g
 // queries the 8-column side, so that 8 queries fill it: S^T = K Q^T, then O^T = V^T P^T. The two products of a tile of
 // 16 keys by d = 128 are 8 + 16 instructions for 8 KB read.
 //
-// Weights enter the second product as two 16-bit numbers, the upper part cut off and the rest (p = hi + lo to 2^-16), because a
-// weight rounded once to bfloat16 would add as much error as the rounding of the result. lo is kept positive: zero times an
-// infinite value would be NaN. Weights of float16 are multiplied by 2^12, since float16 has nothing below 2^-24; l carries
-// the factor too, so it cancels.
+// Weights enter the second product as two 16-bit numbers, the upper part cut off and the rest, because a weight rounded once to
+// bfloat16 would add as much error as the rounding of the result. p = hi + lo to 2^-16 of p in bfloat16, in float16 to 2^-20 of p
+// and 2^-41 of the row's largest weight so far: float16 has nothing below 2^-24, so its weights are multiplied by 2^16 (l carries
+// the factor too, so it cancels). What is cut off is a little less than p, so that neither part of a weight is zero and an infinite
+// value stays one (zero times infinity is NaN); a weight of zero is two zeros and adds nothing.
 constexpr int kKeys   = 16;  // of a tile
 constexpr int kStages = 3;
 
@@ -516,6 +517,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
   return r;
 }
 
+/// A little less than x, by 2^-20 of it and `least`, a step or two of what is subnormal in the type; 0 for 0 (and for NaN, which the
+/// lower part keeps).
+__device__ __forceinline__ float below(float x, float least) { return fmaxf(fmaf(x, 1.f - 0x1p-20f, -least), 0.f); }
+
 template <typename T>
 struct Half;
 template <>
@@ -530,15 +535,15 @@ struct Half<__nv_bfloat16> {
   /// (x, y) as two pairs of numbers whose sum they are; x in the lower halves.
   static __device__ void split(float x, float y, uint32_t& hi, uint32_t& lo)
   {
-    const uint32_t a = __float_as_uint(x) & 0xffff0000u, b = __float_as_uint(y) & 0xffff0000u;
+    const uint32_t a = __float_as_uint(below(x, 0x1p-132f)) & 0xffff0000u, b = __float_as_uint(below(y, 0x1p-132f)) & 0xffff0000u;
     hi = (a >> 16) | b;
-    const __nv_bfloat162 r = __floats2bfloat162_rn(fmaxf(x - __uint_as_float(a), 1.2e-38f), fmaxf(y - __uint_as_float(b), 1.2e-38f));
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(a), y - __uint_as_float(b));
     lo = *reinterpret_cast<const uint32_t*>(&r);
   }
 };
 template <>
 struct Half<__half> {
-  static constexpr float kRaise = 12.f;
+  static constexpr float kRaise = 16.f;  // (the largest weight is cut to 65 504, the largest number)
   static __device__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
   {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -547,9 +552,9 @@ struct Half<__half> {
   }
   static __device__ void split(float x, float y, uint32_t& hi, uint32_t& lo)
   {
-    const __half2 h = __halves2half2(__float2half_rz(x), __float2half_rz(y));
+    const __half2 h = __halves2half2(__float2half_rz(below(x, 0x1p-24f)), __float2half_rz(below(y, 0x1p-24f)));
     hi              = *reinterpret_cast<const uint32_t*>(&h);
-    const __half2 r = __floats2half2_rn(fmaxf(x - __low2float(h), 6e-8f), fmaxf(y - __high2float(h), 6e-8f));
+    const __half2 r = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
     lo              = *reinterpret_cast<const uint32_t*>(&r);
   }
 };

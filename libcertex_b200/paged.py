@@ -439,9 +439,10 @@ class PagedCache:
         """Softmax attention of every row of q (n, heads, head_dim) over the first lengths[i] tokens of its sequence (n,)
         int32, or over the last `window` of those; heads is a multiple of n_kv_heads, query head h reads KV head
         h // (heads / n_kv_heads). scale defaults to head_dim ** -0.5. Returns (n, heads, head_dim), and with return_lse the
-        float32 logarithm of the sum of exponentials (n, heads). A row that sees nothing gets zeros and -inf. Several rows of
-        one sequence (drafted tokens) name it in row_to_batch and have their own lengths. out, if given, is written: memory that
-        no other argument and no page has."""
+        float32 logarithm of the sum of exponentials (n, heads). A row that sees nothing gets zeros and -inf, one whose keys
+        all have scores of minus infinity NaN and -inf, as a softmax of them has. Several rows of one sequence (drafted tokens)
+        name it in row_to_batch and have their own lengths. out, if given, is written: memory that no other argument and no page
+        has."""
         if _current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.attend(q, page_table, lengths, row_to_batch, scale, window, return_lse, out)
