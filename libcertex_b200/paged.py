@@ -160,8 +160,9 @@ class _Turn(torch.autograd.Function):
 class Rotary:
     """Turns queries and keys by their positions: pair i of the first `rotary_dim` coordinates of a head (default: all) by
     the angle position * w_i, w_i = base ** (-2 i / rotary_dim). Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with
-    interleaved=True. Angles are reduced to one turn exactly and off by at most 2**-26 of it at every position up to 2**31, so no
-    table of sines limits the length.
+    interleaved=True. Angles are reduced exactly at every position, so no table of sines limits the length. Sines and cosines
+    are off by 2**-21.4 of themselves at most for float32, by 2**-20 for 16-bit types, and by 2**-65 of a turn a position for the
+    frequency's rounding.
 
     scaling stretches the frequencies for sequences longer than the `original_length` a model was trained on, by `factor`:
       "linear"      w_i / factor
