@@ -332,7 +332,7 @@ CERTEX_B200_EXPORT cuvsError_t certexB200ToHalf(cuvsResources_t res, const void*
  *
  * Indices are read on the device and checked there: a row of a sequence that the table does not have, an entry of the table
  * that is no page, a position or a length beyond the table reads and writes nothing (attention goes on without that key) and
- * sets *fault to 1, where the caller may look.
+ * sets *fault to 1, where the caller may look; certexB200PagedTakeFault looks and clears it at once.
  */
 /** [rows, heads, dim] */
 typedef struct {
@@ -393,6 +393,10 @@ CERTEX_B200_EXPORT cuvsError_t certexB200PagedAppend(cuvsResources_t res, const 
                                                      const certexB200Rows_t* k, const certexB200Rows_t* v,
                                                      const certexB200Rows_t* q, const certexB200Rows_t* q_out, int64_t n_rows,
                                                      int64_t n_q_heads, const void* positions, int32_t positions_64);
+
+/** *was = *fault; *fault = 0, in one step on the device, so that what a call on another stream reports meanwhile is in this answer or
+ *  in the next. was: one int32 of device memory. */
+CERTEX_B200_EXPORT cuvsError_t certexB200PagedTakeFault(cuvsResources_t res, const certexB200PagedCache_t* cache, int32_t* was);
 
 /** Bytes of device memory that an attention of these sizes wants as its workspace (16-byte aligned; it belongs to one call at
  *  a time). n_lists: 0 for certexB200PagedAttend, with k = its pages_per_sequence * page_size; else k is the length of a list

@@ -118,7 +118,7 @@ SYMBOLS = [
     "certexB200DistributedSearchBegin", "certexB200DistributedSearchEnd", "certexB200OrderByLabel",
     "certexB200PackMask", "certexB200ToHalf", "certexB200LabelSample",
     "certexB200Rotate", "certexB200PagedAppend", "certexB200PagedWorkspace", "certexB200PagedAttend",
-    "certexB200PagedAttendSelected",
+    "certexB200PagedAttendSelected", "certexB200PagedTakeFault",
 ]
 
 # void hook(void* ctx, int32_t* keys, int64_t n, cudaStream_t stream)
@@ -206,6 +206,7 @@ def lib():
                 i32, f32, sz = ctypes.c_int32, ctypes.c_float, ctypes.c_size_t
                 L.certexB200Rotate.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, vp, i32, i32]
                 L.certexB200PagedAppend.argtypes = [vp] * 8 + [i64, i64, vp, i32]
+                L.certexB200PagedTakeFault.argtypes = [vp, vp, vp]
                 L.certexB200PagedWorkspace.argtypes = [vp, vp, i64, i64, i64, i64, i64, P(sz)]
                 L.certexB200PagedAttend.argtypes = [vp, vp, vp, vp, i64, vp, vp, i64, i64, f32, vp, vp, sz]
                 L.certexB200PagedAttendSelected.argtypes = [vp, vp, vp, i32, i64, i64, vp, vp, i64, i64, f32, vp, vp, sz]

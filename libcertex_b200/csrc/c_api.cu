@@ -716,6 +716,16 @@ cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCach
   });
 }
 
+cuvsError_t certexB200PagedTakeFault(cuvsResources_t res, const certexB200PagedCache_t* cache, int32_t* was)
+{
+  return translate([=] {
+    const certexB200PagedCache_t& c = checked_cache(cache);
+    CERTEX_EXPECTS(was != nullptr, "certex: null answer");
+    launch_take_fault(c.fault, was, current_res(res).stream);
+    CERTEX_CUDA(cudaGetLastError());
+  });
+}
+
 cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, const certexB200PagedCache_t* cache, int64_t n_rows, int64_t n_heads,
                                      int64_t n_lists, int64_t k, int64_t window, size_t* bytes)
 {

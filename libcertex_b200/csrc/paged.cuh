@@ -29,6 +29,9 @@ void launch_paged_append(const certexB200PagedCache_t& cache, const certexB200Ro
                          const certexB200Rows_t& q_out, int64_t n_rows, int64_t n_q_heads, const void* positions,
                          bool positions_64, cudaStream_t s);
 
+/// *was = *fault, and *fault = 0.
+void launch_take_fault(int32_t* fault, int32_t* was, cudaStream_t s);
+
 /// One call of either attention. `lengths` (with `table`) or `selected` (lists of k physical positions) is given.
 struct AttendArgs {
   certexB200PagedCache_t cache;

@@ -7,6 +7,8 @@
 namespace certex_b200 {
 namespace {
 
+__global__ void take_fault_kernel(int32_t* fault, int32_t* was) { *was = atomicExch(fault, 0); }
+
 /// Shares at most: what the joining kernel's threads read the sums of.
 constexpr int64_t kMostShares = kJoinSums * kJoinThreads;
 /// Tokens that a block of a cluster goes through at most, as far as the host can tell from the width of the table. Without a split
@@ -107,6 +109,8 @@ bool paged_within_reach(const certexB200PagedCache_t& c)
   }
   return true;
 }
+
+void launch_take_fault(int32_t* fault, int32_t* was, cudaStream_t s) { take_fault_kernel<<<1, 1, 0, s>>>(fault, was); }
 
 size_t paged_attend_workspace(const AttendArgs& a, int sm_count) { return plan_of(a, sm_count).bytes; }
 

@@ -335,11 +335,14 @@ class PagedCache:
 
     def faulted(self):
         """Whether an index of a call since the last time was out of range (and was left out). Waits for the current stream, and
-        speaks for calls that were enqueued there, or that it waited for."""
-        bad = bool(self._fault.item())
-        if bad:
-            self._fault.zero_()
-        return bad
+        speaks for calls that were enqueued there, or that it waited for; what a call on another stream finds meanwhile is in this
+        answer or in the next."""
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.faulted()
+        was = torch.empty_like(self._fault)
+        L.check(L.lib().certexB200PagedTakeFault(L.resources(self._index), self._args, was.data_ptr()))
+        return bool(was.item())
 
     def _unmoved(self):
         """The cache as the library takes it, whose memory must still be where it was."""
