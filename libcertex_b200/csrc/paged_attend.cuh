@@ -154,11 +154,14 @@ struct Span {
   int32_t sequence;
 };
 
+/// EARLY: read from L2, before this kernel has waited for the one in front.
+template <bool EARLY = false>
 __device__ __forceinline__ Span span_of(const AttendParams& p, int32_t row)
 {
   if (p.lengths == nullptr) { return {0, p.k, 0}; }
-  int32_t end            = p.lengths[row];
-  const int32_t sequence = p.row_to_sequence ? p.row_to_sequence[row] : row;
+  auto read              = [&](const int32_t* at) { return EARLY ? __ldcg(at + row) : at[row]; };
+  int32_t end            = read(p.lengths);
+  const int32_t sequence = p.row_to_sequence ? read(p.row_to_sequence) : row;
   if (end <= 0) { return {0, 0, 0}; }
   const bool stranger = sequence < 0 || sequence >= p.n_sequences;
   if (stranger || end > p.most) { *p.fault = 1; }
@@ -352,7 +355,7 @@ __device__ __forceinline__ Start start_of(const AttendParams& p, int32_t share)
 }
 
 /// The blocks are there before the kernel in front of them has ended (2 us less between calls in a stream) and wait for that; the
-/// joining kernel, if there is one, is let in the same way.
+/// joining kernel, if there is one, is let in the same way, but never before the wait: it reads what that kernel wrote (joint_of).
 __device__ __forceinline__ void begin(const AttendParams& p)
 {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1468,8 +1471,10 @@ __device__ __forceinline__ Joint joint_of(const AttendParams& p, int32_t x)
     id                 = p.by_unit ? x : mark;
     j.first            = p.by_unit ? mark : divide(x, p.abreast);
   } else {
-    // one length, so every unit has the same steps
-    const int32_t steps = x < p.joints ? steps_for(p, span_of(p, 0).count) : 0;
+    // One length, so every unit has the same steps. It is read ahead of the wait: every block of the first kernel has waited for all that
+    // wrote it before it let this kernel in (begin() keeps that order, and this depends on it), so L2 has it; L1, which may keep what
+    // an earlier kernel read, is passed by.
+    const int32_t steps = x < p.joints ? steps_for(p, span_of<true>(p, 0).count) : 0;
     if (steps > 0) {
       const Split split(steps * p.n_rows * p.in_line, p.shares);
       const int32_t share = divide(x, p.abreast);
