@@ -684,7 +684,8 @@ cuvsError_t certexB200Rotate(cuvsResources_t res, const certexB200Rotary_t* rota
     check_rows(x, "rows");
     check_rows(y, "output");
     CERTEX_EXPECTS(positions != nullptr, "certex: null positions");
-    launch_rotate(plan, *x, *y, n_rows, n_heads, head_dim, dtype, positions, positions_64 != 0, inverse != 0, current_res(res).stream);
+    const Resources& r = current_res(res);
+    launch_rotate(plan, *x, *y, n_rows, n_heads, head_dim, dtype, positions, positions_64 != 0, inverse != 0, r.sm_count, r.stream);
     CERTEX_CUDA(cudaGetLastError());
   });
 }
@@ -710,8 +711,9 @@ cuvsError_t certexB200PagedAppend(cuvsResources_t res, const certexB200PagedCach
     }
     CERTEX_EXPECTS(positions != nullptr, "certex: null positions");
     const certexB200Rows_t none{};
+    const Resources& r = current_res(res);
     launch_paged_append(c, rotary, *table, *k, *v, n_q_heads > 0 ? *q : none, n_q_heads > 0 ? *q_out : none, n_rows, n_q_heads,
-                        positions, positions_64 != 0, current_res(res).stream);
+                        positions, positions_64 != 0, r.sm_count, r.stream);
     CERTEX_CUDA(cudaGetLastError());
   });
 }

@@ -21,13 +21,13 @@ constexpr int64_t kMostTokens = (int64_t(1) << 31) - 64;  // that a row may see:
 /// y = x turned by `positions` (or back, `inverse`): rows x heads x dim, the first rotary_dim coordinates.
 void launch_rotate(const certexB200Rotary_t& plan, const certexB200Rows_t& x, const certexB200Rows_t& y, int64_t n_rows,
                    int64_t n_heads, int64_t head_dim, int dtype, const void* positions, bool positions_64, bool inverse,
-                   cudaStream_t s);
+                   int sm_count, cudaStream_t s);
 
 /// Keys (turned when `plan` is given) and values to their pages; queries turned into q_out when n_q_heads > 0.
 void launch_paged_append(const certexB200PagedCache_t& cache, const certexB200Rotary_t* plan, const certexB200PageTable_t& table,
                          const certexB200Rows_t& k, const certexB200Rows_t& v, const certexB200Rows_t& q,
                          const certexB200Rows_t& q_out, int64_t n_rows, int64_t n_q_heads, const void* positions,
-                         bool positions_64, cudaStream_t s);
+                         bool positions_64, int sm_count, cudaStream_t s);
 
 /// *was = *fault, and *fault = 0.
 void launch_take_fault(int32_t* fault, int32_t* was, cudaStream_t s);

@@ -112,17 +112,14 @@ template <typename T>
 struct Type;
 template <>
 struct Type<float> {
-  static __device__ float up(float v) { return v; }
   static __device__ float down(float v) { return v; }
 };
 template <>
 struct Type<__half> {
-  static __device__ float up(__half v) { return __half2float(v); }
   static __device__ __half down(float v) { return __float2half_rn(v); }
 };
 template <>
 struct Type<__nv_bfloat16> {
-  static __device__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
@@ -996,7 +993,6 @@ struct HalfTile {
   static constexpr int kPitch = D * 2 + 16;  // bytes of a row in shared memory: eight rows start in eight different banks
   static constexpr int kBytes = kKeys * kPitch;
   static constexpr int kWarp  = kStages * 2 * kBytes;
-  static constexpr int kLanes = 32;           // lanes that copy a row
 };
 
 template <typename T, int D, int NT, int W>
@@ -1063,18 +1059,15 @@ __global__ void __launch_bounds__(W * 32, 4 / W) attend_ring_kernel(const Attend
     uint32_t masks = 0;  // of the tiles in the ring: which keys are real, newest lowest
     uint32_t older = 0;
     auto copy = [&](int stage, const Place& at) {
-      constexpr int kRows = 32 / Tile::kLanes;  // rows that the warp copies at once
-      const int chunk = lane % Tile::kLanes, sub = lane / Tile::kLanes;
-      const uint32_t to = ring_at + stage * 2 * Tile::kBytes + chunk * 16;
-      const bool inside = chunk * 8 < p.dim;
+      const uint32_t to = ring_at + stage * 2 * Tile::kBytes + lane * 16;
+      const bool inside = lane * 8 < p.dim;
 #pragma unroll
-      for (int r = 0; r < kKeys; r += kRows) {
-        const int row     = r + sub;
+      for (int row = 0; row < kKeys; ++row) {
         const uint32_t ka = __shfl_sync(~0u, at.k, row), va = __shfl_sync(~0u, at.v, row);
         const bool ok     = ka != kNowhere;
         if (inside) {
-          copy16(to + row * Tile::kPitch, keys + (ok ? static_cast<uint64_t>(ka) << p.unit_shift : 0) + chunk * 16, ok);
-          copy16(to + Tile::kBytes + row * Tile::kPitch, values + (ok ? static_cast<uint64_t>(va) << p.unit_shift : 0) + chunk * 16, ok);
+          copy16(to + row * Tile::kPitch, keys + (ok ? static_cast<uint64_t>(ka) << p.unit_shift : 0) + lane * 16, ok);
+          copy16(to + Tile::kBytes + row * Tile::kPitch, values + (ok ? static_cast<uint64_t>(va) << p.unit_shift : 0) + lane * 16, ok);
         }
       }
       older = masks >> 16;

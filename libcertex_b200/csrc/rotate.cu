@@ -10,7 +10,7 @@
 // position * 2^-65 turns from the rounding of w_i. For float32 outputs the nearest quarter of a turn comes off in whole numbers as well:
 // what is rounded to float32 is an eighth of a turn at most, and Taylor's series to the ninth and tenth power (what they leave out is
 // 1.8e-9 and 1.1e-9 there) gives sines and cosines to a few units of their own last place, small ones too. (With half a turn
-// rounded to float32 they were off by up to 1.1e-7 of a turn's radius, now by 5e-8; 200 000 rows of one head of 256 take 92 us instead of 95.)
+// rounded to float32 they were off by up to 1.1e-7, now by 5e-8; 200 000 rows of one head of 256 take 92 us instead of 95.)
 // 16-bit outputs take the upper 32 bits as an angle in [-1/2, 1/2) turns and the hardware's sine and cosine of it, whose absolute error of
 // 2^-20.9 on [-pi, pi] lies far below half a step of their types (2^-12 of the larger coordinate of a pair and more): the series instead costs
 // a row of one head 30 % (100 000 rows of 128: 17.6 us for 13.3).
@@ -279,14 +279,14 @@ void run(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
 }
 
 template <typename T, int V>
-void run(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
+void run(TurnArgs<T>& a, bool interleaved, int sm_count, cudaStream_t s)
 {
   int64_t heads = 0;
   for (int i = 0; i < a.n_sec; ++i) { heads += a.sec[i].heads; }
   // As many heads of a thread share its sines and cosines, and the row's page, as leave two blocks on every SM, and as the
   // sections come out even with: turning 4099 rows of 32 float32 heads takes 34 us with one head a thread and 21 with eight,
   // 16 384 rows of 12 bfloat16 heads 18 us with eight and 15 with four.
-  const int64_t items = a.n_rows * heads * (a.dim / (2 * V)), wave = int64_t(148) * 2 * 256;
+  const int64_t items = a.n_rows * heads * (a.dim / (2 * V)), wave = int64_t(sm_count) * 2 * 256;
   auto fits           = [&](int n) {
     bool even = items >= n * wave;
     for (int i = 0; i < a.n_sec; ++i) { even = even && (a.sec[i].heads + n - 1) / n * n * 4 <= a.sec[i].heads * 5; }
@@ -316,12 +316,12 @@ bool aligned(const Section<T>& s)
 }
 
 template <typename T>
-void turn(TurnArgs<T>& a, bool interleaved, cudaStream_t s)
+void turn(TurnArgs<T>& a, bool interleaved, int sm_count, cudaStream_t s)
 {
   constexpr int V = 16 / sizeof(T);
   bool wide       = a.dim % (2 * V) == 0 && a.rotary_dim % (2 * V) == 0;
   for (int i = 0; i < a.n_sec; ++i) { wide = wide && aligned(a.sec[i]); }
-  wide ? run<T, V>(a, interleaved, s) : run<T, 1>(a, interleaved, s);
+  wide ? run<T, V>(a, interleaved, sm_count, s) : run<T, 1>(a, interleaved, sm_count, s);
 }
 
 template <typename T>
@@ -362,21 +362,21 @@ void by_type(int dtype, F&& f)
 
 void launch_rotate(const certexB200Rotary_t& plan, const certexB200Rows_t& x, const certexB200Rows_t& y, int64_t n_rows,
                    int64_t n_heads, int64_t head_dim, int dtype, const void* positions, bool positions_64, bool inverse,
-                   cudaStream_t s)
+                   int sm_count, cudaStream_t s)
 {
   by_type(dtype, [&](auto t) {
     using T         = decltype(t);
     TurnArgs<T> a   = turn_args<T>(&plan, head_dim, positions, positions_64, n_rows);
     a.inverse       = inverse;
     a.sec[a.n_sec++] = section<T>(x, y, n_heads, true);
-    turn(a, plan.interleaved != 0, s);
+    turn(a, plan.interleaved != 0, sm_count, s);
   });
 }
 
 void launch_paged_append(const certexB200PagedCache_t& cache, const certexB200Rotary_t* plan, const certexB200PageTable_t& table,
                          const certexB200Rows_t& k, const certexB200Rows_t& v, const certexB200Rows_t& q,
                          const certexB200Rows_t& q_out, int64_t n_rows, int64_t n_q_heads, const void* positions,
-                         bool positions_64, cudaStream_t s)
+                         bool positions_64, int sm_count, cudaStream_t s)
 {
   by_type(static_cast<int>(cache.dtype), [&](auto t) {
     using T       = decltype(t);
@@ -394,7 +394,7 @@ void launch_paged_append(const certexB200PagedCache_t& cache, const certexB200Ro
     };
     a.sec[a.n_sec++] = pages(k, cache.keys, cache.key_strides, plan != nullptr);
     a.sec[a.n_sec++] = pages(v, cache.values, cache.value_strides, false);
-    turn(a, plan && plan->interleaved != 0, s);
+    turn(a, plan && plan->interleaved != 0, sm_count, s);
   });
 }
 
