@@ -208,9 +208,10 @@ class Rotary:
 
     def __call__(self, x, positions, inverse=False, out=None):
         """x (n, heads, head_dim) float32, float16 or bfloat16, its rows turned by positions (n,) int32 or int64, which may be
-        negative; inverse=True turns back. Differentiable in x (as for every function of torch, a backward pass that is captured
-        in a CUDA graph wants leaves of which no eager graph is alive). out: where to write, x itself allowed; without a
-        gradient."""
+        negative. inverse=True is the transpose: it turns back, and multiplies by magnitude too, so that both in a row leave
+        magnitude ** 2 times x. Differentiable in x, backward and by torch.autograd.forward_ad; the transforms of torch.func are
+        refused (as for every function of torch, a backward pass that is captured in a CUDA graph wants leaves of which no eager
+        graph is alive). out: where to write, x itself allowed; without a gradient."""
         x = _check_rows(x, "x", self._index, None, None, self.head_dim)
         positions = _check_index(positions, "positions", x.shape[:1], self._index, True)
         if x.requires_grad and torch.is_grad_enabled() or _has_tangent(x):

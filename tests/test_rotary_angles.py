@@ -29,6 +29,32 @@ def test_the_oracle_agrees_with_64_bits():
 
 
 @pytest.mark.gpu
+def test_the_inverse_is_the_transpose():
+    """It undoes the rotation up to the square of the magnitude: a value is a sum of two products at most, twice, each off by 2^-21.4 and the
+    roundings of products and sum, 2^-23 together, of the sizes of what it is made of, 4 times the largest of the row."""
+    x, y = torch.randn((2, 40, 3, 64), device="cuda")
+    p = torch.arange(40, device="cuda") * 977
+    for plan in (certex.Rotary(64), certex.Rotary(64, 32, scaling="yarn", factor=16.0), certex.Rotary(64, magnitude=0.5, interleaved=True)):
+        back = plan(plan(x, p), p, inverse=True)
+        r, m = plan.rotary_dim, plan.magnitude
+        off = 2 * 4 * m * m * (2.0**-21.4 + 2.0**-23) * float(x.abs().max())
+        assert float((back[..., :r].double() - m * m * x[..., :r].double()).abs().max()) <= off and torch.equal(back[..., r:], x[..., r:])
+        # <R x, y> = <x, R' y>
+        left, right = (plan(x, p).double() * y.double()).sum(), (x.double() * plan(y, p, inverse=True).double()).sum()
+        assert abs(float(left - right)) <= 2 * 2 * m * (2.0**-21.4 + 2.0**-23) * x.numel() * float(x.abs().max() * y.abs().max())
+
+
+@pytest.mark.gpu
+def test_transforms_of_functions_are_refused():
+    """torch.func's transforms wrap their tensors: the kernels cannot read those, and say so."""
+    plan, x, p = certex.Rotary(16), torch.randn((5, 2, 16), device="cuda"), torch.arange(5, device="cuda")
+    for call in (lambda: torch.func.grad(lambda z: plan(z, p).sum())(x), lambda: torch.func.jvp(lambda z: plan(z, p), (x,), (x,)),
+                 lambda: torch.func.vmap(lambda z: plan(z, p))(x[None]), lambda: torch.func.vmap(lambda z: plan(x, z))(p[None])):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dim", [256, 250])
 def test_sines_to_a_part_of_themselves(dim, interleaved):
