@@ -343,7 +343,7 @@ typedef struct {
 
 /** The rotation of pairs of a head's first rotary_dim coordinates, (2i, 2i + 1) when interleaved, else (i, i + rotary_dim / 2):
  *  turns[i] (device memory, rotary_dim / 2 of them) is what a position adds to pair i's angle, as a fraction of a turn in
- *  units of 2^-64 (a negative angle wraps); results are multiplied by magnitude. */
+ *  units of 2^-64 (a negative angle wraps); results are multiplied by magnitude (by the inverse's too: it is the transpose). */
 typedef struct {
   const uint64_t* turns;
   int64_t rotary_dim;
@@ -406,7 +406,8 @@ CERTEX_B200_EXPORT cuvsError_t certexB200PagedWorkspace(cuvsResources_t res, con
 
 /** out[i, h] = the values that row i sees, weighed by the softmax of scale * <q[i, h], key> over KV head h / (n_heads /
  *  n_kv_heads). Row i sees the first lengths[i] tokens of its sequence, of those the last `window` if window > 0; a row that
- *  sees none gets zeros. lse (may be NULL) [n_rows, n_heads]: the logarithm of the sum of exponentials (-inf for such a row).
+ *  sees none gets zeros. lse (may be NULL) [n_rows, n_heads]: the logarithm of the sum of exponentials (-inf for such a row, and for
+ *  one whose keys all have scores of minus infinity, whose answer is NaN).
  *  n_rows * n_heads is below 2^27; a row sees 2^31 - 64 tokens at most. */
 CERTEX_B200_EXPORT cuvsError_t certexB200PagedAttend(cuvsResources_t res, const certexB200PagedCache_t* cache,
                                                      const certexB200PageTable_t* table, const int32_t* lengths, int64_t window,
