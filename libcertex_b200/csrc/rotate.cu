@@ -9,7 +9,7 @@
 // position * w_i is the wrapping 64-bit product: the reduction to one turn is exact at every position, with an error of
 // position * 2^-65 turns from the rounding of w_i. For float32 outputs the nearest quarter of a turn comes off in whole numbers as well:
 // what is rounded to float32 is an eighth of a turn at most, and Taylor's series to the ninth and tenth power (what they leave out is
-// 1.8e-9 and 1.1e-9 there) gives sines and cosines to a few units of their own last place, small ones too. (With half a turn
+// 1.8e-9 and 1.2e-10 there) gives sines and cosines to a few units of their own last place, small ones too. (With half a turn
 // rounded to float32 they were off by up to 1.1e-7, now by 5e-8; 200 000 rows of one head of 256 take 92 us instead of 95.)
 // 16-bit outputs take the upper 32 bits as an angle in [-1/2, 1/2) turns and the hardware's sine and cosine of it, whose absolute error of
 // 2^-20.9 on [-pi, pi] lies far below half a step of their types (2^-12 of the larger coordinate of a pair and more): the series instead costs
